@@ -12,6 +12,10 @@ mirror of that API over the C ABI, used by the tests and the benchmark:
 from ._lib import AcroError, build, lib, LIB_PATH
 from .host import (IndexMapping, PeerGroup, SharedEntryExchange, SlabTensor, SliceTensor, Tensor, TensorEngine, batch_slab, describe_kernel,
                    describe_plan, device_count, isCudaReady, set_stream)
+from .sequence import (layer_norm, layer_norm_backward, layer_norm_backward_scratch_bytes, linear_attention, linear_attention_backward,
+                       linear_attention_backward_scratch_bytes, linear_attention_scratch_bytes, linear_attention_step)
 
-__all__ = ["AcroError", "IndexMapping", "PeerGroup", "SharedEntryExchange", "SlabTensor", "SliceTensor", "Tensor", "TensorEngine", "batch_slab", "build", "describe_kernel", "describe_plan",
+__all__ = ["layer_norm", "layer_norm_backward", "layer_norm_backward_scratch_bytes", "linear_attention", "linear_attention_backward",
+           "linear_attention_backward_scratch_bytes", "linear_attention_scratch_bytes", "linear_attention_step",
+           "AcroError", "IndexMapping", "PeerGroup", "SharedEntryExchange", "SlabTensor", "SliceTensor", "Tensor", "TensorEngine", "batch_slab", "build", "describe_kernel", "describe_plan",
            "device_count", "isCudaReady", "lib", "set_stream", "LIB_PATH"]

@@ -37,6 +37,16 @@ def build(verbose=False, jobs=8):
         raise RuntimeError("building libacrotensor.so failed")
 
 
+class TokenArray(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("sequence_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class LinearAttentionDesc(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("dk", ctypes.c_int32),
+                ("dv", ctypes.c_int32), ("reserved", ctypes.c_int32), ("sequences", ctypes.c_int64), ("tokens", ctypes.c_int64),
+                ("scale", ctypes.c_double)]
+
+
 class GenericDesc(ctypes.Structure):
     _fields_ = [("n_loops", ctypes.c_int32), ("n_outer", ctypes.c_int32), ("n_inputs", ctypes.c_int32),
                 ("op", ctypes.c_int32), ("extent", ctypes.c_int64 * MAX_LOOPS),
@@ -57,6 +67,9 @@ _I64 = ctypes.c_int64
 _D = ctypes.c_double
 _SZ = ctypes.c_size_t
 _S = ctypes.c_char_p
+
+_DESC = ctypes.POINTER(LinearAttentionDesc)
+_ROWS = ctypes.POINTER(TokenArray)
 
 # name -> (restype, argtypes); every symbol include/acro_b200.h declares.
 SIGNATURES = {
@@ -163,6 +176,20 @@ SIGNATURES = {
     "acro_engine_end_multi_describe": (_I, [_P, _P, _SZ]),
     "acro_engine_clear": (_I, [_P]),
     "acro_engine_set_stream": (_I, [_P, _P]),
+    "acro_b200_linear_attention_scratch_bytes": (_SZ, [_DESC, _I]),
+    "acro_b200_linear_attention": (_I, [_DESC, _ROWS, _ROWS, _ROWS, _ROWS, _P, _P, _P, _P, _P, _I64, _P, _SZ, _P]),
+    "acro_b200_linear_attention_step": (_I, [_DESC, _ROWS, _ROWS, _ROWS, _ROWS, _P, _P, _P, _P, _I64, _P]),
+    "acro_b200_linear_attention_backward_scratch_bytes": (_SZ, [_DESC, _I]),
+    "acro_b200_linear_attention_backward": (_I, [_DESC, _ROWS, _ROWS, _ROWS, _ROWS, _P, _P, _P, _P, _ROWS, _ROWS, _ROWS, _P, _P, _SZ, _P]),
+    "acro_b200_layer_norm": (_I, [_I, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _I64, _D, _P]),
+    "acro_b200_layer_norm_backward_scratch_bytes": (_SZ, [_I, _I64, _I64]),
+    "acro_b200_layer_norm_backward": (_I, [_I, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _SZ, _P]),
+    "acro_engine_linear_attention": (_I, [_P, _P, _P, _P, _P, _P, _D, _P, _P]),
+    "acro_engine_linear_attention_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _D]),
+    "acro_engine_linear_attention_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _D, _P, _P, _P]),
+    "acro_engine_layer_norm": (_I, [_P, _P, _P, _P, _P, _D, _P, _P]),
+    "acro_engine_layer_norm_backward": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "acro_b200_get_stream": (_P, []),
     "acro_b200_set_stream": (_I, [_P]),
     "acro_b200_describe_kernel": (_I, [_S, _P, _SZ]),
     "acro_b200_describe_plan": (_I, [_I, ctypes.POINTER(_S), ctypes.POINTER(_I), _I, _P, _SZ]),

@@ -55,6 +55,14 @@ int guarded(F &&body)
     }
 }
 
+void require_handles(const char *name, std::initializer_list<const void *> handles)
+{
+    for (const void *h : handles)
+        if (h == nullptr) acro::throw_error(std::string(name) + ": null handle");
+}
+
+acro::Tensor *optional_tensor(acro_tensor *t) { return t != nullptr ? t->t.get() : nullptr; }
+
 int copy_out(const std::string &text, char *buf, size_t buf_len)
 {
     if (buf == nullptr || buf_len == 0) return ACRO_B200_OK;
@@ -394,6 +402,55 @@ int acro_engine_flat_indexed_sum_gather_shared(acro_engine *e, acro_tensor *Aout
         e->te.FlatIndexedSumGather(*Aout->t, *Ain->t, m->m, halo);
     });
 }
+
+int acro_engine_linear_attention(acro_engine *e, acro_tensor *out, acro_tensor *q, acro_tensor *k, acro_tensor *v, acro_tensor *log_decay, double scale,
+                                 acro_tensor *initial_state, acro_tensor *final_state)
+{
+    return guarded([&] {
+        require_handles("acro_engine_linear_attention", {e, out, q, k, v, log_decay});
+        e->te.LinearAttention(*out->t, *q->t, *k->t, *v->t, *log_decay->t, scale, optional_tensor(initial_state), optional_tensor(final_state));
+    });
+}
+
+int acro_engine_linear_attention_step(acro_engine *e, acro_tensor *out, acro_tensor *state_out, acro_tensor *q, acro_tensor *k, acro_tensor *v,
+                                      acro_tensor *log_decay, acro_tensor *state_in, double scale)
+{
+    return guarded([&] {
+        require_handles("acro_engine_linear_attention_step", {e, out, state_out, q, k, v, log_decay, state_in});
+        e->te.LinearAttentionStep(*out->t, *state_out->t, *q->t, *k->t, *v->t, *log_decay->t, *state_in->t, scale);
+    });
+}
+
+int acro_engine_linear_attention_backward(acro_engine *e, acro_tensor *dq, acro_tensor *dk, acro_tensor *dv, acro_tensor *dout, acro_tensor *q,
+                                          acro_tensor *k, acro_tensor *v, acro_tensor *log_decay, double scale, acro_tensor *initial_state,
+                                          acro_tensor *d_final_state, acro_tensor *d_initial_state)
+{
+    return guarded([&] {
+        require_handles("acro_engine_linear_attention_backward", {e, dq, dk, dv, dout, q, k, v, log_decay});
+        e->te.LinearAttentionBackward(*dq->t, *dk->t, *dv->t, *dout->t, *q->t, *k->t, *v->t, *log_decay->t, scale, optional_tensor(initial_state),
+                                      optional_tensor(d_final_state), optional_tensor(d_initial_state));
+    });
+}
+
+int acro_engine_layer_norm(acro_engine *e, acro_tensor *y, acro_tensor *x, acro_tensor *weight, acro_tensor *bias, double eps, acro_tensor *mean,
+                           acro_tensor *rstd)
+{
+    return guarded([&] {
+        require_handles("acro_engine_layer_norm", {e, y, x});
+        e->te.LayerNorm(*y->t, *x->t, optional_tensor(weight), optional_tensor(bias), eps, optional_tensor(mean), optional_tensor(rstd));
+    });
+}
+
+int acro_engine_layer_norm_backward(acro_engine *e, acro_tensor *dx, acro_tensor *dweight, acro_tensor *dbias, acro_tensor *dy, acro_tensor *x,
+                                    acro_tensor *mean, acro_tensor *rstd, acro_tensor *weight)
+{
+    return guarded([&] {
+        require_handles("acro_engine_layer_norm_backward", {e, dx, dy, x, mean, rstd});
+        e->te.LayerNormBackward(*dx->t, optional_tensor(dweight), optional_tensor(dbias), *dy->t, *x->t, *mean->t, *rstd->t, optional_tensor(weight));
+    });
+}
+
+void *acro_b200_get_stream(void) { return acro::getCudaStream(); }
 
 int acro_b200_set_stream(void *stream)
 {

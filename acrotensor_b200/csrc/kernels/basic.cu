@@ -52,11 +52,12 @@ int sm_count()
 
 }
 
-static __device__ int g_wait_timed_out = 0;
+// [0] a bounded wait gave up, [1] an index array held an entry that is out of range or repeated
+static __device__ int g_status_flags[2] = {0, 0};
 
 namespace
 {
-// Address of g_wait_timed_out on each device.  A device symbol has one address per CUDA context, so
+// Address of g_status_flags on each device.  A device symbol has one address per CUDA context, so
 // acro_b200_set_context clears the table.
 constexpr int kMaxDevices = 64;
 std::mutex g_wait_flag_lock;
@@ -78,10 +79,16 @@ int *wait_flag_device_ptr()
     if (ptr_of_device[dev] == nullptr)
     {
         void *p = nullptr;
-        if (cudaGetSymbolAddress(&p, g_wait_timed_out) != cudaSuccess) return nullptr;
+        if (cudaGetSymbolAddress(&p, g_status_flags) != cudaSuccess) return nullptr;
         ptr_of_device[dev] = static_cast<int *>(p);
     }
     return ptr_of_device[dev];
+}
+
+int *bad_index_flag_device_ptr()
+{
+    int *flags = wait_flag_device_ptr();
+    return flags == nullptr ? nullptr : flags + 1;
 }
 }
 
@@ -153,19 +160,24 @@ int acro_b200_set_context(void *cuda_context)
 
 int acro_b200_device_status(void)
 {
-    // Blocks until the device is idle, then reads (and clears) the bounded-wait flag.
+    // Blocks until the device is idle, then reads (and clears) the flags.
     cudaError_t status = cudaDeviceSynchronize();
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_device_status");
-    int flag = 0;
-    status = cudaMemcpyFromSymbol(&flag, g_wait_timed_out, sizeof flag);
+    int flags[2] = {0, 0};
+    status = cudaMemcpyFromSymbol(flags, g_status_flags, sizeof flags);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_device_status");
-    if (flag != 0)
+    if (flags[0] != 0 || flags[1] != 0)
     {
-        const int zero = 0;
-        cudaMemcpyToSymbol(g_wait_timed_out, &zero, sizeof zero);
+        const int zeros[2] = {0, 0};
+        cudaMemcpyToSymbol(g_status_flags, zeros, sizeof zeros);
+    }
+    if (flags[0] != 0)
+    {
         set_last_error("a bounded device-side wait on an asynchronous copy gave up; results of that launch are invalid");
         return ACRO_B200_ETIMEOUT;
     }
+    if (flags[1] != 0)
+        return fail_invalid("an array of offsets or slots held an entry that is out of range, decreasing or repeated; what belongs to it was skipped");
     return ACRO_B200_OK;
 }
 

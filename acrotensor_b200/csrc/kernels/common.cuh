@@ -24,6 +24,9 @@ int sm_count();
 // up (nullptr on failure); acro_b200_device_status() reads and clears it.
 int *wait_flag_device_ptr();
 
+// The same for index arrays that hold an entry out of range or repeated (ACRO_B200_EINVAL in acro_b200_device_status()).
+int *bad_index_flag_device_ptr();
+
 // Number of acro_b200_set_context calls so far.  The address of a __device__ symbol belongs to one CUDA
 // context, so code that caches such an address stores this value with it and looks the address up
 // again when the value has moved on.

@@ -1,0 +1,819 @@
+// Linear attention with a decay for each head: entry points, the kernels for every type and head size, the step for single
+// tokens.  linear_attention.cuh has the mathematics; linear_attention_mma.cu the main pass on the tensor cores.
+#include "linear_attention.cuh"
+
+#include <algorithm>
+
+using namespace acro_b200_detail;
+
+namespace
+{
+
+constexpr int kThreads = 256;
+constexpr int kMaxHead = 256;           // columns of a head
+
+// Sizes of the pass for one type of sums: CHUNK tokens at a time, SLICE columns of v (of the state) per CTA.
+template <class A> struct PassTile;
+template <> struct PassTile<float> { static constexpr int kChunk = 64, kSlice = 64; };
+template <> struct PassTile<double> { static constexpr int kChunk = 32, kSlice = 32; };
+
+// Rows of shared memory are read in 16-byte packs: an odd number of packs a row keeps 8 consecutive rows in different banks.
+template <class A>
+__host__ __device__ constexpr int padded(int columns)
+{
+    constexpr int n = 16 / sizeof(A);
+    const int packs = (columns + n - 1) / n;
+    return (packs | 1) * n;
+}
+
+template <class A>
+size_t pass_smem_bytes(int dq)
+{
+    constexpr int C = PassTile<A>::kChunk, SV = PassTile<A>::kSlice;
+    const int rows = (dq + 16 / sizeof(A) * 16 - 1) / (16 / sizeof(A) * 16) * (16 / sizeof(A) * 16);
+    return sizeof(A) * (C * static_cast<size_t>(padded<A>(dq) + std::max(padded<A>(dq), padded<A>(C))) + C * SV + static_cast<size_t>(rows) * SV + C + 1);
+}
+
+template <class A> struct alignas(16) Vec { A x[16 / sizeof(A)]; };
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ bool not_finite(double x) { return (__double2hiint(x) & 0x7ff00000) == 0x7ff00000; }
+
+// acc[i][j] += sum_(s < n) P[ty + 16 i][s] V[s][tx TN + j]; with GUARD only over the s that row ty + 16 i sees, because a product
+// of a masked zero with an infinity or NaN of another token would be NaN.
+template <class A, int TM, int TN, int SV, bool GUARD>
+__device__ __forceinline__ void product(A (&acc)[TM][TN], const A *p, int ldp, const A *v, int n, int ty, int tx, bool reverse)
+{
+    constexpr int VN = 16 / sizeof(A);
+    for (int s = 0; s < n; s += VN)
+    {
+        Vec<A> row[TM], col[VN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) row[i] = *reinterpret_cast<const Vec<A> *>(p + (ty + 16 * i) * ldp + s);
+#pragma unroll
+        for (int k = 0; k < VN; ++k) col[k] = *reinterpret_cast<const Vec<A> *>(v + (s + k) * SV + tx * TN);
+#pragma unroll
+        for (int k = 0; k < VN; ++k)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+            {
+                if (GUARD && (reverse ? s + k < ty + 16 * i : s + k > ty + 16 * i)) continue;
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] += row[i].x[k] * col[k].x[j];
+            }
+    }
+}
+
+// The pass for every type and head size: sums of products in the type of sums on the ordinary cores, a chunk of Q, K and V, the
+// scores and the state in shared memory, register tiles of 4 x 4 (2 x 2 in 64 bits) per thread.  Bound by those cores (0.75 of
+// its operations are multiply-adds), not by HBM.
+template <class T>
+__global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs a, int slices, bool states_only)
+{
+    using A = typename Element<T>::Acc;
+    constexpr int C = PassTile<A>::kChunk, SV = PassTile<A>::kSlice, VN = 16 / sizeof(A), TM = C / 16, TN = SV / 16;
+    static_assert(TN == VN, "a thread's columns are one pack");
+    const AttentionPass &p = a.pass[blockIdx.y];
+    const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads % slices;
+    const int c0 = slice * SV;
+    if (c0 >= p.dv) return;
+    const int64_t item_index = blockIdx.x / (static_cast<int64_t>(a.heads) * slices);
+    const bool reverse = p.reverse != 0;
+    const SegmentItem item = find_item(a, item_index, reverse);
+    if (item.sequence < 0) return;
+    const bool cut = segments_of(item.sequence_end - item.sequence_begin, a.segment) > 1;
+    if (states_only && (!cut || item.last)) return;
+
+    extern __shared__ __align__(16) unsigned char smem_bytes[];
+    const int ld = padded<A>(p.dq), ldp = padded<A>(C), cols = min(SV, p.dv - c0);
+    const int state_rows = (p.dq + VN * 16 - 1) / (VN * 16) * (VN * 16);
+    A *sq = reinterpret_cast<A *>(smem_bytes), *sp = sq, *sk = sq + C * max(ld, ldp), *sv = sk + C * ld, *st = sv + C * SV, *power = st + state_rows * SV;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+
+    const double g = decay_log<A>(a.log_decay, head);
+    for (int i = threadIdx.x; i <= C; i += kThreads) power[i] = static_cast<A>(exp(g * i));
+
+    // the state this segment starts from
+    const int64_t size = static_cast<int64_t>(p.dq) * p.dv;
+    const A *from = nullptr;
+    int turned = 0;
+    if (!states_only)
+    {
+        if (cut) from = static_cast<const A *>(p.segment_states) + (item_index * a.heads + head) * size;
+        else if (p.initial != nullptr)
+        {
+            from = static_cast<const A *>(p.initial) + (item.state * a.heads + head) * size;
+            turned = p.turned;
+        }
+    }
+    for (int i = threadIdx.x; i < state_rows * SV; i += kThreads)
+    {
+        const int d = i / SV, c = i % SV;
+        A x = 0;
+        if (from != nullptr && d < p.dq && c < cols) x = turned ? from[static_cast<int64_t>(c0 + c) * p.dq + d] : from[static_cast<int64_t>(d) * p.dv + c0 + c];
+        st[i] = x;
+    }
+    const T *q = rows_of<const T>(p.q, a, item.sequence, head), *k = rows_of<const T>(p.k, a, item.sequence, head),
+            *v = rows_of<const T>(p.v, a, item.sequence, head);
+
+    const int64_t chunks = (item.end - item.begin + C - 1) / C;
+    for (int64_t index = 0; index < chunks; ++index)
+    {
+        const int64_t t0 = item.begin + (reverse ? chunks - 1 - index : index) * C;
+        const int m = static_cast<int>(min(static_cast<int64_t>(C), item.end - t0));
+        __syncthreads();
+        // rows behind the chunk's last token and columns behind the head's last one are zeros
+        bool odd = false;
+        for (int i = threadIdx.x; i < C * ld; i += kThreads)
+        {
+            const int r = i / ld, d = i % ld;
+            const bool there = r < m && d < p.dq;
+            if (!states_only) sq[i] = there ? widen(q[(t0 + r) * p.q.token + d]) : A(0);
+            sk[i] = there ? widen(k[(t0 + r) * p.k.token + d]) : A(0);
+        }
+        for (int i = threadIdx.x; i < C * SV; i += kThreads)
+        {
+            const int r = i / SV, c = i % SV;
+            const A x = r < m && c < cols ? static_cast<A>(widen(v[(t0 + r) * p.v.token + c0 + c])) : A(0);
+            sv[i] = x;
+            odd |= not_finite(x);
+        }
+        odd = __syncthreads_or(odd) != 0;
+        if (!states_only)
+        {
+            A acc[TM][TM];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TM; ++j) acc[i][j] = 0;
+            for (int d = 0; d < p.dq; d += VN)
+            {
+                Vec<A> x[TM], y[TM];
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+                {
+                    x[i] = *reinterpret_cast<const Vec<A> *>(sq + (ty + 16 * i) * ld + d);
+                    y[i] = *reinterpret_cast<const Vec<A> *>(sk + (tx + 16 * i) * ld + d);
+                }
+#pragma unroll
+                for (int n = 0; n < VN; ++n)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TM; ++j) acc[i][j] += x[i].x[n] * y[j].x[n];
+            }
+            A near[TM][TN], far[TM][TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) near[i][j] = far[i][j] = 0;
+            product<A, TM, TN, SV, false>(far, sq, ld, st, p.dq, ty, tx, reverse);
+            __syncthreads();            // the scores take Q's place
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TM; ++j)
+                {
+                    const int r = ty + 16 * i, s = tx + 16 * j, n = reverse ? s - r : r - s;
+                    sp[r * ldp + s] = n < 0 ? A(0) : acc[i][j] * power[n] * static_cast<A>(p.state_scale);
+                }
+            __syncthreads();
+            if (odd) product<A, TM, TN, SV, true>(near, sp, ldp, sv, C, ty, tx, reverse);
+            else product<A, TM, TN, SV, false>(near, sp, ldp, sv, C, ty, tx, reverse);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+            {
+                const int r = ty + 16 * i;
+                if (r >= m) continue;
+                const A come = power[reverse ? m - 1 - r : r + 1];
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                {
+                    const int c = tx * TN + j;
+                    if (c >= cols) continue;
+                    const A o = static_cast<A>(p.out_scale) * (near[i][j] + come * far[i][j]);
+                    const int64_t at = (t0 + r) * p.out.token + c0 + c;
+                    if (p.sums) rows_of<A>(p.out, a, item.sequence, head)[at] = o;
+                    else rows_of<T>(p.out, a, item.sequence, head)[at] = narrow<T>(o);
+                }
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < C * SV; i += kThreads)
+        {
+            const int r = i / SV;
+            if (r < m) sv[i] *= power[reverse ? r + 1 : m - 1 - r] * static_cast<A>(p.state_scale);
+        }
+        __syncthreads();
+        // what is left of the state after m tokens, to twice the digits: the rounding of one factor would come back in every chunk
+        const double exact = exp(g * m);
+        const A keep = static_cast<A>(exact), rest = static_cast<A>(exact - static_cast<double>(keep));
+        for (int d = ty * VN; d < state_rows; d += 16 * VN)
+        {
+            A acc[VN][TN];
+#pragma unroll
+            for (int i = 0; i < VN; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = 0;
+            if (d < p.dq)
+                for (int s = 0; s < m; ++s)
+                {
+                    const Vec<A> x = *reinterpret_cast<const Vec<A> *>(sk + s * ld + d), y = *reinterpret_cast<const Vec<A> *>(sv + s * SV + tx * TN);
+#pragma unroll
+                    for (int i = 0; i < VN; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j] += x.x[i] * y.x[j];
+                }
+#pragma unroll
+            for (int i = 0; i < VN; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                {
+                    A &s = st[(d + i) * SV + tx * TN + j];
+                    s = keep * s + (rest * s + acc[i][j]);
+                }
+        }
+    }
+    __syncthreads();
+    A *to = nullptr;
+    turned = 0;
+    if (states_only) to = static_cast<A *>(p.segment_states) + (item_index * a.heads + head) * size;
+    else if (item.last && p.final != nullptr)
+    {
+        to = static_cast<A *>(p.final) + (item.state * a.heads + head) * size;
+        turned = p.turned;
+    }
+    if (to == nullptr) return;
+    for (int i = threadIdx.x; i < p.dq * SV; i += kThreads)
+    {
+        const int d = i / SV, c = i % SV;
+        if (c < cols) to[turned ? static_cast<int64_t>(c0 + c) * p.dq + d : static_cast<int64_t>(d) * p.dv + c0 + c] = st[i];
+    }
+}
+
+// Turns the segments' own states into the states that they start from: one thread per entry of a state, walking a sequence's
+// segments in the order of time.
+template <class A>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(AttentionArgs a)
+{
+    __shared__ int64_t total;
+    const AttentionPass &p = a.pass[blockIdx.z];
+    const int head = blockIdx.x % a.heads;
+    const int64_t n = blockIdx.x / a.heads;
+    const bool reverse = p.reverse != 0;
+    int64_t begin = 0, end = a.tokens, first = n * segments_of(a.tokens, a.segment);
+    if (a.offsets != nullptr)
+    {
+        packed_range(a, n, &begin, &end);
+        if (threadIdx.x == 0) total = 0;
+        __syncthreads();
+        int64_t before = 0;
+        for (int64_t i = threadIdx.x; i < n; i += kThreads)
+        {
+            int64_t b, e;
+            packed_range(a, i, &b, &e);
+            before += segments_of(e - b, a.segment);
+        }
+        if (before > 0) atomicAdd(reinterpret_cast<unsigned long long *>(&total), static_cast<unsigned long long>(before));
+        __syncthreads();
+        first = total;
+    }
+    const int64_t count = segments_of(end - begin, a.segment);
+    if (count <= 1 || first + count > a.items) return;     // more segments than rows allow: only with offsets that decrease
+    const int64_t state = state_of(a.slots, n, a.state_count, a.bad_index);
+    if (state < 0) return;
+    const double g = decay_log<A>(a.log_decay, head);
+    const int64_t size = static_cast<int64_t>(p.dq) * p.dv;
+    for (int64_t i = static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x; i < size; i += static_cast<int64_t>(gridDim.y) * kThreads)
+    {
+        double run = 0;
+        if (p.initial != nullptr)
+        {
+            const A *from = static_cast<const A *>(p.initial) + (state * a.heads + head) * size;
+            run = p.turned ? from[i % p.dv * p.dq + i / p.dv] : from[i];
+        }
+#pragma unroll 4
+        for (int64_t k = 0; k < count; ++k)
+        {
+            const int64_t at = reverse ? count - 1 - k : k;
+            A *s = static_cast<A *>(p.segment_states) + ((first + at) * a.heads + head) * size + i;
+            const int64_t length = min(a.segment, end - begin - at * a.segment);
+            const A own = k + 1 < count ? *s : A(0);
+            *s = static_cast<A>(run);
+            run = exp(g * static_cast<double>(length)) * run + own;
+        }
+    }
+}
+
+// out[row, h, c] = sum over the query heads of head h, in ascending order: the gradients of shared keys and values.
+template <class T>
+__global__ void __launch_bounds__(kThreads) attention_share_kernel(AttentionArgs a, const typename Element<T>::Acc *sums, TokenRows out, int heads, int group,
+                                                                   int columns)
+{
+    using A = typename Element<T>::Acc;
+    int64_t begin = 0, end = a.sequences * a.tokens;
+    if (a.offsets != nullptr)
+    {
+        begin = min(max(a.offsets[0], int64_t(0)), a.tokens);
+        end = min(max(a.offsets[a.sequences], int64_t(0)), a.tokens);
+    }
+    const int64_t each = static_cast<int64_t>(heads) * columns, total = (end - begin) * each;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads)
+    {
+        const int64_t row = begin + i / each;
+        const int h = static_cast<int>(i % each / columns), c = static_cast<int>(i % columns);
+        const A *from = sums + (row * heads * group + static_cast<int64_t>(h) * group) * columns + c;
+        A s = from[0];
+        for (int k = 1; k < group; ++k) s += from[static_cast<int64_t>(k) * columns];
+        const int64_t n = a.offsets == nullptr ? row / a.tokens : 0, t = a.offsets == nullptr ? row % a.tokens : row;
+        static_cast<T *>(out.data)[n * out.sequence + t * out.token + h * out.head + c] = narrow<T>(s);
+    }
+}
+
+struct StepArgs
+{
+    TokenRows q, k, v, out;             // token: the distance of two requests
+    int32_t heads, dk, dv, lanes;       // lanes: threads of one row of the state, a power of two
+    int32_t tiles;
+    const void *log_decay, *state_in;
+    void *state_out;
+    const int32_t *slots;
+    int64_t requests, state_count;
+    double scale;
+    int *bad_index;
+};
+
+// One token of every request: state <- lam state + k v^T, out = scale q^T state.  Bound by HBM: the state is read and written
+// once (8 bytes per entry in 32 bits) for five operations.  A CTA takes one head's state (or a tile of its columns), neighbouring
+// lanes neighbouring packs of a row; a thread has UNROLL rows' packs in flight.  The rows' parts of `out` are added per thread,
+// then over the lanes of a warp, then over the warps in ascending order.
+template <class T, int VN>
+__global__ void __launch_bounds__(kThreads) attention_step_kernel(StepArgs a)
+{
+    using A = typename Element<T>::Acc;
+    constexpr int UNROLL = 8;
+    __shared__ A sk[kMaxHead], sq[kMaxHead], part[kThreads / 32][32 * VN];
+    const int head = blockIdx.x % a.heads, tile = blockIdx.x / a.heads % a.tiles;
+    const int64_t n = blockIdx.x / (static_cast<int64_t>(a.heads) * a.tiles);
+    const int64_t state = state_of(a.slots, n, a.state_count, a.bad_index);
+    if (state < 0) return;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int row0 = threadIdx.x / a.lanes, rows = kThreads / a.lanes;
+    const int c = tile * 32 * VN + threadIdx.x % a.lanes * VN;
+    const bool there = c < a.dv;
+    const int64_t base = (state * a.heads + head) * static_cast<int64_t>(a.dk) * a.dv + c;
+    const A *in = static_cast<const A *>(a.state_in) + base;
+    A *to = static_cast<A *>(a.state_out) + base;
+    Pack<A, VN> s[UNROLL];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i)
+    {
+        const int d = row0 + i * rows;
+        if (there && d < a.dk) s[i] = *reinterpret_cast<const Pack<A, VN> *>(in + static_cast<int64_t>(d) * a.dv);
+    }
+    const T *q = static_cast<const T *>(a.q.data) + n * a.q.token + static_cast<int64_t>(head / a.q.group) * a.q.head,
+            *k = static_cast<const T *>(a.k.data) + n * a.k.token + static_cast<int64_t>(head / a.k.group) * a.k.head,
+            *v = static_cast<const T *>(a.v.data) + n * a.v.token + static_cast<int64_t>(head / a.v.group) * a.v.head;
+    for (int d = threadIdx.x; d < a.dk; d += kThreads)
+    {
+        sk[d] = widen(k[d]);
+        sq[d] = widen(q[d]);
+    }
+    const A lam = static_cast<A>(exp(static_cast<double>(decay_log<A>(a.log_decay, head))));
+    A x[VN], o[VN];
+#pragma unroll
+    for (int j = 0; j < VN; ++j)
+    {
+        x[j] = there ? static_cast<A>(widen(v[c + j])) : A(0);
+        o[j] = 0;
+    }
+    __syncthreads();
+    for (int d0 = row0; d0 < a.dk; d0 += UNROLL * rows)
+    {
+        if (d0 != row0)
+        {
+#pragma unroll
+            for (int i = 0; i < UNROLL; ++i)
+            {
+                const int d = d0 + i * rows;
+                if (there && d < a.dk) s[i] = *reinterpret_cast<const Pack<A, VN> *>(in + static_cast<int64_t>(d) * a.dv);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i)
+        {
+            const int d = d0 + i * rows;
+            if (!there || d >= a.dk) continue;
+            const A kd = sk[d], qd = sq[d];
+#pragma unroll
+            for (int j = 0; j < VN; ++j)
+            {
+                s[i].x[j] = lam * s[i].x[j] + kd * x[j];
+                o[j] += qd * s[i].x[j];
+            }
+            *reinterpret_cast<Pack<A, VN> *>(to + static_cast<int64_t>(d) * a.dv) = s[i];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VN; ++j)
+        for (int w = a.lanes; w < 32; w <<= 1) o[j] += __shfl_xor_sync(0xffffffffu, o[j], w);
+    if (lane < a.lanes)
+    {
+#pragma unroll
+        for (int j = 0; j < VN; ++j) part[warp][lane * VN + j] = o[j];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.lanes * VN; i += kThreads)
+    {
+        const int column = tile * 32 * VN + i;
+        if (column >= a.dv) continue;
+        A sum = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) sum += part[w][i];
+        (static_cast<T *>(a.out.data) + n * a.out.token + static_cast<int64_t>(head / a.out.group) * a.out.head)[column] =
+            narrow<T>(static_cast<A>(a.scale) * sum);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+constexpr int kSegmentQuantum = 128;    // every kernel's chunk divides it
+
+std::string head_fault(const acro_b200_linear_attention_desc *d)
+{
+    if (d == nullptr) return "null descriptor";
+    if (!known_type(d->type)) return "unknown element type";
+    if (d->q_heads < 1 || d->kv_heads < 1 || d->q_heads % d->kv_heads != 0) return "q_heads is not a positive multiple of kv_heads";
+    if (d->q_heads > 65535) return "more than 65535 heads";
+    if (d->dk < 1 || d->dk > kMaxHead || d->dv < 1 || d->dv > kMaxHead) return "head sizes are not in 1 .. 256";
+    if (d->sequences < 0 || d->tokens < 0) return "negative number of sequences or tokens";
+    if (!(d->scale - d->scale == 0)) return "the scale is not finite";
+    return "";
+}
+
+// Tokens of a segment.  With at least half as many (sequence, head) pairs as SMs the pairs alone fill the GPU (a cut reads k
+// and v twice); fewer are cut so that segments x heads come to about one per SM.  Packed sequences are treated as one axis of
+// all their rows, since their lengths are not known here.
+int64_t segment_tokens(const acro_b200_linear_attention_desc &d, bool packed)
+{
+    const int64_t sms = sm_count() > 0 ? sm_count() : 148;
+    const int64_t whole = (d.tokens + kSegmentQuantum - 1) / kSegmentQuantum * kSegmentQuantum;
+    const int64_t pairs = (packed ? 1 : std::max<int64_t>(1, d.sequences)) * d.q_heads;
+    const int64_t wanted = std::max<int64_t>(1, sms / pairs);
+    int64_t segment = (d.tokens + wanted - 1) / wanted;
+    segment = (segment + kSegmentQuantum - 1) / kSegmentQuantum * kSegmentQuantum;
+    segment = std::max<int64_t>(segment, 4 * kSegmentQuantum);
+    return std::max<int64_t>(kSegmentQuantum, std::min(segment, whole));
+}
+
+int64_t item_bound(const acro_b200_linear_attention_desc &d, bool packed, int64_t segment)
+{
+    const int64_t each = d.tokens <= segment ? 1 : (d.tokens + segment - 1) / segment;
+    if (!packed) return d.sequences * each;
+    return d.tokens <= segment ? d.sequences : d.sequences + d.tokens / segment;
+}
+
+bool may_cut(const acro_b200_linear_attention_desc &d, int64_t segment) { return d.tokens > segment; }
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t states_bytes(const acro_b200_linear_attention_desc &d, bool packed)
+{
+    const int64_t segment = segment_tokens(d, packed);
+    if (!may_cut(d, segment)) return 0;
+    return round256(static_cast<size_t>(item_bound(d, packed, segment)) * d.q_heads * d.dk * d.dv * statistic_bytes(d.type));
+}
+
+size_t shared_bytes(const acro_b200_linear_attention_desc &d, bool packed, int columns)
+{
+    if (d.q_heads == d.kv_heads) return 0;
+    const int64_t rows = packed ? d.tokens : d.sequences * d.tokens;
+    return round256(static_cast<size_t>(rows) * d.q_heads * columns * statistic_bytes(d.type));
+}
+
+TokenRows rows_from(const acro_b200_token_array &x, int group) { return {x.data, x.sequence_stride, x.token_stride, x.head_stride, group}; }
+
+std::string array_fault(const acro_b200_token_array *x, int64_t columns, int heads, int64_t tokens, int64_t sequences, bool packed, const char *name)
+{
+    const std::string n(name);
+    if (x == nullptr || x->data == nullptr) return n + " is a null pointer";
+    if ((heads > 1 && x->head_stride < columns) || (tokens > 1 && x->token_stride < columns) || (!packed && sequences > 1 && x->sequence_stride < columns))
+        return n + " has rows that overlap";
+    if (!on_current_device(x->data)) return n + " is not memory of the current device";
+    return "";
+}
+
+template <class T>
+int run_pass(const AttentionArgs &a, bool states_only, cudaStream_t stream)
+{
+    using A = typename Element<T>::Acc;
+    int slices = 1;
+    size_t smem = 0;
+    for (int i = 0; i < a.passes; ++i)
+    {
+        slices = std::max(slices, (a.pass[i].dv + PassTile<A>::kSlice - 1) / PassTile<A>::kSlice);
+        smem = std::max(smem, pass_smem_bytes<A>(a.pass[i].dq));
+    }
+    cudaError_t status = cudaFuncSetAttribute(attention_pass_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (status != cudaSuccess) return fail_cuda(status, "acro_b200_linear_attention");
+    const int64_t grid = a.items * a.heads * slices;
+    if (grid > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 segments x heads");
+    attention_pass_kernel<T><<<dim3(static_cast<unsigned>(grid), a.passes), kThreads, smem, stream>>>(a, slices, states_only);
+    return launch_status("acro_b200_linear_attention");
+}
+
+int run_pass_of(int type, const AttentionArgs &a, bool states_only, cudaStream_t stream)
+{
+    switch (type)
+    {
+    case ACRO_B200_F64: return run_pass<double>(a, states_only, stream);
+    case ACRO_B200_F32: return run_pass<float>(a, states_only, stream);
+    case ACRO_B200_BF16: return run_pass<__nv_bfloat16>(a, states_only, stream);
+    default: return run_pass<__half>(a, states_only, stream);
+    }
+}
+
+int run_all(int type, const AttentionArgs &a, bool cut, cudaStream_t stream)
+{
+    if (cut)
+    {
+        int status = run_pass_of(type, a, true, stream);
+        if (status != ACRO_B200_OK) return status;
+        const dim3 grid(static_cast<unsigned>(a.sequences * a.heads), 16, a.passes);
+        if (type == ACRO_B200_F64) attention_join_kernel<double><<<grid, kThreads, 0, stream>>>(a);
+        else attention_join_kernel<float><<<grid, kThreads, 0, stream>>>(a);
+        status = launch_status("acro_b200_linear_attention");
+        if (status != ACRO_B200_OK) return status;
+    }
+    return run_pass_of(type, a, false, stream);
+}
+
+int common_args(const acro_b200_linear_attention_desc &d, const void *log_decay, const int64_t *offsets, AttentionArgs *a)
+{
+    a->heads = d.q_heads;
+    a->log_decay = log_decay;
+    a->offsets = offsets;
+    a->slots = nullptr;
+    a->state_count = d.sequences;
+    a->sequences = d.sequences;
+    a->tokens = d.tokens;
+    a->segment = segment_tokens(d, offsets != nullptr);
+    a->items = item_bound(d, offsets != nullptr, a->segment);
+    a->bad_index = bad_index_flag_device_ptr();
+    a->wait_flag = wait_flag_device_ptr();
+    if (a->bad_index == nullptr || a->wait_flag == nullptr) return fail_cuda(cudaErrorUnknown, "acro_b200_linear_attention (device flag)");
+    if (d.sequences * d.q_heads > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 sequences x heads");
+    return ACRO_B200_OK;
+}
+
+}
+
+extern "C" {
+
+size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
+{
+    if (!head_fault(desc).empty()) return 0;
+    return states_bytes(*desc, packed != 0);
+}
+
+int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
+                               const acro_b200_token_array *v, const acro_b200_token_array *out, const void *log_decay, const int64_t *offsets,
+                               const void *initial_state, void *final_state, const int32_t *slots, int64_t state_count, void *scratch, size_t scratch_bytes,
+                               void *stream)
+{
+    const std::string name = "acro_b200_linear_attention: ";
+    std::string fault = head_fault(desc);
+    if (!fault.empty()) return fail_invalid(name + fault);
+    const acro_b200_linear_attention_desc &d = *desc;
+    if (d.sequences == 0) return ACRO_B200_OK;
+    const bool packed = offsets != nullptr, rows = d.tokens > 0;
+    if (rows)
+    {
+        if (fault.empty()) fault = array_fault(q, d.dk, d.q_heads, d.tokens, d.sequences, packed, "q");
+        if (fault.empty()) fault = array_fault(k, d.dk, d.kv_heads, d.tokens, d.sequences, packed, "k");
+        if (fault.empty()) fault = array_fault(v, d.dv, d.kv_heads, d.tokens, d.sequences, packed, "v");
+        if (fault.empty()) fault = array_fault(out, d.dv, d.q_heads, d.tokens, d.sequences, packed, "out");
+    }
+    if (fault.empty() && log_decay == nullptr) fault = "log_decay is a null pointer";
+    if (fault.empty() && slots != nullptr && state_count < 0) fault = "negative state_count";
+    if (fault.empty() && slots == nullptr && state_count != d.sequences && (initial_state != nullptr || final_state != nullptr))
+        fault = "without slots there is one state per sequence";
+    const size_t need = states_bytes(d, packed);
+    if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
+        fault = "scratch is smaller than acro_b200_linear_attention_scratch_bytes or not 16-byte aligned";
+    if (fault.empty() && need > 0 && !on_current_device(scratch)) fault = "scratch is not memory of the current device";
+    if (fault.empty() && ((initial_state != nullptr && !on_current_device(initial_state)) || (final_state != nullptr && !on_current_device(final_state))))
+        fault = "a state is not memory of the current device";
+    if (fault.empty() && rows && (out->data == q->data || out->data == k->data || out->data == v->data))
+        fault = "out takes the place of an operand that is still read";
+    if (!fault.empty()) return fail_invalid(name + fault);
+    AttentionArgs a = {};
+    int status = common_args(d, log_decay, offsets, &a);
+    if (status != ACRO_B200_OK) return status;
+    if (slots != nullptr)
+    {
+        a.slots = slots;
+        a.state_count = state_count;
+    }
+    const acro_b200_token_array none = {};
+    const int group = d.q_heads / d.kv_heads;
+    a.passes = 1;
+    AttentionPass &p = a.pass[0];
+    p.q = rows_from(rows ? *q : none, 1);
+    p.k = rows_from(rows ? *k : none, group);
+    p.v = rows_from(rows ? *v : none, group);
+    p.out = rows_from(rows ? *out : none, 1);
+    p.dq = d.dk;
+    p.dv = d.dv;
+    p.state_scale = 1;
+    p.out_scale = d.scale;
+    p.initial = initial_state;
+    p.final = final_state;
+    p.segment_states = scratch;
+    return run_all(d.type, a, need > 0, as_stream(stream));
+}
+
+int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
+                                    const acro_b200_token_array *v, const acro_b200_token_array *out, const void *log_decay, const void *state_in,
+                                    void *state_out, const int32_t *slots, int64_t state_count, void *stream)
+{
+    const std::string name = "acro_b200_linear_attention_step: ";
+    std::string fault = head_fault(desc);
+    if (!fault.empty()) return fail_invalid(name + fault);
+    const acro_b200_linear_attention_desc &d = *desc;
+    if (d.tokens != 1) return fail_invalid(name + "a step takes one token of each sequence");
+    if (d.sequences == 0) return ACRO_B200_OK;
+    // the distance of two requests is that of two sequences
+    fault = array_fault(q, d.dk, d.q_heads, 1, d.sequences, false, "q");
+    if (fault.empty()) fault = array_fault(k, d.dk, d.kv_heads, 1, d.sequences, false, "k");
+    if (fault.empty()) fault = array_fault(v, d.dv, d.kv_heads, 1, d.sequences, false, "v");
+    if (fault.empty()) fault = array_fault(out, d.dv, d.q_heads, 1, d.sequences, false, "out");
+    if (fault.empty() && (log_decay == nullptr || state_in == nullptr || state_out == nullptr)) fault = "null pointer";
+    if (fault.empty() && (!on_current_device(state_in) || !on_current_device(state_out))) fault = "a state is not memory of the current device";
+    if (fault.empty() && (state_count < 0 || (slots == nullptr && state_count != d.sequences))) fault = "without slots there is one state per sequence";
+    if (!fault.empty()) return fail_invalid(name + fault);
+    StepArgs a = {};
+    const int group = d.q_heads / d.kv_heads;
+    a.q = rows_from(*q, 1);
+    a.k = rows_from(*k, group);
+    a.v = rows_from(*v, group);
+    a.out = rows_from(*out, 1);
+    a.q.token = q->sequence_stride;
+    a.k.token = k->sequence_stride;
+    a.v.token = v->sequence_stride;
+    a.out.token = out->sequence_stride;
+    a.heads = d.q_heads;
+    a.dk = d.dk;
+    a.dv = d.dv;
+    a.log_decay = log_decay;
+    a.state_in = state_in;
+    a.state_out = state_out;
+    a.slots = slots;
+    a.requests = d.sequences;
+    a.state_count = state_count;
+    a.scale = d.scale;
+    a.bad_index = bad_index_flag_device_ptr();
+    if (a.bad_index == nullptr) return fail_cuda(cudaErrorUnknown, "acro_b200_linear_attention_step (device flag)");
+    // packs of 16 bytes when every row of the states starts on their boundary
+    const int pack = static_cast<int>(16 / statistic_bytes(d.type));
+    const bool packs = d.dv % pack == 0 && aligned16(state_in) && aligned16(state_out);
+    const int columns = 32 * (packs ? pack : 1), per_row = (std::min(d.dv, columns) + (packs ? pack : 1) - 1) / (packs ? pack : 1);
+    a.tiles = (d.dv + columns - 1) / columns;
+    a.lanes = 1;
+    while (a.lanes < per_row) a.lanes *= 2;
+    const int64_t grid = d.sequences * d.q_heads * a.tiles;
+    if (grid > INT32_MAX) return fail_unsupported(name + "more than 2^31 requests x heads");
+    const unsigned g = static_cast<unsigned>(grid);
+    cudaStream_t st = as_stream(stream);
+    switch (d.type)
+    {
+    case ACRO_B200_F64:
+        if (packs) attention_step_kernel<double, 2><<<g, kThreads, 0, st>>>(a);
+        else attention_step_kernel<double, 1><<<g, kThreads, 0, st>>>(a);
+        break;
+    case ACRO_B200_F32:
+        if (packs) attention_step_kernel<float, 4><<<g, kThreads, 0, st>>>(a);
+        else attention_step_kernel<float, 1><<<g, kThreads, 0, st>>>(a);
+        break;
+    case ACRO_B200_BF16:
+        if (packs) attention_step_kernel<__nv_bfloat16, 4><<<g, kThreads, 0, st>>>(a);
+        else attention_step_kernel<__nv_bfloat16, 1><<<g, kThreads, 0, st>>>(a);
+        break;
+    default:
+        if (packs) attention_step_kernel<__half, 4><<<g, kThreads, 0, st>>>(a);
+        else attention_step_kernel<__half, 1><<<g, kThreads, 0, st>>>(a);
+    }
+    return launch_status("acro_b200_linear_attention_step");
+}
+
+size_t acro_b200_linear_attention_backward_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
+{
+    if (!head_fault(desc).empty()) return 0;
+    return 3 * states_bytes(*desc, packed != 0) + shared_bytes(*desc, packed != 0, desc->dk) + shared_bytes(*desc, packed != 0, desc->dv);
+}
+
+int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
+                                        const acro_b200_token_array *v, const acro_b200_token_array *dout, const void *log_decay, const int64_t *offsets,
+                                        const void *initial_state, const void *d_final_state, const acro_b200_token_array *dq,
+                                        const acro_b200_token_array *dk, const acro_b200_token_array *dv, void *d_initial_state, void *scratch,
+                                        size_t scratch_bytes, void *stream)
+{
+    const std::string name = "acro_b200_linear_attention_backward: ";
+    std::string fault = head_fault(desc);
+    if (!fault.empty()) return fail_invalid(name + fault);
+    const acro_b200_linear_attention_desc &d = *desc;
+    if (d.sequences == 0) return ACRO_B200_OK;
+    const bool packed = offsets != nullptr, rows = d.tokens > 0;
+    const struct { const acro_b200_token_array *x; int columns, heads; const char *name; } arrays[] = {
+        {q, d.dk, d.q_heads, "q"}, {k, d.dk, d.kv_heads, "k"}, {v, d.dv, d.kv_heads, "v"}, {dout, d.dv, d.q_heads, "dout"},
+        {dq, d.dk, d.q_heads, "dq"}, {dk, d.dk, d.kv_heads, "dk"}, {dv, d.dv, d.kv_heads, "dv"}};
+    if (rows)
+        for (const auto &x : arrays)
+            if (fault.empty()) fault = array_fault(x.x, x.columns, x.heads, d.tokens, d.sequences, packed, x.name);
+    if (fault.empty() && log_decay == nullptr) fault = "log_decay is a null pointer";
+    const size_t need = acro_b200_linear_attention_backward_scratch_bytes(desc, packed);
+    if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
+        fault = "scratch is smaller than acro_b200_linear_attention_backward_scratch_bytes or not 16-byte aligned";
+    if (fault.empty() && need > 0 && !on_current_device(scratch)) fault = "scratch is not memory of the current device";
+    for (const void *s : {initial_state, d_final_state, static_cast<const void *>(d_initial_state)})
+        if (fault.empty() && s != nullptr && !on_current_device(s)) fault = "a state is not memory of the current device";
+    if (fault.empty() && d_initial_state != nullptr && (d_initial_state == d_final_state || d_initial_state == initial_state))
+        fault = "d_initial_state takes the place of a state that is still read";
+    if (fault.empty() && rows)
+        for (const acro_b200_token_array *to : {dq, dk, dv})
+            for (const acro_b200_token_array *from : {q, k, v, dout})
+                if (to->data == from->data) fault = "a gradient takes the place of an operand that is still read";
+    if (!fault.empty()) return fail_invalid(name + fault);
+    AttentionArgs a = {};
+    int status = common_args(d, log_decay, offsets, &a);
+    if (status != ACRO_B200_OK) return status;
+    const acro_b200_token_array none = {};
+    const int group = d.q_heads / d.kv_heads;
+    const TokenRows rq = rows_from(rows ? *q : none, 1), rk = rows_from(rows ? *k : none, group), rv = rows_from(rows ? *v : none, group),
+                    ro = rows_from(rows ? *dout : none, 1);
+    const size_t states = states_bytes(d, packed);
+    unsigned char *at = static_cast<unsigned char *>(scratch);
+    a.passes = 3;
+    for (int i = 0; i < 3; ++i)
+    {
+        AttentionPass &p = a.pass[i];
+        p.segment_states = at;
+        at += states;
+        p.reverse = i > 0;
+        p.state_scale = i > 0 ? d.scale : 1;
+        p.out_scale = i > 0 ? 1 : d.scale;
+        p.turned = i < 2;
+        p.dq = i < 2 ? d.dv : d.dk;
+        p.dv = i < 2 ? d.dk : d.dv;
+        p.initial = i > 0 ? d_final_state : initial_state;
+        p.final = i == 2 ? d_initial_state : nullptr;
+    }
+    a.pass[0].q = ro;
+    a.pass[0].k = rv;
+    a.pass[0].v = rk;
+    a.pass[0].out = rows_from(rows ? *dq : none, 1);
+    a.pass[1].q = rv;
+    a.pass[1].k = ro;
+    a.pass[1].v = rq;
+    a.pass[2].q = rk;
+    a.pass[2].k = rq;
+    a.pass[2].v = ro;
+    if (group == 1)
+    {
+        a.pass[1].out = rows_from(rows ? *dk : none, 1);
+        a.pass[2].out = rows_from(rows ? *dv : none, 1);
+        return run_all(d.type, a, states > 0, as_stream(stream));
+    }
+    // a row of sums per query head, added up afterwards
+    void *sums[2];
+    const int columns[2] = {d.dk, d.dv};
+    for (int i = 0; i < 2; ++i)
+    {
+        sums[i] = at;
+        at += shared_bytes(d, packed, columns[i]);
+        const int64_t row = static_cast<int64_t>(d.q_heads) * columns[i];
+        a.pass[1 + i].out = {sums[i], row * d.tokens, row, columns[i], 1};
+        a.pass[1 + i].sums = 1;
+    }
+    cudaStream_t st = as_stream(stream);
+    status = run_all(d.type, a, states > 0, st);
+    if (status != ACRO_B200_OK || !rows) return status;
+    for (int i = 0; i < 2; ++i)
+    {
+        const TokenRows out = rows_from(i == 0 ? *dk : *dv, 1);
+        const int64_t entries = (packed ? 1 : d.sequences) * d.tokens * d.kv_heads * columns[i];
+        const unsigned grid = static_cast<unsigned>(std::min<int64_t>((entries + kThreads - 1) / kThreads, 148 * 16));
+        switch (d.type)
+        {
+        case ACRO_B200_F64: attention_share_kernel<double><<<grid, kThreads, 0, st>>>(a, static_cast<double *>(sums[i]), out, d.kv_heads, group, columns[i]); break;
+        case ACRO_B200_F32: attention_share_kernel<float><<<grid, kThreads, 0, st>>>(a, static_cast<float *>(sums[i]), out, d.kv_heads, group, columns[i]); break;
+        case ACRO_B200_BF16:
+            attention_share_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, static_cast<float *>(sums[i]), out, d.kv_heads, group, columns[i]);
+            break;
+        default: attention_share_kernel<__half><<<grid, kThreads, 0, st>>>(a, static_cast<float *>(sums[i]), out, d.kv_heads, group, columns[i]);
+        }
+    }
+    return launch_status("acro_b200_linear_attention_backward");
+}
+
+}

@@ -1,0 +1,199 @@
+// Linear attention with a decay for each head: what its kernels share.
+//
+// Per sequence and head, with lam = exp(log_decay):   S_t = lam S_(t-1) + k_t v_t^T,   o_t = scale q_t^T S_t.
+// A chunk of m tokens starting from the state S (row r of the chunk, natural order):
+//   o_r = scale ( come_r q_r^T S + sum_(s <= r) lam^(r-s) (q_r.k_s) v_s ),   come_r = lam^(r+1)
+//   S'  = lam^m S + sum_s left_s k_s v_s^T,                                  left_s = lam^(m-1-s)
+// Every gradient is a pass of the same form with its operands in other places:
+//   dq = pass(q := do, k := v, v := k), forward in time, with the transposed state
+//   dk = pass(q := v, k := do, v := q), dv = pass(q := k, k := q, v := do), both backward in time with the gradient of the state,
+//        which a backward pass holds already decayed: sums over s >= r, come_r = lam^(m-1-r), left_s = lam^(s+1)
+// so come and left change places, and the state after the first token is the gradient of the initial state.
+//
+// A long sequence is cut into segments so that few heads still fill the GPU: a first pass over all segments but the last
+// makes each one's own state from zero, a small kernel turns these into the states the segments start from, and the main pass
+// runs the segments beside one another.  That reads k and v twice, so it is done only when sequences x heads leave SMs idle.
+#ifndef ACRO_B200_KERNELS_LINEAR_ATTENTION_CUH
+#define ACRO_B200_KERNELS_LINEAR_ATTENTION_CUH
+
+#include "element.cuh"
+
+namespace acro_b200_detail
+{
+
+// Rows of one operand: element (sequence n, token t, head h, column c) at data[n * sequence + t * token + h * head + c]; with
+// packed sequences `sequence` is not used and t counts over all rows.  group: query heads that share a head of this operand.
+struct TokenRows
+{
+    void *data;
+    int64_t sequence, token, head;
+    int32_t group;
+};
+
+// One pass over all sequences and heads.
+struct AttentionPass
+{
+    TokenRows q, k, v, out;
+    int32_t dq, dv;                     // columns of q and k; of v and out
+    int32_t reverse;                    // backward in time
+    int32_t turned;                     // the user's states are [dv][dq]: read and written transposed
+    int32_t sums;                       // out is in the type of sums (one row per query head, to be added up), not the element type
+    double state_scale, out_scale;      // on k v^T as it enters the state, on q^T S; their product on (q.k) v
+    const void *initial;                // state a sequence starts from, or null: zero
+    void *final;                        // state it ends with, or null
+    void *segment_states;               // [items][heads][dq][dv], or null when no sequence is cut
+};
+
+struct AttentionArgs
+{
+    AttentionPass pass[3];
+    int32_t passes;
+    int32_t heads;
+    const void *log_decay;
+    const int64_t *offsets;             // sequences + 1 row numbers, or null: all sequences have `tokens` tokens
+    const int32_t *slots;               // state of each sequence, or null: the n-th
+    int64_t state_count;                // number of states behind `slots`
+    int64_t sequences, tokens;          // tokens: with offsets, the number of rows
+    int64_t segment;                    // tokens of a segment, a multiple of every kernel's chunk
+    int64_t items;                      // upper bound of the number of segments of all sequences
+    int *bad_index;
+    int *wait_flag;
+};
+
+struct SegmentItem
+{
+    int64_t begin, end;                 // tokens of the sequence (of all rows when packed)
+    int64_t sequence;                   // -1: no such item, or a sequence that is not there
+    int64_t first_item;                 // the sequence's first item
+    int64_t sequence_begin, sequence_end;
+    int64_t state;                      // which of the user's states
+    int32_t last;                       // is this the sequence's last item in the order of time?
+    int32_t first;
+};
+
+__device__ __forceinline__ int64_t segments_of(int64_t length, int64_t segment) { return length <= segment ? 1 : (length + segment - 1) / segment; }
+
+// Rows [*begin, *end) of a packed sequence.  Offsets that decrease or leave the arrays are cut back (and reported): no access
+// ever leaves the rows.
+__device__ __forceinline__ void packed_range(const AttentionArgs &a, int64_t n, int64_t *begin, int64_t *end)
+{
+    const int64_t b = a.offsets[n], e = a.offsets[n + 1];
+    int64_t lo = b < 0 ? 0 : b > a.tokens ? a.tokens : b;
+    int64_t hi = e < lo ? lo : e > a.tokens ? a.tokens : e;
+    if (lo != b || hi != e) atomicOr(a.bad_index, 1);
+    *begin = lo;
+    *end = hi;
+}
+
+// Which state belongs to entry n of `slots`: -1 when the entry is negative (a request that is not there), out of range or the
+// same as an earlier entry (both reported).  Every thread of the CTA calls it; holds a CTA barrier.
+__device__ __forceinline__ int64_t state_of(const int32_t *slots, int64_t n, int64_t count, int *bad_index)
+{
+    if (slots == nullptr) return n;
+    const int32_t mine = slots[n];
+    bool twice = false;
+    if (mine >= 0)
+        for (int64_t i = threadIdx.x; i < n; i += blockDim.x) twice |= slots[i] == mine;
+    twice = __syncthreads_or(twice) != 0;
+    if (mine < 0) return -1;
+    if (twice || mine >= count)
+    {
+        if (threadIdx.x == 0) atomicOr(bad_index, 1);
+        return -1;
+    }
+    return mine;
+}
+
+// Item `item` of the list of all sequences' segments (in natural order).  Every thread of the CTA (at most 1024, whole warps)
+// calls it and gets the same answer; holds CTA barriers.
+__device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t item, bool reverse)
+{
+    SegmentItem s;
+    if (a.offsets == nullptr)
+    {
+        const int64_t each = segments_of(a.tokens, a.segment);
+        s.sequence = item / each;
+        s.first_item = s.sequence * each;
+        s.sequence_begin = 0;
+        s.sequence_end = a.tokens;
+    }
+    else
+    {
+        __shared__ int64_t found[4], warp_sums[33];
+        if (threadIdx.x == 0) found[0] = -1;
+        int64_t before = 0;
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+        for (int64_t base = 0; base < a.sequences; base += blockDim.x)
+        {
+            const int64_t n = base + threadIdx.x;
+            int64_t b = 0, e = 0, mine = 0;
+            if (n < a.sequences)
+            {
+                packed_range(a, n, &b, &e);
+                mine = segments_of(e - b, a.segment);
+            }
+            int64_t sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1)
+            {
+                const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += up;
+            }
+            __syncthreads();
+            if (lane == 31) warp_sums[warp] = sum;
+            __syncthreads();
+            int64_t total = 0, ahead = 0;
+            for (int w = 0; w < warps; ++w)
+            {
+                if (w == warp) ahead = total;
+                total += warp_sums[w];
+            }
+            const int64_t start = before + ahead + sum - mine;
+            if (mine > 0 && item >= start && item < start + mine)
+            {
+                found[0] = n;
+                found[1] = start;
+                found[2] = b;
+                found[3] = e;
+            }
+            before += total;
+            if (item < before) break;       // the same for every thread
+        }
+        __syncthreads();
+        s.sequence = found[0];
+        s.first_item = found[1];
+        s.sequence_begin = found[2];
+        s.sequence_end = found[3];
+    }
+    if (s.sequence < 0) return s;
+    s.state = state_of(a.slots, s.sequence, a.state_count, a.bad_index);
+    if (s.state < 0)
+    {
+        s.sequence = -1;
+        return s;
+    }
+    const int64_t index = item - s.first_item, count = segments_of(s.sequence_end - s.sequence_begin, a.segment);
+    s.begin = s.sequence_begin + index * a.segment;
+    s.end = s.begin + a.segment < s.sequence_end ? s.begin + a.segment : s.sequence_end;
+    s.first = reverse ? index == count - 1 : index == 0;
+    s.last = reverse ? index == 0 : index == count - 1;
+    return s;
+}
+
+template <class T>
+__device__ __forceinline__ T *rows_of(const TokenRows &r, const AttentionArgs &a, int64_t sequence, int head)
+{
+    return static_cast<T *>(r.data) + (a.offsets == nullptr ? sequence * r.sequence : 0) + static_cast<int64_t>(head / r.group) * r.head;
+}
+
+// The logarithm of a head's decay.  A decay of zero (-inf) becomes one so small that every power but the zeroth is zero.
+template <class A>
+__device__ __forceinline__ A decay_log(const void *log_decay, int head)
+{
+    const A g = static_cast<const A *>(log_decay)[head];
+    return g < A(-1e5) ? A(-1e5) : g;
+}
+
+}
+
+#endif

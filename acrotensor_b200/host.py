@@ -392,6 +392,32 @@ class TensorEngine:
         else:
             check(lib().acro_engine_flat_indexed_sum_gather_shared(self._h, Aout._h, Ain._h, M._h, shared._h))
 
+    @staticmethod
+    def _optional(t):
+        return t._h if t is not None else None
+
+    def LinearAttention(self, Out, Q, K, V, LogDecay, scale, InitialState=None, FinalState=None):
+        """Linear attention with a decay for each head on fp64 tensors (acro::TensorEngine::LinearAttention); see
+        :func:`acrotensor_b200.linear_attention` for narrower types and packed sequences."""
+        check(lib().acro_engine_linear_attention(self._h, Out._h, Q._h, K._h, V._h, LogDecay._h, float(scale), self._optional(InitialState),
+                                                 self._optional(FinalState)))
+
+    def LinearAttentionStep(self, Out, StateOut, Q, K, V, LogDecay, StateIn, scale):
+        check(lib().acro_engine_linear_attention_step(self._h, Out._h, StateOut._h, Q._h, K._h, V._h, LogDecay._h, StateIn._h, float(scale)))
+
+    def LinearAttentionBackward(self, dQ, dK, dV, dOut, Q, K, V, LogDecay, scale, InitialState=None, dFinalState=None, dInitialState=None):
+        check(lib().acro_engine_linear_attention_backward(self._h, dQ._h, dK._h, dV._h, dOut._h, Q._h, K._h, V._h, LogDecay._h, float(scale),
+                                                          self._optional(InitialState), self._optional(dFinalState),
+                                                          self._optional(dInitialState)))
+
+    def LayerNorm(self, Y, X, Weight=None, Bias=None, eps=1e-5, Mean=None, Rstd=None):
+        check(lib().acro_engine_layer_norm(self._h, Y._h, X._h, self._optional(Weight), self._optional(Bias), float(eps), self._optional(Mean),
+                                           self._optional(Rstd)))
+
+    def LayerNormBackward(self, dX, dWeight, dBias, dY, X, Mean, Rstd, Weight=None):
+        check(lib().acro_engine_layer_norm_backward(self._h, dX._h, self._optional(dWeight), self._optional(dBias), dY._h, X._h, Mean._h,
+                                                    Rstd._h, self._optional(Weight)))
+
     def Clear(self):
         check(lib().acro_engine_clear(self._h))
 

@@ -86,6 +86,21 @@ class TensorEngine
     // (an acro_b200_halo, see acro_b200.h, or a SharedEntryExchange).  Collective over the ranks.
     void FlatIndexedSumGather(Tensor &Aout, Tensor &Ain, IndexMapping &M, void *halo);
 
+    // Sequence operators (no counterpart in the reference; acro_b200.h has the formulas and the forms for narrower types and packed
+    // sequences).  Q is [tokens][heads][dk] or [sequences][tokens][heads][dk], K and V the same with a number of heads that
+    // divides Q's, Out like V with Q's heads, LogDecay [heads], states [heads][dk][dv] or [sequences][heads][dk][dv].
+    void LinearAttention(Tensor &Out, Tensor &Q, Tensor &K, Tensor &V, Tensor &LogDecay, double scale, Tensor *InitialState = nullptr,
+                         Tensor *FinalState = nullptr);
+    // One token of each request: Q [requests][heads][dk], states [requests][heads][dk][dv]; StateOut may be StateIn.
+    void LinearAttentionStep(Tensor &Out, Tensor &StateOut, Tensor &Q, Tensor &K, Tensor &V, Tensor &LogDecay, Tensor &StateIn, double scale);
+    void LinearAttentionBackward(Tensor &dQ, Tensor &dK, Tensor &dV, Tensor &dOut, Tensor &Q, Tensor &K, Tensor &V, Tensor &LogDecay, double scale,
+                                 Tensor *InitialState = nullptr, Tensor *dFinalState = nullptr, Tensor *dInitialState = nullptr);
+    // Norm over the last dimension of X; Weight and Bias [width], Mean and Rstd [all entries / width].
+    void LayerNorm(Tensor &Y, Tensor &X, Tensor *Weight, Tensor *Bias, double eps, Tensor *Mean = nullptr, Tensor *Rstd = nullptr);
+    // dWeight and dBias are sums over the leading indices: with a peer group attached and X flagged sharded they are summed over
+    // the ranks, as contractions over a sharded index are.
+    void LayerNormBackward(Tensor &dX, Tensor *dWeight, Tensor *dBias, Tensor &dY, Tensor &X, Tensor &Mean, Tensor &Rstd, Tensor *Weight);
+
     void Clear();
     bool IsGPUAvailable() { return isCudaReady(); }
 

@@ -61,6 +61,7 @@ int acro_b200_device_count(void);
 
 /* Waits for the current device to go idle and reports ACRO_B200_ETIMEOUT if, since the last
  * call, a kernel's bounded wait on an asynchronous copy gave up (its results are invalid),
+ * ACRO_B200_EINVAL if a sequence operator met an index that is out of range or repeated,
  * ACRO_B200_ECUDA on a CUDA failure, else ACRO_B200_OK.  Plays the role of the reference's
  * acroCudaErrorCheck after a launch (util/CudaUtil.hpp:59-89). */
 int acro_b200_device_status(void);
@@ -388,6 +389,91 @@ int acro_b200_halo_combine(acro_b200_halo *halo, double *values, void *stream);
 int acro_b200_halo_exchange_sum(acro_b200_halo *halo, double *values, void *stream);
 int acro_b200_halo_destroy(acro_b200_halo *halo);
 
+/*
+ * Sequence operators: what a layer over token sequences needs beside its contractions.  No counterpart in the reference.
+ * Element types: 64, 32 and 16 bits.  Sums, states, decays and row statistics are in 32 bits (64 for ACRO_B200_F64): the
+ * "type of sums" below.  All pointers are device memory of the current device; memory of another device is refused.
+ * Entries of index arrays are read on the device only: one that is out of range or repeated is skipped, nothing outside the
+ * arrays is touched, and acro_b200_device_status() reports ACRO_B200_EINVAL.
+ */
+#define ACRO_B200_F64 0
+#define ACRO_B200_F32 1
+#define ACRO_B200_BF16 2
+#define ACRO_B200_F16 3
+
+/* Rows of heads: element (sequence n, token t, head h, column c) is at data[n * sequence_stride + t * token_stride + h * head_stride + c]
+ * (strides in elements; columns are contiguous, rows do not overlap).  With packed sequences (`offsets`) t counts over all rows. */
+typedef struct acro_b200_token_array
+{
+    void *data;
+    int64_t sequence_stride, token_stride, head_stride;
+} acro_b200_token_array;
+
+typedef struct acro_b200_linear_attention_desc
+{
+    int32_t type;               /* ACRO_B200_F64 ... ACRO_B200_F16, of q, k, v, out and their gradients */
+    int32_t q_heads, kv_heads;  /* q_heads a multiple of kv_heads; query head h reads key and value head h / (q_heads / kv_heads) */
+    int32_t dk, dv;             /* columns of q and k, of v and out: 1 .. 256 */
+    int32_t reserved;
+    int64_t sequences;
+    int64_t tokens;             /* of every sequence; with `offsets` the number of rows of the arrays */
+    double scale;
+} acro_b200_linear_attention_desc;
+
+/*
+ * linear_attention:  per sequence and query head, with lam = exp(log_decay[head]) and states S [dk][dv] in the type of sums,
+ *     S_t = lam S_(t-1) + k_t v_t^T,     out_t = scale q_t^T S_t,
+ * a Gram form that forgets, chained with a product.  Computed in chunks of tokens (the tokens of a chunk against one another,
+ * the earlier ones through the state), long sequences cut into segments when there are few heads.
+ *   log_decay      q_heads values of the type of sums; 0 never forgets, -infinity keeps the token itself only
+ *   offsets        NULL, or sequences + 1 ascending row numbers: sequence n has the rows offsets[n] .. offsets[n+1]-1.  Rows that belong
+ *                  to no sequence are neither read nor written.  A sequence may be empty: its final state is its initial state.
+ *   initial_state  NULL (zero), or states [state_count][q_heads][dk][dv], contiguous; final_state NULL or the same, and may be the same memory
+ *   slots          NULL (state n belongs to sequence n, state_count = sequences), or the state of each sequence.  A negative slot marks
+ *                  a sequence that is not there: its rows and states are left as they were.
+ *   scratch        acro_b200_linear_attention_scratch_bytes(desc, packed) bytes (0 is possible), 16-byte aligned; calls that share
+ *                  it must not overlap on the device.
+ * out must not be q, k or v.  No host synchronisation; may be captured.
+ */
+size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed);
+int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
+                               const acro_b200_token_array *v, const acro_b200_token_array *out, const void *log_decay, const int64_t *offsets,
+                               const void *initial_state, void *final_state, const int32_t *slots, int64_t state_count, void *scratch, size_t scratch_bytes,
+                               void *stream);
+/* One token of each of desc->sequences requests (desc->tokens = 1): state_out[slot] = lam state_in[slot] + k v^T,
+ * out = scale q^T state_out[slot].  state_out may be state_in.  Request n is sequence n of the arrays. */
+int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
+                                    const acro_b200_token_array *v, const acro_b200_token_array *out, const void *log_decay, const void *state_in,
+                                    void *state_out, const int32_t *slots, int64_t state_count, void *stream);
+/* Gradients for dout (and d_final_state, NULL: zero) with respect to q, k, v and the initial state (d_initial_state, may be NULL):
+ *     dq_t = scale S_t dout_t,  dk_t = G_t v_t,  dv_t = G_t^T k_t,  G_t = lam G_(t+1) + scale q_t dout_t^T,  lam G_T := d_final_state,
+ * d_initial_state = lam G_0.  States are [sequences][q_heads][dk][dv].  The gradients of shared key and value heads are summed over
+ * their query heads in ascending order.  The decays are constants of the layer: they get no gradient.  Fixed summation orders: the
+ * same bits on every run on one device. */
+size_t acro_b200_linear_attention_backward_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed);
+int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
+                                        const acro_b200_token_array *v, const acro_b200_token_array *dout, const void *log_decay, const int64_t *offsets,
+                                        const void *initial_state, const void *d_final_state, const acro_b200_token_array *dq,
+                                        const acro_b200_token_array *dk, const acro_b200_token_array *dv, void *d_initial_state, void *scratch,
+                                        size_t scratch_bytes, void *stream);
+
+/*
+ * layer_norm:  y = (x - mean) rstd weight + bias per row of `width` entries, mean and rstd = 1/sqrt(variance + eps) of the row (type of
+ * sums; written to mean and rstd unless these are NULL).  weight and bias are of the element type and may be NULL.  Row strides in
+ * elements; y may be x.
+ */
+int acro_b200_layer_norm(int type, const void *x, int64_t x_stride, const void *weight, const void *bias, void *y, int64_t y_stride, void *mean,
+                         void *rstd, int64_t rows, int64_t width, double eps, void *stream);
+/* Gradients for dy: with xhat = (x - mean) rstd and g = dy weight,
+ *     dx = rstd (g - sum(g)/width - xhat sum(g xhat)/width),  dweight = sum over the rows of dy xhat,  dbias = sum over the rows of dy
+ * (the column sums are what reduce_batch computes for one operand; here they leave with the same walk over the rows).  dweight
+ * and dbias are of the type of sums, may be NULL; without both, scratch may be NULL.  dx may be dy or x up to a width of 16384.
+ * Fixed summation orders: the same bits on every run on one device. */
+size_t acro_b200_layer_norm_backward_scratch_bytes(int type, int64_t rows, int64_t width);
+int acro_b200_layer_norm_backward(int type, const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const void *weight, const void *mean,
+                                  const void *rstd, void *dx, int64_t dx_stride, void *dweight, void *dbias, int64_t rows, int64_t width, void *scratch,
+                                  size_t scratch_bytes, void *stream);
+
 /* ---------------------------------------------------------------- engine layer */
 
 typedef struct acro_tensor acro_tensor;   /* an acro::Tensor */
@@ -478,9 +564,25 @@ int acro_engine_flat_indexed_sum_gather(acro_engine *e, acro_tensor *Aout, acro_
 int acro_engine_flat_indexed_sum_gather_shared(acro_engine *e, acro_tensor *Aout, acro_tensor *Ain, acro_index_mapping *m,
                                                acro_b200_halo *halo);
 
+/* LinearAttention, LinearAttentionStep, LinearAttentionBackward, LayerNorm and LayerNormBackward of acro::TensorEngine on fp64 tensors
+ * (include/TensorEngine.hpp; no counterpart in the reference).  States, weight, bias, mean, rstd, dweight and dbias may be NULL where
+ * the C++ methods take pointers. */
+int acro_engine_linear_attention(acro_engine *e, acro_tensor *out, acro_tensor *q, acro_tensor *k, acro_tensor *v, acro_tensor *log_decay, double scale,
+                                 acro_tensor *initial_state, acro_tensor *final_state);
+int acro_engine_linear_attention_step(acro_engine *e, acro_tensor *out, acro_tensor *state_out, acro_tensor *q, acro_tensor *k, acro_tensor *v,
+                                      acro_tensor *log_decay, acro_tensor *state_in, double scale);
+int acro_engine_linear_attention_backward(acro_engine *e, acro_tensor *dq, acro_tensor *dk, acro_tensor *dv, acro_tensor *dout, acro_tensor *q,
+                                          acro_tensor *k, acro_tensor *v, acro_tensor *log_decay, double scale, acro_tensor *initial_state,
+                                          acro_tensor *d_final_state, acro_tensor *d_initial_state);
+int acro_engine_layer_norm(acro_engine *e, acro_tensor *y, acro_tensor *x, acro_tensor *weight, acro_tensor *bias, double eps, acro_tensor *mean,
+                           acro_tensor *rstd);
+int acro_engine_layer_norm_backward(acro_engine *e, acro_tensor *dx, acro_tensor *dweight, acro_tensor *dbias, acro_tensor *dy, acro_tensor *x,
+                                    acro_tensor *mean, acro_tensor *rstd, acro_tensor *weight);
+
 /* Stream used by the calling host thread's tensor copies / fills and by engines without their
  * own stream (per thread; NULL = legacy default stream). */
 int acro_b200_set_stream(void *stream);
+void *acro_b200_get_stream(void);
 
 /* Host-only introspection (no device needed): a text dump of the parser's view of a
  * kernel string — variables, AllIndexNames, ContractionIndexNames
