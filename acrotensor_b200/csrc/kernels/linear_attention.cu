@@ -528,7 +528,9 @@ int run_pass_of(int type, const AttentionArgs &a, bool states_only, cudaStream_t
     {
     case ACRO_B200_F64: return run_pass<double>(a, states_only, stream);
     case ACRO_B200_F32: return run_pass<float>(a, states_only, stream);
-    case ACRO_B200_BF16: return run_pass<__nv_bfloat16>(a, states_only, stream);
+    case ACRO_B200_BF16:
+        if (attention_mma_supported(a)) return attention_mma_launch(a, states_only, stream);
+        return run_pass<__nv_bfloat16>(a, states_only, stream);
     default: return run_pass<__half>(a, states_only, stream);
     }
 }

@@ -194,6 +194,10 @@ __device__ __forceinline__ A decay_log(const void *log_decay, int head)
     return g < A(-1e5) ? A(-1e5) : g;
 }
 
+// The pass on the tcgen05 tensor cores for bf16 (linear_attention_mma.cu), for operands that tiled copies can read.
+bool attention_mma_supported(const AttentionArgs &a);
+int attention_mma_launch(const AttentionArgs &a, bool states_only, cudaStream_t stream);
+
 }
 
 #endif

@@ -1,0 +1,550 @@
+// Linear attention's pass on the tcgen05 tensor cores, for bf16 operands of up to 128 columns.
+//
+// A CTA walks one segment of one head in chunks of 64 tokens (r, s: tokens of the chunk; a: columns of q and k; b: of v):
+//   scores  P[r][s]     = Q[r][a] K[s][a]                            M = r (64 of 128 lanes used)
+//   near    O'[b][r]    = V[s][b] P~[r][s]                           P~: scores times powers of the decay, zero where masked
+//   far     O"[b][r]    = S[b][a] Q[r][a]                            S: the state before the chunk, A operand in tensor memory
+//   change  D[b][a]     = V[s][b] K~[s][a]                           K~: rows of K times what the decay leaves of them
+//   out[r][b] = out_scale (O' + come_r O"),   S <- lam^m S + state_scale D
+// The transposed forms put b on the 128 lanes: the state stays in registers (fp32), one row of S^T per thread and half its columns,
+// and becomes an A operand by a store into tensor memory, without a way through shared memory.
+//
+// Precision: accumulators and the state are fp32.  The operands that are not inputs are sums of bf16 parts: P~ and S two parts (an
+// error of 2^-18 of an entry, 2^-9 of what the result's own rounding to bf16 loses), K~ three (2^-26), because the final state is an
+// fp32 result and collects every chunk's change.
+//
+// Bound: by HBM 128 KB a chunk at 128 columns, about 2850 cycles of an SM at its share of 6.5 TB/s; the products take 1800 cycles of
+// the tensor pipe, the conversions about 2000 issue slots of the four schedulers, shared memory (operands of the products included)
+// about 2600 cycles.  So the roles overlap: one warp issues copies and products, eight warps convert.
+#include "linear_attention.cuh"
+#include "umma.cuh"
+
+#include <algorithm>
+#include <cuda.h>
+
+using namespace acro_b200_detail;
+
+namespace
+{
+
+constexpr int kChunk = 64;
+constexpr int kBox = kChunk * 128;          // bytes of 64 rows of 64 columns
+constexpr int kWorkers = 256;               // threads that convert: warps 0 .. 7; warp 8 issues
+constexpr int kBlock = kWorkers + 32;
+constexpr int kRing = 4;                    // slots of the flags that tell of non-finite values
+
+// Columns of tensor memory.
+constexpr uint32_t kScores = 0, kNear = 64, kFar = 128, kDelta = 192, kStateHigh = 320, kStateLow = 384, kColumns = 512;
+
+struct Maps { CUtensorMap q[3], k[3], v[3]; };
+
+template <int NQ, int NV>
+struct Layout
+{
+    static constexpr int kStages = NQ == 2 ? 3 : 4;
+    static constexpr int kQ = 0, kK = NQ * kBox, kV = 2 * NQ * kBox, kStage = (2 * NQ + NV) * kBox;
+    static constexpr int kScaled = kStages * kStage;            // K~, three parts
+    static constexpr int kWeights = kScaled + 3 * NQ * kBox;    // P~, two parts
+    static constexpr int kTables = kWeights + 2 * kBox;
+    static constexpr int kBytes = kTables + 2048;
+    // a first product of M = 128 reads 64 rows behind a box: they lie inside the allocation
+    static constexpr int kDynamic = kBytes + 1024;              // the base is rounded up to 1024
+};
+
+struct Shared
+{
+    float power[kChunk + 1];
+    int odd[kRing];
+    uint32_t tmem;
+    uint64_t full[4], scores, scaled, weights, state, out, out_free, change, drained;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float low, float high)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    return r;
+}
+__device__ __forceinline__ float low_of(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high_of(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// What a bf16 part leaves of x; nothing of an infinity.
+__device__ __forceinline__ float left_over(float x, float part)
+{
+    const float d = x - part;
+    return fabsf(part) == __int_as_float(0x7f800000) ? 0.0f : d;
+}
+
+__device__ __forceinline__ bool odd_half(uint32_t x) { return (x & 0x7f80u) == 0x7f80u; }
+__device__ __forceinline__ bool odd_pair(uint32_t x) { return odd_half(x) || odd_half(x >> 16); }
+// The pair with zeros in the place of infinities and NaN.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t x) { return (odd_half(x) ? 0u : x & 0xffffu) | (odd_half(x >> 16) ? 0u : x & 0xffff0000u); }
+
+__device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+
+template <int NQ, int NV>
+__global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ Maps maps, bool states_only)
+{
+    using L = Layout<NQ, NV>;
+    constexpr int HALF = NQ * 32;               // columns of the state per thread
+    const int pass = blockIdx.y;
+    const AttentionPass &p = a.pass[pass];
+    const int head = blockIdx.x % a.heads;
+    const int64_t item_index = blockIdx.x / a.heads;
+    const bool reverse = p.reverse != 0;
+    const SegmentItem item = find_item(a, item_index, reverse);
+    if (item.sequence < 0) return;
+    const bool cut = segments_of(item.sequence_end - item.sequence_begin, a.segment) > 1;
+    if (states_only && (!cut || item.last)) return;
+
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    Shared &sh = *reinterpret_cast<Shared *>(smem + L::kTables);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    const double g = decay_log<float>(a.log_decay, head);
+    for (int i = threadIdx.x; i <= kChunk; i += kBlock) sh.power[i] = static_cast<float>(exp(g * i));
+    if (threadIdx.x < kRing) sh.odd[threadIdx.x] = 0;
+    if (threadIdx.x == 0)
+    {
+        for (int i = 0; i < L::kStages; ++i) mbar_init(&sh.full[i], 1);
+        mbar_init(&sh.scores, 1);
+        mbar_init(&sh.out, 1);
+        mbar_init(&sh.change, 1);
+        mbar_init(&sh.drained, 1);
+        mbar_init(&sh.scaled, kWorkers);
+        mbar_init(&sh.weights, kWorkers / 2);
+        mbar_init(&sh.state, kWorkers);
+        mbar_init(&sh.out_free, kWorkers);
+        fence_mbar_init();
+    }
+    if (warp == 8) tmem_alloc(&sh.tmem, kColumns);
+    tmem_fence_before_sync();
+    __syncthreads();
+    tmem_fence_after_sync();
+    const uint32_t tmem = sh.tmem;
+    const int64_t length = item.end - item.begin;
+    const int chunks = static_cast<int>((length + kChunk - 1) / kChunk);
+    const auto chunk_of = [&](int c) { return reverse ? chunks - 1 - c : c; };
+    bool ok = true;
+
+    if (warp == 8)
+    {
+        if (lane == 0)
+        {
+            const int stage_bytes = states_only ? (NQ + NV) * kBox : L::kStage;
+            const int hq = head / p.q.group, hk = head / p.k.group, hv = head / p.v.group, n = a.offsets == nullptr ? static_cast<int>(item.sequence) : 0;
+            const auto load = [&](int c) {
+                unsigned char *stage = smem + c % L::kStages * L::kStage;
+                uint64_t *bar = &sh.full[c % L::kStages];
+                const int t = static_cast<int>(item.begin + static_cast<int64_t>(chunk_of(c)) * kChunk);
+                mbar_arrive_expect_tx(bar, stage_bytes);
+                for (int i = 0; i < NQ; ++i)
+                {
+                    if (!states_only) box_load(stage + L::kQ + i * kBox, &maps.q[pass], i * kBoxColumns, hq, t, n, bar);
+                    box_load(stage + L::kK + i * kBox, &maps.k[pass], i * kBoxColumns, hk, t, n, bar);
+                }
+                for (int i = 0; i < NV; ++i) box_load(stage + L::kV + i * kBox, &maps.v[pass], i * kBoxColumns, hv, t, n, bar);
+            };
+            int loaded = 0;
+            for (; loaded < min(chunks, L::kStages - 1); ++loaded) load(loaded);
+            const uint32_t base = smem_addr(smem);
+            const int steps = (p.dq + 15) / 16;
+            const uint32_t by_columns = umma_shape(kChunk, false, false), near_shape = umma_shape(kChunk, true, false),
+                           change_shape = umma_shape((p.dq + 15) / 16 * 16, true, true);
+            int c = 0;
+            for (; c < chunks && ok; ++c)
+            {
+                const uint32_t stage = base + c % L::kStages * L::kStage, parity = c & 1;
+                ok = mbar_wait(&sh.full[c % L::kStages], c / L::kStages & 1);
+                if (!ok) break;
+                if (!states_only)
+                {
+                    // the score columns are free: the previous chunk's weights were waited for
+                    for (int k = 0; k < steps; ++k)
+                    {
+                        const uint32_t at = k / 4 * kBox + k % 4 * 32;
+                        umma(tmem + kScores, umma_operand(stage + L::kQ + at, 16, 1024), umma_operand(stage + L::kK + at, 16, 1024), by_columns, k > 0);
+                    }
+                    umma_commit(&sh.scores);
+                }
+                // the stage of the previous chunk takes the chunk kStages - 1 ahead once its products are complete and its readers done
+                if (c > 0)
+                {
+                    ok = mbar_wait(&sh.change, parity ^ 1) && (states_only || mbar_wait(&sh.out_free, parity ^ 1));
+                    if (!ok) break;
+                }
+                if (loaded < chunks) load(loaded++);
+                if (!states_only)
+                {
+                    ok = mbar_wait(&sh.state, parity);
+                    if (!ok) break;
+                    tmem_fence_after_sync();
+                    for (int part = 0; part < 2; ++part)
+                        for (int k = 0; k < steps; ++k)
+                            umma_tmem(tmem + kFar, tmem + (part ? kStateLow : kStateHigh) + k * 8,
+                                      umma_operand(stage + L::kQ + k / 4 * kBox + k % 4 * 32, 16, 1024), by_columns, part + k > 0);
+                }
+                ok = mbar_wait(&sh.scaled, parity);
+                if (!ok) break;
+                tmem_fence_after_sync();
+                for (int part = 0; part < 3; ++part)
+                    for (int k = 0; k < kChunk / 16; ++k)
+                        umma(tmem + kDelta, umma_operand(stage + L::kV + k * 2048, NV == 2 ? kBox : 0, 1024),
+                             umma_operand(base + L::kScaled + part * NQ * kBox + k * 2048, kBox, 1024), change_shape, part + k > 0);
+                umma_commit(&sh.change);
+                if (states_only) continue;
+                ok = mbar_wait(&sh.weights, parity);
+                if (!ok) break;
+                tmem_fence_after_sync();
+                for (int part = 0; part < 2; ++part)
+                    for (int k = 0; k < kChunk / 16; ++k)
+                        umma(tmem + kNear, umma_operand(stage + L::kV + k * 2048, NV == 2 ? kBox : 0, 1024),
+                             umma_operand(base + L::kWeights + part * kBox + k * 32, 16, 1024), near_shape, part + k > 0);
+                umma_commit(&sh.out);
+            }
+            if (!ok)
+            {
+                *a.wait_flag = 1;
+                // copies and products of this CTA that are still in flight
+                for (int i = c; i < loaded; ++i) mbar_wait(&sh.full[i % L::kStages], i / L::kStages & 1);
+                umma_commit(&sh.drained);
+                mbar_wait(&sh.drained, 0);
+            }
+        }
+        __syncwarp();
+    }
+    else
+    {
+        // this thread's row of the transposed state, and which half of its columns
+        const int b = warp % 4 * 32 + lane, half = warp / 4;
+        const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+        const bool used = b < p.dv;
+        float s[HALF];
+        const int64_t size = static_cast<int64_t>(p.dq) * p.dv;
+        {
+            const float *from = nullptr;
+            int turned = 0;
+            if (!states_only)
+            {
+                if (cut) from = static_cast<const float *>(p.segment_states) + (item_index * a.heads + head) * size;
+                else if (p.initial != nullptr)
+                {
+                    from = static_cast<const float *>(p.initial) + (item.state * a.heads + head) * size;
+                    turned = p.turned;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < HALF; ++j)
+            {
+                const int d = half * HALF + j;
+                s[j] = from != nullptr && used && d < p.dq ? (turned ? from[b * p.dq + d] : from[static_cast<int64_t>(d) * p.dv + b]) : 0.0f;
+            }
+        }
+        const auto publish = [&]() {
+            // the state as the A operand of the next chunk: two bf16 parts, pairs of columns
+#pragma unroll
+            for (int j = 0; j < HALF; j += 32)
+            {
+                uint32_t high[16], low[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                {
+                    const float x = s[j + 2 * i], y = s[j + 2 * i + 1];
+                    high[i] = pack_bf16(x, y);
+                    low[i] = pack_bf16(left_over(x, low_of(high[i])), left_over(y, high_of(high[i])));
+                }
+                const uint32_t at = lanes + (half * HALF + j) / 2;
+                tmem_store_16(tmem + kStateHigh + at, high);
+                tmem_store_16(tmem + kStateLow + at, low);
+            }
+            tmem_wait_stores();
+            tmem_fence_before_sync();
+            mbar_arrive(&sh.state);
+        };
+        if (!states_only) publish();
+        const float state_scale = static_cast<float>(p.state_scale), out_scale = static_cast<float>(p.out_scale);
+        const __nv_bfloat16 *k = rows_of<const __nv_bfloat16>(p.k, a, item.sequence, head), *v = rows_of<const __nv_bfloat16>(p.v, a, item.sequence, head);
+        float keep = 1, rest = 0;
+        int kept = 0;
+        float *sums = rows_of<float>(p.out, a, item.sequence, head);
+        __nv_bfloat16 *out = rows_of<__nv_bfloat16>(p.out, a, item.sequence, head);
+
+        for (int c = 0; c < chunks; ++c)
+        {
+            unsigned char *stage = smem + c % L::kStages * L::kStage;
+            const uint32_t parity = c & 1;
+            const int64_t t0 = item.begin + static_cast<int64_t>(chunk_of(c)) * kChunk;
+            const int m = static_cast<int>(min(static_cast<int64_t>(kChunk), item.end - t0));
+            ok = all_wait(&sh.full[c % L::kStages], c / L::kStages & 1);
+            if (!ok) break;
+            // K~; rows behind the chunk's last token are zeros in K~ and V.  Infinities and NaN of V become zeros too, because a masked
+            // weight times one of them would be NaN: where there are any, the rows and states that they do meet get them below.
+            if (threadIdx.x == 0) sh.odd[(c + 2) % kRing] = 0;
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < NQ * 2; ++i)
+            {
+                const int piece = i * kWorkers + threadIdx.x, r = piece / 8 % kChunk;
+                const uint4 x = *reinterpret_cast<const uint4 *>(stage + L::kK + piece * 16);
+                const float w = r < m ? sh.power[reverse ? r + 1 : m - 1 - r] : 0.0f;
+                const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                uint32_t part[3][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    float lo = r < m ? low_of(in[j]) * w : 0.0f, hi = r < m ? high_of(in[j]) * w : 0.0f;
+                    part[0][j] = pack_bf16(lo, hi);
+                    lo = left_over(lo, low_of(part[0][j]));
+                    hi = left_over(hi, high_of(part[0][j]));
+                    part[1][j] = pack_bf16(lo, hi);
+                    part[2][j] = pack_bf16(lo - low_of(part[1][j]), hi - high_of(part[1][j]));
+                }
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    *reinterpret_cast<uint4 *>(smem + L::kScaled + k * NQ * kBox + piece * 16) = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < NV * 2; ++i)
+            {
+                const int piece = i * kWorkers + threadIdx.x, r = piece / 8 % kChunk;
+                uint4 *x = reinterpret_cast<uint4 *>(stage + L::kV + piece * 16);
+                if (r >= m) *x = make_uint4(0, 0, 0, 0);
+                else if (odd_pair(x->x) | odd_pair(x->y) | odd_pair(x->z) | odd_pair(x->w))
+                {
+                    *x = make_uint4(finite_pair(x->x), finite_pair(x->y), finite_pair(x->z), finite_pair(x->w));
+                    odd = true;
+                }
+            }
+            if (odd) sh.odd[c % kRing] = 1;
+            fence_proxy_async();
+            mbar_arrive(&sh.scaled);
+
+            if (!states_only)
+            {
+                if (warp % 4 < 2)
+                {
+                    ok = all_wait(&sh.scores, parity);
+                    if (!ok) break;
+                    tmem_fence_after_sync();
+                    const int r = b;
+                    uint32_t x[32];
+                    tmem_load_32(tmem + kScores + lanes + half * 32, x);
+                    const int last = reverse ? m - 1 : r, first = reverse ? r : 0;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                    {
+                        uint32_t high[4], low[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                        {
+                            float y[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                            {
+                                const int col = half * 32 + j + 2 * i + e;
+                                y[e] = col >= first && col <= last ? __uint_as_float(x[j + 2 * i + e]) * (sh.power[abs(r - col)] * state_scale) : 0.0f;
+                            }
+                            high[i] = pack_bf16(y[0], y[1]);
+                            low[i] = pack_bf16(left_over(y[0], low_of(high[i])), left_over(y[1], high_of(high[i])));
+                        }
+                        const int at = r * 128 + ((half * 4 + j / 8) ^ (r & 7)) * 16;
+                        *reinterpret_cast<uint4 *>(smem + L::kWeights + at) = make_uint4(high[0], high[1], high[2], high[3]);
+                        *reinterpret_cast<uint4 *>(smem + L::kWeights + kBox + at) = make_uint4(low[0], low[1], low[2], low[3]);
+                    }
+                    tmem_fence_before_sync();
+                    fence_proxy_async();
+                    mbar_arrive(&sh.weights);
+                }
+            }
+
+            ok = all_wait(&sh.change, parity);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            if (m != kept)
+            {
+                // what is left of the state after m tokens, to twice the digits: the rounding of one factor would come back in every chunk
+                const double exact = exp(g * m);
+                keep = static_cast<float>(exact);
+                rest = static_cast<float>(exact - static_cast<double>(keep));
+                kept = m;
+            }
+#pragma unroll
+            for (int j = 0; j < HALF; j += 32)
+            {
+                uint32_t x[32];
+                tmem_load_32(tmem + kDelta + lanes + half * HALF + j, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) s[j + i] = fmaf(keep, s[j + i], fmaf(rest, s[j + i], state_scale * __uint_as_float(x[i])));
+            }
+            const bool any_odd = sh.odd[c % kRing] != 0;
+            if (any_odd && used)
+                for (int t = 0; t < m; ++t)
+                {
+                    const float x = __bfloat162float(v[(t0 + t) * p.v.token + b]);
+                    if (isfinite(x)) continue;
+                    const float left = sh.power[reverse ? t + 1 : m - 1 - t] * state_scale * x;
+                    const __nv_bfloat16 *row = k + (t0 + t) * p.k.token;
+#pragma unroll
+                    for (int j = 0; j < HALF; ++j)
+                        if (half * HALF + j < p.dq) s[j] += left * __bfloat162float(row[half * HALF + j]);
+                }
+            if (states_only)
+            {
+                tmem_fence_before_sync();
+                continue;
+            }
+            publish();
+
+            ok = all_wait(&sh.out, parity);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            uint32_t near[32], far[32];
+            tmem_load_32(tmem + kNear + lanes + half * 32, near);
+            tmem_load_32(tmem + kFar + lanes + half * 32, far);
+            tmem_fence_before_sync();
+            mbar_arrive(&sh.out_free);
+            if (any_odd)
+            {
+                if (used)
+                    for (int t = 0; t < m; ++t)
+                    {
+                        const float x = __bfloat162float(v[(t0 + t) * p.v.token + b]);
+                        if (isfinite(x)) continue;
+                        const __nv_bfloat16 *w = reinterpret_cast<const __nv_bfloat16 *>(smem + L::kWeights);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                        {
+                            const int r = half * 32 + i, at = r * 64 + ((t / 8) ^ (r & 7)) * 8 + t % 8;
+                            if (reverse ? t >= r : t <= r)
+                                near[i] = __float_as_uint(__uint_as_float(near[i]) + (__bfloat162float(w[at]) + __bfloat162float(w[kBox / 2 + at])) * x);
+                        }
+                    }
+                named_barrier(1, kWorkers);     // the next chunk's weights overwrite these
+            }
+            if (used)
+            {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                {
+                    const int r = half * 32 + i;
+                    if (r >= m) break;
+                    const float o = out_scale * (__uint_as_float(near[i]) + sh.power[reverse ? m - 1 - r : r + 1] * __uint_as_float(far[i]));
+                    if (p.sums) sums[(t0 + r) * p.out.token + b] = o;
+                    else out[(t0 + r) * p.out.token + b] = __float2bfloat16_rn(o);
+                }
+            }
+        }
+        if (!ok && lane == 0) *a.wait_flag = 1;
+        float *to = nullptr;
+        int turned = 0;
+        if (states_only) to = static_cast<float *>(p.segment_states) + (item_index * a.heads + head) * size;
+        else if (item.last && p.final != nullptr)
+        {
+            to = static_cast<float *>(p.final) + (item.state * a.heads + head) * size;
+            turned = p.turned;
+        }
+        if (to != nullptr && used)
+        {
+#pragma unroll
+            for (int j = 0; j < HALF; ++j)
+            {
+                const int d = half * HALF + j;
+                if (d < p.dq) to[turned ? b * p.dq + d : static_cast<int64_t>(d) * p.dv + b] = s[j];
+            }
+        }
+    }
+    tmem_fence_before_sync();
+    __syncthreads();
+    if (warp == 8) tmem_free(tmem, kColumns);
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder()
+{
+    static const EncodeTiled found = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &result) != cudaSuccess ||
+            result != cudaDriverEntryPointSuccess)
+        {
+            cudaGetLastError();
+            return static_cast<EncodeTiled>(nullptr);
+        }
+        return reinterpret_cast<EncodeTiled>(fn);
+    }();
+    return found;
+}
+
+// A distance of one entry of a dimension that has only one entry is never used: any valid one will do.
+bool stride_fits(int64_t stride, int64_t entries) { return entries <= 1 || (stride * 2 % 16 == 0 && stride > 0 && stride * 2 < (int64_t(1) << 40)); }
+
+int64_t heads_of(const AttentionArgs &a, const TokenRows &r) { return a.heads / r.group; }
+
+bool rows_fit(const AttentionArgs &a, const TokenRows &r)
+{
+    return aligned16(r.data) && stride_fits(r.head, heads_of(a, r)) && stride_fits(r.token, a.tokens) &&
+           (a.offsets != nullptr || stride_fits(r.sequence, a.sequences));
+}
+
+bool make_map(CUtensorMap *map, const AttentionArgs &a, const TokenRows &r, int columns)
+{
+    const bool packed = a.offsets != nullptr;
+    const int64_t heads = heads_of(a, r), sequences = packed ? 1 : a.sequences;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(a.tokens),
+                                static_cast<cuuint64_t>(sequences)};
+    const cuuint64_t strides[3] = {heads > 1 ? static_cast<cuuint64_t>(r.head) * 2 : 256, a.tokens > 1 ? static_cast<cuuint64_t>(r.token) * 2 : 256,
+                                   sequences > 1 ? static_cast<cuuint64_t>(r.sequence) * 2 : 256};
+    const cuuint32_t box[4] = {kBoxColumns, 1, kChunk, 1}, ones[4] = {1, 1, 1, 1};
+    return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, r.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NQ, int NV>
+int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStream_t stream)
+{
+    const char *name = "acro_b200_linear_attention";
+    cudaError_t status = cudaFuncSetAttribute(attention_mma_kernel<NQ, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<NQ, NV>::kDynamic);
+    if (status != cudaSuccess) return fail_cuda(status, name);
+    const int64_t grid = a.items * a.heads;
+    if (grid > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 segments x heads");
+    attention_mma_kernel<NQ, NV><<<dim3(static_cast<unsigned>(grid), a.passes), kBlock, Layout<NQ, NV>::kDynamic, stream>>>(a, maps, states_only);
+    return launch_status(name);
+}
+
+}
+
+namespace acro_b200_detail
+{
+
+// bf16 rows that tiled copies can read: 16-byte boundaries and strides, at most 128 columns, 31-bit numbers of tokens and sequences.
+bool attention_mma_supported(const AttentionArgs &a)
+{
+    if (a.tokens < 1 || a.tokens > INT32_MAX - 2 * kChunk || a.sequences > INT32_MAX || encoder() == nullptr) return false;
+    for (int i = 0; i < a.passes; ++i)
+    {
+        const AttentionPass &p = a.pass[i];
+        if (p.dq > 128 || p.dv > 128 || !rows_fit(a, p.q) || !rows_fit(a, p.k) || !rows_fit(a, p.v)) return false;
+    }
+    return true;
+}
+
+int attention_mma_launch(const AttentionArgs &a, bool states_only, cudaStream_t stream)
+{
+    Maps maps = {};
+    int q = 1, v = 1;
+    for (int i = 0; i < a.passes; ++i)
+    {
+        const AttentionPass &p = a.pass[i];
+        q = std::max(q, (p.dq + 63) / 64);
+        v = std::max(v, (p.dv + 63) / 64);
+        if (!make_map(&maps.q[i], a, p.q, p.dq) || !make_map(&maps.k[i], a, p.k, p.dq) || !make_map(&maps.v[i], a, p.v, p.dv))
+            return fail_cuda(cudaErrorInvalidValue, "acro_b200_linear_attention (tensor map)");
+    }
+    if (q == 1) return v == 1 ? launch<1, 1>(a, maps, states_only, stream) : launch<1, 2>(a, maps, states_only, stream);
+    return v == 1 ? launch<2, 1>(a, maps, states_only, stream) : launch<2, 2>(a, maps, states_only, stream);
+}
+
+}

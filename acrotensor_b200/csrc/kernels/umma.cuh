@@ -1,0 +1,115 @@
+// The sm_100a tensor cores (tcgen05) for bf16 operands with fp32 accumulators in tensor memory, and tiled bulk copies that leave
+// their operands in the 128-byte swizzle.
+//
+// An operand tile in shared memory is a column of boxes: 64 bf16 (128 bytes) a row, rows one behind the other, each group of 8 rows
+// (1024 bytes, aligned) swizzled: the 16-byte piece p of row r sits at piece p ^ (r & 7).  A tiled copy with the 128-byte swizzle
+// writes it so.  The same tile serves as an operand whose contracted index runs along the rows' columns ("by columns", K-major: rows
+// are M or N) or along the rows ("by rows", MN-major: columns are M or N).
+//
+// Rules kept by every user: one thread issues the products and their commits; A and B are both bf16; waits are bounded.
+#ifndef ACRO_B200_KERNELS_UMMA_CUH
+#define ACRO_B200_KERNELS_UMMA_CUH
+
+#include <cstdint>
+#include <cuda.h>
+#include "tma.cuh"
+#include "tmem.cuh"
+
+namespace acro_b200_detail
+{
+
+constexpr uint32_t kBoxColumns = 64;        // bf16 of one row of a box
+
+// Shared-memory operand descriptor: address, leading and stride byte offsets in units of 16 bytes, version 1, 128-byte swizzle.
+// By columns: stride = distance of 8-row groups; the leading offset is not used.  By rows: stride = distance of 8-row groups along the
+// contracted index, leading = distance of boxes along M or N.
+__device__ __forceinline__ uint64_t umma_operand(uint32_t address, uint32_t leading, uint32_t stride)
+{
+    return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | static_cast<uint64_t>(leading >> 4) << 16 | static_cast<uint64_t>(stride >> 4) << 32 |
+           1ull << 46 | 2ull << 61;
+}
+
+// Instruction descriptor: fp32 accumulators, bf16 operands, M = 128, N columns; by_rows as above.
+__host__ __device__ constexpr uint32_t umma_shape(int n, bool a_by_rows, bool b_by_rows)
+{
+    return 1u << 4 | 1u << 7 | 1u << 10 | static_cast<uint32_t>(a_by_rows) << 15 | static_cast<uint32_t>(b_by_rows) << 16 |
+           static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(128 >> 4) << 24;
+}
+
+// D[128 lanes][n columns] (+)= A (16 columns) * B, A and B in shared memory.
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+
+// The same with A in tensor memory: lane = row of A, a 32-bit column holds two neighbouring entries of the contracted index.
+__device__ __forceinline__ void umma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+
+// One arrival on `bar` when every product this thread has issued so far is complete.
+__device__ __forceinline__ void umma_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// One box of a four-dimensional array (column, head, token, sequence).
+__device__ __forceinline__ void box_load(void *smem, const CUtensorMap *map, int column, int head, int token, int sequence, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(smem)),
+                 "l"(map), "r"(column), "r"(head), "r"(token), "r"(sequence), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// 32 columns of this thread's lane.  The wait is part of the statement, so that no use of the registers can move in front of it.
+__device__ __forceinline__ void tmem_load_32(uint32_t addr, uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+
+// One column of this thread's lane.
+__device__ __forceinline__ uint32_t tmem_load_1(uint32_t addr)
+{
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\ntcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(addr) : "memory");
+    return r;
+}
+
+// 16 columns of this thread's lane.
+__device__ __forceinline__ void tmem_store_16(uint32_t addr, const uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+}
+
+#endif
