@@ -29,9 +29,11 @@ namespace
 
 constexpr int kChunk = 64;
 constexpr int kBox = kChunk * 128;          // bytes of 64 rows of 64 columns
-constexpr int kWorkers = 256;               // threads that convert: warps 0 .. 7; warp 8 issues
-constexpr int kBlock = kWorkers + 32;
-constexpr int kRing = 4;                    // slots of the flags that tell of non-finite values
+// Warps 0 .. 15 keep the state and write `out` (a quarter of the state's columns and of the chunk's rows each, for 32 lanes).
+// Warps 16 .. 23 make operands: those on tensor memory lanes 0 .. 63 the weights, the others K~.  Warp 24 issues copies and products.
+constexpr int kStateWarps = 16, kOperandWarps = 8, kBlock = (kStateWarps + kOperandWarps + 1) * 32;
+constexpr int kStateThreads = kStateWarps * 32, kOperandThreads = kOperandWarps * 32;
+constexpr int kRing = 16;                   // slots of the flags that tell of non-finite values; operand warps run at most 5 chunks ahead
 
 // Columns of tensor memory.
 constexpr uint32_t kScores = 0, kNear = 64, kFar = 128, kDelta = 192, kStateHigh = 320, kStateLow = 384, kColumns = 512;
@@ -46,33 +48,64 @@ struct Layout
     static constexpr int kScaled = kStages * kStage;            // K~, three parts
     static constexpr int kWeights = kScaled + 3 * NQ * kBox;    // P~, two parts
     static constexpr int kTables = kWeights + 2 * kBox;
-    static constexpr int kBytes = kTables + 2048;
     // a first product of M = 128 reads 64 rows behind a box: they lie inside the allocation
+    static constexpr int kBytes = kTables + 2048;
     static constexpr int kDynamic = kBytes + 1024;              // the base is rounded up to 1024
 };
 
 struct Shared
 {
-    float power[kChunk + 1];
+    float power[kChunk + 4];
     int odd[kRing];
     uint32_t tmem;
-    uint64_t full[4], scores, scaled, weights, state, out, out_free, change, drained;
+    uint64_t full[4], checked[4], scores, scaled, weights, state, far, out, out_free, change, change_free, drained;
 };
 
-__device__ __forceinline__ uint32_t pack_bf16(float low, float high)
+// Two neighbouring fp32 values in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n"
+        ".reg .b64 x, y, z, w;\n"
+        "mov.b64 x, {%2, %3};\n"
+        "mov.b64 y, {%4, %5};\n"
+        "mov.b64 z, {%6, %7};\n"
+        "fma.rn.f32x2 w, x, y, z;\n"
+        "mov.b64 {%0, %1}, w;\n"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n"
+        ".reg .b64 x, y, w;\n"
+        "mov.b64 x, {%2, %3};\n"
+        "mov.b64 y, {%4, %5};\n"
+        "mul.rn.f32x2 w, x, y;\n"
+        "mov.b64 {%0, %1}, w;\n"
+        "}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float2 x)
 {
     uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
     return r;
 }
-__device__ __forceinline__ float low_of(uint32_t x) { return __uint_as_float(x << 16); }
-__device__ __forceinline__ float high_of(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+__device__ __forceinline__ float2 unpack_bf16(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 
-// What a bf16 part leaves of x; nothing of an infinity.
-__device__ __forceinline__ float left_over(float x, float part)
+// The next bf16 part of x: returns it and leaves the remainder.  (Of an infinity the remainder is NaN: sums that meet one are not finite.)
+__device__ __forceinline__ uint32_t take_part(float2 &x)
 {
-    const float d = x - part;
-    return fabsf(part) == __int_as_float(0x7f800000) ? 0.0f : d;
+    const uint32_t part = pack_bf16(x);
+    x = fma2(unpack_bf16(part), make_float2(-1.0f, -1.0f), x);
+    return part;
 }
 
 __device__ __forceinline__ bool odd_half(uint32_t x) { return (x & 0x7f80u) == 0x7f80u; }
@@ -86,7 +119,7 @@ template <int NQ, int NV>
 __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ Maps maps, bool states_only)
 {
     using L = Layout<NQ, NV>;
-    constexpr int HALF = NQ * 32;               // columns of the state per thread
+    constexpr int PART = NQ * 16;               // columns of the state per thread
     const int pass = blockIdx.y;
     const AttentionPass &p = a.pass[pass];
     const int head = blockIdx.x % a.heads;
@@ -107,18 +140,24 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     if (threadIdx.x < kRing) sh.odd[threadIdx.x] = 0;
     if (threadIdx.x == 0)
     {
-        for (int i = 0; i < L::kStages; ++i) mbar_init(&sh.full[i], 1);
+        for (int i = 0; i < L::kStages; ++i)
+        {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.checked[i], kOperandThreads / 2);
+        }
         mbar_init(&sh.scores, 1);
+        mbar_init(&sh.far, 1);
         mbar_init(&sh.out, 1);
         mbar_init(&sh.change, 1);
         mbar_init(&sh.drained, 1);
-        mbar_init(&sh.scaled, kWorkers);
-        mbar_init(&sh.weights, kWorkers / 2);
-        mbar_init(&sh.state, kWorkers);
-        mbar_init(&sh.out_free, kWorkers);
+        mbar_init(&sh.scaled, kOperandThreads / 2);
+        mbar_init(&sh.weights, kOperandThreads / 2);
+        mbar_init(&sh.state, kStateThreads);
+        mbar_init(&sh.out_free, kStateThreads);
+        mbar_init(&sh.change_free, kStateThreads);
         fence_mbar_init();
     }
-    if (warp == 8) tmem_alloc(&sh.tmem, kColumns);
+    if (warp == kStateWarps + kOperandWarps) tmem_alloc(&sh.tmem, kColumns);
     tmem_fence_before_sync();
     __syncthreads();
     tmem_fence_after_sync();
@@ -126,9 +165,10 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     const int64_t length = item.end - item.begin;
     const int chunks = static_cast<int>((length + kChunk - 1) / kChunk);
     const auto chunk_of = [&](int c) { return reverse ? chunks - 1 - c : c; };
+    const auto tokens_of = [&](int c) { return static_cast<int>(min(static_cast<int64_t>(kChunk), length - static_cast<int64_t>(chunk_of(c)) * kChunk)); };
     bool ok = true;
 
-    if (warp == 8)
+    if (warp == kStateWarps + kOperandWarps)
     {
         if (lane == 0)
         {
@@ -153,7 +193,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             const uint32_t by_columns = umma_shape(kChunk, false, false), near_shape = umma_shape(kChunk, true, false),
                            change_shape = umma_shape((p.dq + 15) / 16 * 16, true, true);
             int c = 0;
-            for (; c < chunks && ok; ++c)
+            for (; c < chunks; ++c)
             {
                 const uint32_t stage = base + c % L::kStages * L::kStage, parity = c & 1;
                 ok = mbar_wait(&sh.full[c % L::kStages], c / L::kStages & 1);
@@ -168,24 +208,8 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                     }
                     umma_commit(&sh.scores);
                 }
-                // the stage of the previous chunk takes the chunk kStages - 1 ahead once its products are complete and its readers done
-                if (c > 0)
-                {
-                    ok = mbar_wait(&sh.change, parity ^ 1) && (states_only || mbar_wait(&sh.out_free, parity ^ 1));
-                    if (!ok) break;
-                }
-                if (loaded < chunks) load(loaded++);
-                if (!states_only)
-                {
-                    ok = mbar_wait(&sh.state, parity);
-                    if (!ok) break;
-                    tmem_fence_after_sync();
-                    for (int part = 0; part < 2; ++part)
-                        for (int k = 0; k < steps; ++k)
-                            umma_tmem(tmem + kFar, tmem + (part ? kStateLow : kStateHigh) + k * 8,
-                                      umma_operand(stage + L::kQ + k / 4 * kBox + k % 4 * 32, 16, 1024), by_columns, part + k > 0);
-                }
-                ok = mbar_wait(&sh.scaled, parity);
+                ok = (c == 0 || mbar_wait(&sh.change_free, parity ^ 1)) && mbar_wait(&sh.checked[c % L::kStages], c / L::kStages & 1) &&
+                     mbar_wait(&sh.scaled, parity);
                 if (!ok) break;
                 tmem_fence_after_sync();
                 for (int part = 0; part < 3; ++part)
@@ -193,7 +217,22 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                         umma(tmem + kDelta, umma_operand(stage + L::kV + k * 2048, NV == 2 ? kBox : 0, 1024),
                              umma_operand(base + L::kScaled + part * NQ * kBox + k * 2048, kBox, 1024), change_shape, part + k > 0);
                 umma_commit(&sh.change);
-                if (states_only) continue;
+                if (states_only)
+                {
+                    // the previous chunk's stage is free: its change is complete (its reader was waited for above)
+                    if (loaded < chunks) load(loaded++);
+                    continue;
+                }
+                ok = mbar_wait(&sh.state, parity) && (c == 0 || mbar_wait(&sh.out_free, parity ^ 1));
+                if (!ok) break;
+                // so is it here: all of the previous chunk's products were waited for by the readers of their results
+                if (loaded < chunks) load(loaded++);
+                tmem_fence_after_sync();
+                for (int part = 0; part < 2; ++part)
+                    for (int k = 0; k < steps; ++k)
+                        umma_tmem(tmem + kFar, tmem + (part ? kStateLow : kStateHigh) + k * 8,
+                                  umma_operand(stage + L::kQ + k / 4 * kBox + k % 4 * 32, 16, 1024), by_columns, part + k > 0);
+                umma_commit(&sh.far);
                 ok = mbar_wait(&sh.weights, parity);
                 if (!ok) break;
                 tmem_fence_after_sync();
@@ -214,13 +253,118 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         }
         __syncwarp();
     }
+    else if (warp >= kStateWarps)
+    {
+        const bool scores = warp % 4 < 2;
+        const int half = (warp - kStateWarps) / 4;
+        const int id = half * 64 + warp % 2 * 32 + lane;        // among the 128 threads of either kind
+        const float state_scale = static_cast<float>(p.state_scale);
+        for (int c = 0; c < chunks; ++c)
+        {
+            unsigned char *stage = smem + c % L::kStages * L::kStage;
+            const uint32_t parity = c & 1;
+            const int m = tokens_of(c);
+            ok = all_wait(&sh.full[c % L::kStages], c / L::kStages & 1);
+            if (!ok) break;
+            if (!scores)
+            {
+                // the three parts are read by the previous chunk's products until its change is complete
+                if (c > 0) ok = all_wait(&sh.change, parity ^ 1);
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < NQ * 4; ++i)
+                {
+                    const int piece = i * 128 + id, r = piece / 8 % kChunk;
+                    uint4 x = *reinterpret_cast<const uint4 *>(stage + L::kK + piece * 16);
+                    if (r >= m) x = make_uint4(0, 0, 0, 0);     // whatever stands behind the last token
+                    const float w = sh.power[r >= m ? 0 : reverse ? r + 1 : m - 1 - r];
+                    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                    uint32_t part[3][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                    {
+                        float2 y = mul2(unpack_bf16(in[j]), make_float2(w, w));
+                        part[0][j] = take_part(y);
+                        part[1][j] = take_part(y);
+                        part[2][j] = pack_bf16(y);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+                        *reinterpret_cast<uint4 *>(smem + L::kScaled + k * NQ * kBox + piece * 16) = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
+                }
+                fence_proxy_async();
+                mbar_arrive(&sh.scaled);
+                continue;
+            }
+            // Rows of V behind the last token become zeros.  So do its infinities and NaN, because a masked weight times one of them would
+            // be NaN: where there are any, the rows and states that they do meet get them from the state warps.
+            if (id == 0) sh.odd[(c + kRing / 2) % kRing] = 0;
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < NV * 4; ++i)
+            {
+                const int piece = i * 128 + id, r = piece / 8 % kChunk;
+                uint4 *at = reinterpret_cast<uint4 *>(stage + L::kV + piece * 16);
+                const uint4 x = *at;
+                if (r >= m) *at = make_uint4(0, 0, 0, 0);
+                else if (odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w))
+                {
+                    *at = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
+                    odd = true;
+                }
+            }
+            if (odd) sh.odd[c % kRing] = 1;
+            fence_proxy_async();
+            mbar_arrive(&sh.checked[c % L::kStages]);      // one barrier per stage: these warps may be a few chunks ahead
+            if (states_only) continue;
+            // the weights are read by the previous chunk's products, and by its state warps where V was not finite
+            ok = all_wait(&sh.scores, parity) && (c == 0 || all_wait(&sh.out_free, parity ^ 1));
+            if (!ok) break;
+            tmem_fence_after_sync();
+            const int r = warp % 4 * 32 + lane, last = reverse ? m - 1 : r, first = reverse ? r : 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+            {
+                const int c0 = half * 32 + h * 16;
+                uint32_t x[16];
+                tmem_load_16(tmem + kScores + (static_cast<uint32_t>(warp % 4 * 32) << 16) + c0, x);
+#pragma unroll
+                for (int j = 0; j < 16; j += 8)
+                {
+                    uint32_t high[4], low[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                    {
+                        float y[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                        {
+                            const int col = c0 + j + 2 * i + e;
+                            const float w = sh.power[abs(r - col)] * state_scale;
+                            y[e] = col >= first && col <= last ? __uint_as_float(x[j + 2 * i + e]) * w : 0.0f;
+                        }
+                        float2 z = make_float2(y[0], y[1]);
+                        high[i] = take_part(z);
+                        low[i] = pack_bf16(z);
+                    }
+                    const int at = r * 128 + (((c0 + j) / 8) ^ (r & 7)) * 16;
+                    *reinterpret_cast<uint4 *>(smem + L::kWeights + at) = make_uint4(high[0], high[1], high[2], high[3]);
+                    *reinterpret_cast<uint4 *>(smem + L::kWeights + kBox + at) = make_uint4(low[0], low[1], low[2], low[3]);
+                }
+            }
+            tmem_fence_before_sync();
+            fence_proxy_async();
+            mbar_arrive(&sh.weights);
+        }
+        if (!ok && lane == 0) *a.wait_flag = 1;
+    }
     else
     {
-        // this thread's row of the transposed state, and which half of its columns
-        const int b = warp % 4 * 32 + lane, half = warp / 4;
+        // this thread's row of the transposed state, and which quarter of its columns
+        const int b = warp % 4 * 32 + lane, part = warp / 4, d0 = part * PART, r0 = part * 16;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
         const bool used = b < p.dv;
-        float s[HALF];
+        float s[PART];
         const int64_t size = static_cast<int64_t>(p.dq) * p.dv;
         {
             const float *from = nullptr;
@@ -235,28 +379,24 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                 }
             }
 #pragma unroll
-            for (int j = 0; j < HALF; ++j)
-            {
-                const int d = half * HALF + j;
-                s[j] = from != nullptr && used && d < p.dq ? (turned ? from[b * p.dq + d] : from[static_cast<int64_t>(d) * p.dv + b]) : 0.0f;
-            }
+            for (int j = 0; j < PART; ++j)
+                s[j] = from != nullptr && used && d0 + j < p.dq ? (turned ? from[b * p.dq + d0 + j] : from[static_cast<int64_t>(d0 + j) * p.dv + b]) : 0.0f;
         }
         const auto publish = [&]() {
             // the state as the A operand of the next chunk: two bf16 parts, pairs of columns
 #pragma unroll
-            for (int j = 0; j < HALF; j += 32)
+            for (int j = 0; j < PART; j += 16)
             {
-                uint32_t high[16], low[16];
+                uint32_t high[8], low[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
+                for (int i = 0; i < 8; ++i)
                 {
-                    const float x = s[j + 2 * i], y = s[j + 2 * i + 1];
-                    high[i] = pack_bf16(x, y);
-                    low[i] = pack_bf16(left_over(x, low_of(high[i])), left_over(y, high_of(high[i])));
+                    float2 x = make_float2(s[j + 2 * i], s[j + 2 * i + 1]);
+                    high[i] = take_part(x);
+                    low[i] = pack_bf16(x);
                 }
-                const uint32_t at = lanes + (half * HALF + j) / 2;
-                tmem_store_16(tmem + kStateHigh + at, high);
-                tmem_store_16(tmem + kStateLow + at, low);
+                tmem_store_8(tmem + kStateHigh + lanes + (d0 + j) / 2, high);
+                tmem_store_8(tmem + kStateLow + lanes + (d0 + j) / 2, low);
             }
             tmem_wait_stores();
             tmem_fence_before_sync();
@@ -267,100 +407,11 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         const __nv_bfloat16 *k = rows_of<const __nv_bfloat16>(p.k, a, item.sequence, head), *v = rows_of<const __nv_bfloat16>(p.v, a, item.sequence, head);
         float keep = 1, rest = 0;
         int kept = 0;
-        float *sums = rows_of<float>(p.out, a, item.sequence, head);
-        __nv_bfloat16 *out = rows_of<__nv_bfloat16>(p.out, a, item.sequence, head);
-
         for (int c = 0; c < chunks; ++c)
         {
-            unsigned char *stage = smem + c % L::kStages * L::kStage;
             const uint32_t parity = c & 1;
             const int64_t t0 = item.begin + static_cast<int64_t>(chunk_of(c)) * kChunk;
-            const int m = static_cast<int>(min(static_cast<int64_t>(kChunk), item.end - t0));
-            ok = all_wait(&sh.full[c % L::kStages], c / L::kStages & 1);
-            if (!ok) break;
-            // K~; rows behind the chunk's last token are zeros in K~ and V.  Infinities and NaN of V become zeros too, because a masked
-            // weight times one of them would be NaN: where there are any, the rows and states that they do meet get them below.
-            if (threadIdx.x == 0) sh.odd[(c + 2) % kRing] = 0;
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < NQ * 2; ++i)
-            {
-                const int piece = i * kWorkers + threadIdx.x, r = piece / 8 % kChunk;
-                const uint4 x = *reinterpret_cast<const uint4 *>(stage + L::kK + piece * 16);
-                const float w = r < m ? sh.power[reverse ? r + 1 : m - 1 - r] : 0.0f;
-                const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-                uint32_t part[3][4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                {
-                    float lo = r < m ? low_of(in[j]) * w : 0.0f, hi = r < m ? high_of(in[j]) * w : 0.0f;
-                    part[0][j] = pack_bf16(lo, hi);
-                    lo = left_over(lo, low_of(part[0][j]));
-                    hi = left_over(hi, high_of(part[0][j]));
-                    part[1][j] = pack_bf16(lo, hi);
-                    part[2][j] = pack_bf16(lo - low_of(part[1][j]), hi - high_of(part[1][j]));
-                }
-#pragma unroll
-                for (int k = 0; k < 3; ++k)
-                    *reinterpret_cast<uint4 *>(smem + L::kScaled + k * NQ * kBox + piece * 16) = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
-            }
-#pragma unroll
-            for (int i = 0; i < NV * 2; ++i)
-            {
-                const int piece = i * kWorkers + threadIdx.x, r = piece / 8 % kChunk;
-                uint4 *x = reinterpret_cast<uint4 *>(stage + L::kV + piece * 16);
-                if (r >= m) *x = make_uint4(0, 0, 0, 0);
-                else if (odd_pair(x->x) | odd_pair(x->y) | odd_pair(x->z) | odd_pair(x->w))
-                {
-                    *x = make_uint4(finite_pair(x->x), finite_pair(x->y), finite_pair(x->z), finite_pair(x->w));
-                    odd = true;
-                }
-            }
-            if (odd) sh.odd[c % kRing] = 1;
-            fence_proxy_async();
-            mbar_arrive(&sh.scaled);
-
-            if (!states_only)
-            {
-                if (warp % 4 < 2)
-                {
-                    ok = all_wait(&sh.scores, parity);
-                    if (!ok) break;
-                    tmem_fence_after_sync();
-                    const int r = b;
-                    uint32_t x[32];
-                    tmem_load_32(tmem + kScores + lanes + half * 32, x);
-                    const int last = reverse ? m - 1 : r, first = reverse ? r : 0;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                    {
-                        uint32_t high[4], low[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                        {
-                            float y[2];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                            {
-                                const int col = half * 32 + j + 2 * i + e;
-                                y[e] = col >= first && col <= last ? __uint_as_float(x[j + 2 * i + e]) * (sh.power[abs(r - col)] * state_scale) : 0.0f;
-                            }
-                            high[i] = pack_bf16(y[0], y[1]);
-                            low[i] = pack_bf16(left_over(y[0], low_of(high[i])), left_over(y[1], high_of(high[i])));
-                        }
-                        const int at = r * 128 + ((half * 4 + j / 8) ^ (r & 7)) * 16;
-                        *reinterpret_cast<uint4 *>(smem + L::kWeights + at) = make_uint4(high[0], high[1], high[2], high[3]);
-                        *reinterpret_cast<uint4 *>(smem + L::kWeights + kBox + at) = make_uint4(low[0], low[1], low[2], low[3]);
-                    }
-                    tmem_fence_before_sync();
-                    fence_proxy_async();
-                    mbar_arrive(&sh.weights);
-                }
-            }
-
-            ok = all_wait(&sh.change, parity);
-            if (!ok) break;
-            tmem_fence_after_sync();
+            const int m = tokens_of(c);
             if (m != kept)
             {
                 // what is left of the state after m tokens, to twice the digits: the rounding of one factor would come back in every chunk
@@ -369,13 +420,24 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                 rest = static_cast<float>(exact - static_cast<double>(keep));
                 kept = m;
             }
-#pragma unroll
-            for (int j = 0; j < HALF; j += 32)
+            ok = all_wait(&sh.change, parity);
+            if (!ok) break;
+            tmem_fence_after_sync();
             {
-                uint32_t x[32];
-                tmem_load_32(tmem + kDelta + lanes + half * HALF + j, x);
+                uint32_t x[PART];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[j + i] = fmaf(keep, s[j + i], fmaf(rest, s[j + i], state_scale * __uint_as_float(x[i])));
+                for (int j = 0; j < PART; j += 16) tmem_load_16(tmem + kDelta + lanes + d0 + j, *reinterpret_cast<uint32_t (*)[16]>(x + j));
+                tmem_fence_before_sync();
+                mbar_arrive(&sh.change_free);
+                const float2 keeps = make_float2(keep, keep), rests = make_float2(rest, rest), scales = make_float2(state_scale, state_scale);
+#pragma unroll
+                for (int j = 0; j < PART; j += 2)
+                {
+                    const float2 was = make_float2(s[j], s[j + 1]);
+                    const float2 now = fma2(keeps, was, fma2(rests, was, mul2(scales, make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])))));
+                    s[j] = now.x;
+                    s[j + 1] = now.y;
+                }
             }
             const bool any_odd = sh.odd[c % kRing] != 0;
             if (any_odd && used)
@@ -386,52 +448,67 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                     const float left = sh.power[reverse ? t + 1 : m - 1 - t] * state_scale * x;
                     const __nv_bfloat16 *row = k + (t0 + t) * p.k.token;
 #pragma unroll
-                    for (int j = 0; j < HALF; ++j)
-                        if (half * HALF + j < p.dq) s[j] += left * __bfloat162float(row[half * HALF + j]);
+                    for (int j = 0; j < PART; ++j)
+                        if (d0 + j < p.dq) s[j] += left * __bfloat162float(row[d0 + j]);
                 }
-            if (states_only)
-            {
-                tmem_fence_before_sync();
-                continue;
-            }
+            if (states_only) continue;
+            ok = all_wait(&sh.far, parity);         // the old state has been read
+            if (!ok) break;
+            tmem_fence_after_sync();
             publish();
 
             ok = all_wait(&sh.out, parity);
             if (!ok) break;
             tmem_fence_after_sync();
-            uint32_t near[32], far[32];
-            tmem_load_32(tmem + kNear + lanes + half * 32, near);
-            tmem_load_32(tmem + kFar + lanes + half * 32, far);
+            uint32_t near[16], far[16];
+            tmem_load_16(tmem + kNear + lanes + r0, near);
+            tmem_load_16(tmem + kFar + lanes + r0, far);
+            if (any_odd && used)
+                for (int t = 0; t < m; ++t)
+                {
+                    const float x = __bfloat162float(v[(t0 + t) * p.v.token + b]);
+                    if (isfinite(x)) continue;
+                    const __nv_bfloat16 *w = reinterpret_cast<const __nv_bfloat16 *>(smem + L::kWeights);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                    {
+                        const int r = r0 + i, at = r * 64 + ((t / 8) ^ (r & 7)) * 8 + t % 8;
+                        if (reverse ? t >= r : t <= r)
+                            near[i] = __float_as_uint(__uint_as_float(near[i]) + (__bfloat162float(w[at]) + __bfloat162float(w[kBox / 2 + at])) * x);
+                    }
+                }
             tmem_fence_before_sync();
             mbar_arrive(&sh.out_free);
-            if (any_odd)
-            {
-                if (used)
-                    for (int t = 0; t < m; ++t)
-                    {
-                        const float x = __bfloat162float(v[(t0 + t) * p.v.token + b]);
-                        if (isfinite(x)) continue;
-                        const __nv_bfloat16 *w = reinterpret_cast<const __nv_bfloat16 *>(smem + L::kWeights);
+            if (!used) continue;
+            float o[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                        {
-                            const int r = half * 32 + i, at = r * 64 + ((t / 8) ^ (r & 7)) * 8 + t % 8;
-                            if (reverse ? t >= r : t <= r)
-                                near[i] = __float_as_uint(__uint_as_float(near[i]) + (__bfloat162float(w[at]) + __bfloat162float(w[kBox / 2 + at])) * x);
-                        }
-                    }
-                named_barrier(1, kWorkers);     // the next chunk's weights overwrite these
+            for (int i = 0; i < 16; ++i)
+            {
+                const int r = r0 + i;
+                const float come = sh.power[r >= m ? 0 : reverse ? m - 1 - r : r + 1];
+                o[i] = out_scale * fmaf(come, __uint_as_float(far[i]), __uint_as_float(near[i]));
             }
-            if (used)
+            const int64_t at = (t0 + r0) * p.out.token + b;
+            if (p.sums)
             {
+                float *to = rows_of<float>(p.out, a, item.sequence, head) + at;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
+                for (int i = 0; i < 16; ++i)
+                    if (r0 + i < m) to[i * p.out.token] = o[i];
+            }
+            else
+            {
+                __nv_bfloat16 *to = rows_of<__nv_bfloat16>(p.out, a, item.sequence, head) + at;
+                if (r0 + 16 <= m)
                 {
-                    const int r = half * 32 + i;
-                    if (r >= m) break;
-                    const float o = out_scale * (__uint_as_float(near[i]) + sh.power[reverse ? m - 1 - r : r + 1] * __uint_as_float(far[i]));
-                    if (p.sums) sums[(t0 + r) * p.out.token + b] = o;
-                    else out[(t0 + r) * p.out.token + b] = __float2bfloat16_rn(o);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) to[i * p.out.token] = __float2bfloat16_rn(o[i]);
+                }
+                else
+                {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (r0 + i < m) to[i * p.out.token] = __float2bfloat16_rn(o[i]);
                 }
             }
         }
@@ -447,16 +524,13 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         if (to != nullptr && used)
         {
 #pragma unroll
-            for (int j = 0; j < HALF; ++j)
-            {
-                const int d = half * HALF + j;
-                if (d < p.dq) to[turned ? b * p.dq + d : static_cast<int64_t>(d) * p.dv + b] = s[j];
-            }
+            for (int j = 0; j < PART; ++j)
+                if (d0 + j < p.dq) to[turned ? b * p.dq + d0 + j : static_cast<int64_t>(d0 + j) * p.dv + b] = s[j];
         }
     }
     tmem_fence_before_sync();
     __syncthreads();
-    if (warp == 8) tmem_free(tmem, kColumns);
+    if (warp == kStateWarps + kOperandWarps) tmem_free(tmem, kColumns);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
