@@ -30,9 +30,9 @@ namespace
 constexpr int kChunk = 64;
 constexpr int kBox = kChunk * 128;          // bytes of 64 rows of 64 columns
 // Warps 0 .. 15 keep the state and write `out` (a quarter of the state's columns and of the chunk's rows each, for 32 lanes).
-// Warps 16 .. 23 make operands: those on tensor memory lanes 0 .. 63 the weights, the others K~.  Warp 24 issues copies and products.
-constexpr int kStateWarps = 16, kOperandWarps = 8, kBlock = (kStateWarps + kOperandWarps + 1) * 32;
-constexpr int kStateThreads = kStateWarps * 32, kOperandThreads = kOperandWarps * 32;
+// Warps 16 .. 23 make operands: those on tensor memory lanes 0 .. 63 the weights, the others K~.  Warp 26 issues copies and products (24 and 25 idle: so the
+// issuing warp shares a scheduler, and its instruction cache, with the short loop of K~ and not with the weights').
+constexpr int kStateWarps = 16, kOperandWarps = 8, kIssueWarp = 26, kBlock = (kIssueWarp + 1) * 32;
 constexpr int kRing = 16;                   // slots of the flags that tell of non-finite values; operand warps run at most 5 chunks ahead
 
 // Columns of tensor memory.
@@ -55,7 +55,10 @@ struct Layout
 
 struct Shared
 {
-    float power[kChunk + 4];
+    float power[kChunk + 4];                // lam^n
+    float weight[2 * kChunk];               // of tokens kChunk - i apart, times the state's scale; zero for those not seen
+    float come[2 * kChunk];                 // what the state before a whole chunk has kept at row r, times the output's scale (backward in
+                                            // time the rows of a shorter chunk stand behind one another at its end)
     int odd[kRing];
     uint32_t tmem;
     uint64_t full[4], checked[4], scores, scaled, weights, state, far, out, out_free, change, change_free, drained;
@@ -113,9 +116,16 @@ __device__ __forceinline__ bool odd_pair(uint32_t x) { return odd_half(x) || odd
 // The pair with zeros in the place of infinities and NaN.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t x) { return (odd_half(x) ? 0u : x & 0xffffu) | (odd_half(x >> 16) ? 0u : x & 0xffff0000u); }
 
+// One arrival for the whole warp, after all its lanes have come here.
+__device__ __forceinline__ void warp_arrive(uint64_t *bar)
+{
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) mbar_arrive(bar);
+}
+
 __device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
-template <int NQ, int NV>
+template <int NQ, int NV, bool SUMS>
 __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ Maps maps, bool states_only)
 {
     using L = Layout<NQ, NV>;
@@ -136,129 +146,162 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     const double g = decay_log<float>(a.log_decay, head);
-    for (int i = threadIdx.x; i <= kChunk; i += kBlock) sh.power[i] = static_cast<float>(exp(g * i));
+    if (threadIdx.x < 2 * kChunk)
+    {
+        const int i = threadIdx.x, near = reverse ? i - kChunk : kChunk - i, come = reverse ? kChunk - 1 - i : i + 1;
+        if (i <= kChunk) sh.power[i] = static_cast<float>(exp(g * i));
+        sh.weight[i] = near >= 0 ? static_cast<float>(exp(g * near) * p.state_scale) : 0.0f;
+        sh.come[i] = come >= 0 ? static_cast<float>(exp(g * come) * p.out_scale) : 0.0f;
+    }
     if (threadIdx.x < kRing) sh.odd[threadIdx.x] = 0;
     if (threadIdx.x == 0)
     {
         for (int i = 0; i < L::kStages; ++i)
         {
             mbar_init(&sh.full[i], 1);
-            mbar_init(&sh.checked[i], kOperandThreads / 2);
+            mbar_init(&sh.checked[i], kOperandWarps / 2);
         }
         mbar_init(&sh.scores, 1);
         mbar_init(&sh.far, 1);
         mbar_init(&sh.out, 1);
         mbar_init(&sh.change, 1);
         mbar_init(&sh.drained, 1);
-        mbar_init(&sh.scaled, kOperandThreads / 2);
-        mbar_init(&sh.weights, kOperandThreads / 2);
-        mbar_init(&sh.state, kStateThreads);
-        mbar_init(&sh.out_free, kStateThreads);
-        mbar_init(&sh.change_free, kStateThreads);
+        mbar_init(&sh.scaled, kOperandWarps / 2);
+        mbar_init(&sh.weights, kOperandWarps / 2);
+        mbar_init(&sh.state, kStateWarps);
+        mbar_init(&sh.out_free, kStateWarps);
+        mbar_init(&sh.change_free, kStateWarps);
         fence_mbar_init();
     }
-    if (warp == kStateWarps + kOperandWarps) tmem_alloc(&sh.tmem, kColumns);
+    if (warp == kIssueWarp) tmem_alloc(&sh.tmem, kColumns);
     tmem_fence_before_sync();
     __syncthreads();
     tmem_fence_after_sync();
     const uint32_t tmem = sh.tmem;
-    const int64_t length = item.end - item.begin;
-    const int chunks = static_cast<int>((length + kChunk - 1) / kChunk);
+    const int length = static_cast<int>(item.end - item.begin);
+    const int chunks = (length + kChunk - 1) / kChunk;
     const auto chunk_of = [&](int c) { return reverse ? chunks - 1 - c : c; };
-    const auto tokens_of = [&](int c) { return static_cast<int>(min(static_cast<int64_t>(kChunk), length - static_cast<int64_t>(chunk_of(c)) * kChunk)); };
+    const auto tokens_of = [&](int c) { return min(kChunk, length - chunk_of(c) * kChunk); };
     bool ok = true;
 
-    if (warp == kStateWarps + kOperandWarps)
+    if (warp == kIssueWarp)
     {
-        if (lane == 0)
-        {
-            const int stage_bytes = states_only ? (NQ + NV) * kBox : L::kStage;
-            const int hq = head / p.q.group, hk = head / p.k.group, hv = head / p.v.group, n = a.offsets == nullptr ? static_cast<int>(item.sequence) : 0;
-            const auto load = [&](int c) {
-                unsigned char *stage = smem + c % L::kStages * L::kStage;
-                uint64_t *bar = &sh.full[c % L::kStages];
-                const int t = static_cast<int>(item.begin + static_cast<int64_t>(chunk_of(c)) * kChunk);
-                mbar_arrive_expect_tx(bar, stage_bytes);
-                for (int i = 0; i < NQ; ++i)
-                {
-                    if (!states_only) box_load(stage + L::kQ + i * kBox, &maps.q[pass], i * kBoxColumns, hq, t, n, bar);
-                    box_load(stage + L::kK + i * kBox, &maps.k[pass], i * kBoxColumns, hk, t, n, bar);
-                }
-                for (int i = 0; i < NV; ++i) box_load(stage + L::kV + i * kBox, &maps.v[pass], i * kBoxColumns, hv, t, n, bar);
-            };
-            int loaded = 0;
-            for (; loaded < min(chunks, L::kStages - 1); ++loaded) load(loaded);
-            const uint32_t base = smem_addr(smem);
-            const int steps = (p.dq + 15) / 16;
-            const uint32_t by_columns = umma_shape(kChunk, false, false), near_shape = umma_shape(kChunk, true, false),
-                           change_shape = umma_shape((p.dq + 15) / 16 * 16, true, true);
-            int c = 0;
-            for (; c < chunks; ++c)
+        // The whole warp walks the loop, one lane issues: addresses and descriptors stay in uniform registers.
+        const int stage_bytes = states_only ? (NQ + NV) * kBox : L::kStage;
+        const int hq = head / p.q.group, hk = head / p.k.group, hv = head / p.v.group, n = a.offsets == nullptr ? static_cast<int>(item.sequence) : 0;
+        const auto load = [&](int c) {
+            unsigned char *stage = smem + c % L::kStages * L::kStage;
+            uint64_t *bar = &sh.full[c % L::kStages];
+            const int t = static_cast<int>(item.begin) + chunk_of(c) * kChunk;
+            if (!elect_lane()) return;
+            mbar_arrive_expect_tx(bar, stage_bytes);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
             {
-                const uint32_t stage = base + c % L::kStages * L::kStage, parity = c & 1;
-                ok = mbar_wait(&sh.full[c % L::kStages], c / L::kStages & 1);
-                if (!ok) break;
-                if (!states_only)
-                {
-                    // the score columns are free: the previous chunk's weights were waited for
-                    for (int k = 0; k < steps; ++k)
-                    {
-                        const uint32_t at = k / 4 * kBox + k % 4 * 32;
-                        umma(tmem + kScores, umma_operand(stage + L::kQ + at, 16, 1024), umma_operand(stage + L::kK + at, 16, 1024), by_columns, k > 0);
-                    }
-                    umma_commit(&sh.scores);
-                }
-                ok = (c == 0 || mbar_wait(&sh.change_free, parity ^ 1)) && mbar_wait(&sh.checked[c % L::kStages], c / L::kStages & 1) &&
-                     mbar_wait(&sh.scaled, parity);
-                if (!ok) break;
-                tmem_fence_after_sync();
+                if (!states_only) box_load(stage + L::kQ + i * kBox, &maps.q[pass], i * kBoxColumns, hq, t, n, bar);
+                box_load(stage + L::kK + i * kBox, &maps.k[pass], i * kBoxColumns, hk, t, n, bar);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) box_load(stage + L::kV + i * kBox, &maps.v[pass], i * kBoxColumns, hv, t, n, bar);
+        };
+        int loaded = 0;
+        for (; loaded < min(chunks, L::kStages - 1); ++loaded) load(loaded);
+        const uint32_t base = smem_addr(smem);
+        const uint32_t by_columns = umma_shape(kChunk, false, false), near_shape = umma_shape(kChunk, true, false),
+                       change_shape = umma_shape(NQ * 64, true, true);
+        const uint64_t scaled = umma_operand(base + L::kScaled, kBox, 1024), weights = umma_operand(base + L::kWeights, 16, 1024);
+        // descriptors count in units of 16 bytes
+        const auto issue_scores = [&](int c) {
+            const uint32_t stage = base + c % L::kStages * L::kStage;
+            const uint64_t q = umma_operand(stage + L::kQ, 16, 1024), k = umma_operand(stage + L::kK, 16, 1024);
+            if (!elect_lane()) return;
+#pragma unroll
+            for (int i = 0; i < NQ * 4; ++i)
+                umma(tmem + kScores, q + (i / 4 * kBox + i % 4 * 32) / 16, k + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, i > 0);
+            umma_commit(&sh.scores);
+        };
+        int c = 0;
+        if (!states_only && chunks > 0)
+        {
+            ok = all_wait(&sh.full[0], 0);
+            if (ok) issue_scores(0);
+        }
+#pragma unroll 1
+        for (; c < chunks && ok; ++c)
+        {
+            const uint32_t stage = base + c % L::kStages * L::kStage, parity = c & 1;
+            const uint64_t q = umma_operand(stage + L::kQ, 16, 1024), v = umma_operand(stage + L::kV, NV == 2 ? kBox : 0, 1024);
+            ok = (!states_only || all_wait(&sh.full[c % L::kStages], c / L::kStages & 1)) && (c == 0 || all_wait(&sh.change_free, parity ^ 1)) &&
+                 all_wait(&sh.checked[c % L::kStages], c / L::kStages & 1) && all_wait(&sh.scaled, parity);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            if (elect_lane())
+            {
+#pragma unroll
                 for (int part = 0; part < 3; ++part)
+#pragma unroll
                     for (int k = 0; k < kChunk / 16; ++k)
-                        umma(tmem + kDelta, umma_operand(stage + L::kV + k * 2048, NV == 2 ? kBox : 0, 1024),
-                             umma_operand(base + L::kScaled + part * NQ * kBox + k * 2048, kBox, 1024), change_shape, part + k > 0);
+                        umma(tmem + kDelta, v + k * 2048 / 16, scaled + (part * NQ * kBox + k * 2048) / 16, change_shape, part + k > 0);
                 umma_commit(&sh.change);
-                if (states_only)
-                {
-                    // the previous chunk's stage is free: its change is complete (its reader was waited for above)
-                    if (loaded < chunks) load(loaded++);
-                    continue;
-                }
-                ok = mbar_wait(&sh.state, parity) && (c == 0 || mbar_wait(&sh.out_free, parity ^ 1));
-                if (!ok) break;
-                // so is it here: all of the previous chunk's products were waited for by the readers of their results
+            }
+            __syncwarp();
+            if (states_only)
+            {
+                // the previous chunk's stage is free: its change is complete (its reader was waited for above)
                 if (loaded < chunks) load(loaded++);
-                tmem_fence_after_sync();
+                continue;
+            }
+            ok = all_wait(&sh.state, parity) && (c == 0 || all_wait(&sh.out_free, parity ^ 1));
+            if (!ok) break;
+            // so is it here: all of the previous chunk's products were waited for by the readers of their results
+            if (loaded < chunks) load(loaded++);
+            tmem_fence_after_sync();
+            if (elect_lane())
+            {
+#pragma unroll
                 for (int part = 0; part < 2; ++part)
-                    for (int k = 0; k < steps; ++k)
-                        umma_tmem(tmem + kFar, tmem + (part ? kStateLow : kStateHigh) + k * 8,
-                                  umma_operand(stage + L::kQ + k / 4 * kBox + k % 4 * 32, 16, 1024), by_columns, part + k > 0);
+#pragma unroll
+                    for (int i = 0; i < NQ * 4; ++i)
+                        umma_tmem(tmem + kFar, tmem + (part ? kStateLow : kStateHigh) + i * 8, q + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, part + i > 0);
                 umma_commit(&sh.far);
-                ok = mbar_wait(&sh.weights, parity);
-                if (!ok) break;
-                tmem_fence_after_sync();
+            }
+            __syncwarp();
+            ok = all_wait(&sh.weights, parity);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            if (elect_lane())
+            {
+#pragma unroll
                 for (int part = 0; part < 2; ++part)
+#pragma unroll
                     for (int k = 0; k < kChunk / 16; ++k)
-                        umma(tmem + kNear, umma_operand(stage + L::kV + k * 2048, NV == 2 ? kBox : 0, 1024),
-                             umma_operand(base + L::kWeights + part * kBox + k * 32, 16, 1024), near_shape, part + k > 0);
+                        umma(tmem + kNear, v + k * 2048 / 16, weights + (part * kBox + k * 32) / 16, near_shape, part + k > 0);
                 umma_commit(&sh.out);
             }
-            if (!ok)
+            __syncwarp();
+            if (c + 1 < chunks)
             {
-                *a.wait_flag = 1;
-                // copies and products of this CTA that are still in flight
-                for (int i = c; i < loaded; ++i) mbar_wait(&sh.full[i % L::kStages], i / L::kStages & 1);
-                umma_commit(&sh.drained);
-                mbar_wait(&sh.drained, 0);
+                ok = all_wait(&sh.full[(c + 1) % L::kStages], (c + 1) / L::kStages & 1);
+                if (!ok) break;
+                issue_scores(c + 1);
+                __syncwarp();
             }
         }
-        __syncwarp();
+        if (!ok)
+        {
+            if (lane == 0) *a.wait_flag = 1;
+            // copies and products of this CTA that are still in flight
+            for (int i = c; i < loaded; ++i) all_wait(&sh.full[i % L::kStages], i / L::kStages & 1);
+            if (elect_lane()) umma_commit(&sh.drained);
+            __syncwarp();
+            all_wait(&sh.drained, 0);
+        }
     }
-    else if (warp >= kStateWarps)
+    else if (warp >= kStateWarps && warp < kStateWarps + kOperandWarps)
     {
         const bool scores = warp % 4 < 2;
         const int half = (warp - kStateWarps) / 4;
         const int id = half * 64 + warp % 2 * 32 + lane;        // among the 128 threads of either kind
-        const float state_scale = static_cast<float>(p.state_scale);
         for (int c = 0; c < chunks; ++c)
         {
             unsigned char *stage = smem + c % L::kStages * L::kStage;
@@ -271,7 +314,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                 // the three parts are read by the previous chunk's products until its change is complete
                 if (c > 0) ok = all_wait(&sh.change, parity ^ 1);
                 if (!ok) break;
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < NQ * 4; ++i)
                 {
                     const int piece = i * 128 + id, r = piece / 8 % kChunk;
@@ -293,14 +336,14 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                         *reinterpret_cast<uint4 *>(smem + L::kScaled + k * NQ * kBox + piece * 16) = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
                 }
                 fence_proxy_async();
-                mbar_arrive(&sh.scaled);
+                warp_arrive(&sh.scaled);
                 continue;
             }
             // Rows of V behind the last token become zeros.  So do its infinities and NaN, because a masked weight times one of them would
             // be NaN: where there are any, the rows and states that they do meet get them from the state warps.
             if (id == 0) sh.odd[(c + kRing / 2) % kRing] = 0;
             bool odd = false;
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < NV * 4; ++i)
             {
                 const int piece = i * 128 + id, r = piece / 8 % kChunk;
@@ -315,50 +358,42 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             }
             if (odd) sh.odd[c % kRing] = 1;
             fence_proxy_async();
-            mbar_arrive(&sh.checked[c % L::kStages]);      // one barrier per stage: these warps may be a few chunks ahead
+            warp_arrive(&sh.checked[c % L::kStages]);      // one barrier per stage: these warps may be a few chunks ahead
             if (states_only) continue;
-            // the weights are read by the previous chunk's products, and by its state warps where V was not finite
+            // the previous chunk's weights have been read when its results have
             ok = all_wait(&sh.scores, parity) && (c == 0 || all_wait(&sh.out_free, parity ^ 1));
             if (!ok) break;
             tmem_fence_after_sync();
-            const int r = warp % 4 * 32 + lane, last = reverse ? m - 1 : r, first = reverse ? r : 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
+            const int r = warp % 4 * 32 + lane;
+            const unsigned first = reverse ? r : 0, seen = reverse ? m - 1 - r : r;     // columns first .. first + seen
+            const bool none = reverse && r >= m;
+#pragma unroll 1
+            for (int i = half * 4; i < half * 4 + 4; ++i)
             {
-                const int c0 = half * 32 + h * 16;
-                uint32_t x[16];
-                tmem_load_16(tmem + kScores + (static_cast<uint32_t>(warp % 4 * 32) << 16) + c0, x);
+                uint32_t x[8], high[4], low[4];
+                tmem_load_8(tmem + kScores + (static_cast<uint32_t>(warp % 4 * 32) << 16) + i * 8, x);
+                const float *weight = sh.weight + kChunk - r + i * 8;
 #pragma unroll
-                for (int j = 0; j < 16; j += 8)
+                for (int j = 0; j < 4; ++j)
                 {
-                    uint32_t high[4], low[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                    {
-                        float y[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                        {
-                            const int col = c0 + j + 2 * i + e;
-                            const float w = sh.power[abs(r - col)] * state_scale;
-                            y[e] = col >= first && col <= last ? __uint_as_float(x[j + 2 * i + e]) * w : 0.0f;
-                        }
-                        float2 z = make_float2(y[0], y[1]);
-                        high[i] = take_part(z);
-                        low[i] = pack_bf16(z);
-                    }
-                    const int at = r * 128 + (((c0 + j) / 8) ^ (r & 7)) * 16;
-                    *reinterpret_cast<uint4 *>(smem + L::kWeights + at) = make_uint4(high[0], high[1], high[2], high[3]);
-                    *reinterpret_cast<uint4 *>(smem + L::kWeights + kBox + at) = make_uint4(low[0], low[1], low[2], low[3]);
+                    float2 z = mul2(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), make_float2(weight[2 * j], weight[2 * j + 1]));
+                    // not a product with a zero: the score may be an infinity or NaN of another token
+                    if (i * 8 + 2 * j - first > seen) z.x = 0;
+                    if (i * 8 + 2 * j + 1 - first > seen) z.y = 0;
+                    high[j] = take_part(z);
+                    low[j] = pack_bf16(z);
                 }
+                unsigned char *to = smem + L::kWeights + r * 128 + (i ^ (r & 7)) * 16;
+                *reinterpret_cast<uint4 *>(to) = none ? make_uint4(0, 0, 0, 0) : make_uint4(high[0], high[1], high[2], high[3]);
+                *reinterpret_cast<uint4 *>(to + kBox) = none ? make_uint4(0, 0, 0, 0) : make_uint4(low[0], low[1], low[2], low[3]);
             }
             tmem_fence_before_sync();
             fence_proxy_async();
-            mbar_arrive(&sh.weights);
+            warp_arrive(&sh.weights);
         }
         if (!ok && lane == 0) *a.wait_flag = 1;
     }
-    else
+    else if (warp < kStateWarps)
     {
         // this thread's row of the transposed state, and which quarter of its columns
         const int b = warp % 4 * 32 + lane, part = warp / 4, d0 = part * PART, r0 = part * 16;
@@ -400,17 +435,19 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             }
             tmem_wait_stores();
             tmem_fence_before_sync();
-            mbar_arrive(&sh.state);
+            warp_arrive(&sh.state);
         };
         if (!states_only) publish();
         const float state_scale = static_cast<float>(p.state_scale), out_scale = static_cast<float>(p.out_scale);
-        const __nv_bfloat16 *k = rows_of<const __nv_bfloat16>(p.k, a, item.sequence, head), *v = rows_of<const __nv_bfloat16>(p.v, a, item.sequence, head);
+        // rows of `out` are a 32-bit number of bytes apart
+        const uint32_t step = static_cast<uint32_t>(p.out.token) * (SUMS ? 4u : 2u);
+        char *out = reinterpret_cast<char *>(SUMS ? static_cast<void *>(rows_of<float>(p.out, a, item.sequence, head) + item.begin * p.out.token + b)
+                                                  : static_cast<void *>(rows_of<__nv_bfloat16>(p.out, a, item.sequence, head) + item.begin * p.out.token + b));
         float keep = 1, rest = 0;
         int kept = 0;
         for (int c = 0; c < chunks; ++c)
         {
             const uint32_t parity = c & 1;
-            const int64_t t0 = item.begin + static_cast<int64_t>(chunk_of(c)) * kChunk;
             const int m = tokens_of(c);
             if (m != kept)
             {
@@ -423,34 +460,37 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             ok = all_wait(&sh.change, parity);
             if (!ok) break;
             tmem_fence_after_sync();
+            const float2 keeps = make_float2(keep, keep), rests = make_float2(rest, rest);
+#pragma unroll
+            for (int j = 0; j < PART; j += 16)
             {
-                uint32_t x[PART];
+                uint32_t x[16];
+                tmem_load_16(tmem + kDelta + lanes + d0 + j, x);
 #pragma unroll
-                for (int j = 0; j < PART; j += 16) tmem_load_16(tmem + kDelta + lanes + d0 + j, *reinterpret_cast<uint32_t (*)[16]>(x + j));
-                tmem_fence_before_sync();
-                mbar_arrive(&sh.change_free);
-                const float2 keeps = make_float2(keep, keep), rests = make_float2(rest, rest), scales = make_float2(state_scale, state_scale);
-#pragma unroll
-                for (int j = 0; j < PART; j += 2)
+                for (int i = 0; i < 16; i += 2)
                 {
-                    const float2 was = make_float2(s[j], s[j + 1]);
-                    const float2 now = fma2(keeps, was, fma2(rests, was, mul2(scales, make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])))));
-                    s[j] = now.x;
-                    s[j + 1] = now.y;
+                    const float2 was = make_float2(s[j + i], s[j + i + 1]);
+                    const float2 now = fma2(keeps, was, fma2(rests, was, mul2(make_float2(state_scale, state_scale),
+                                                                              make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])))));
+                    s[j + i] = now.x;
+                    s[j + i + 1] = now.y;
                 }
             }
-            const bool any_odd = sh.odd[c % kRing] != 0;
-            if (any_odd && used)
+            tmem_fence_before_sync();
+            warp_arrive(&sh.change_free);
+            // A column of V with an infinity or NaN: the state's, and the rows' that see its token, become NaN.  `odd`: the first such
+            // token in the order of time, as a row.
+            int odd = reverse ? -1 : kChunk;
+            if (__builtin_expect(sh.odd[c % kRing] != 0, 0) && used)
+            {
+                const __nv_bfloat16 *v = rows_of<const __nv_bfloat16>(p.v, a, item.sequence, head) + (item.begin + chunk_of(c) * kChunk) * p.v.token + b;
+#pragma unroll 1
                 for (int t = 0; t < m; ++t)
-                {
-                    const float x = __bfloat162float(v[(t0 + t) * p.v.token + b]);
-                    if (isfinite(x)) continue;
-                    const float left = sh.power[reverse ? t + 1 : m - 1 - t] * state_scale * x;
-                    const __nv_bfloat16 *row = k + (t0 + t) * p.k.token;
+                    if (!isfinite(__bfloat162float(v[t * p.v.token]))) odd = reverse ? t : min(odd, t);
+                if (odd >= 0 && odd < kChunk)
 #pragma unroll
-                    for (int j = 0; j < PART; ++j)
-                        if (d0 + j < p.dq) s[j] += left * __bfloat162float(row[d0 + j]);
-                }
+                    for (int j = 0; j < PART; ++j) s[j] = __int_as_float(0x7fffffff);
+            }
             if (states_only) continue;
             ok = all_wait(&sh.far, parity);         // the old state has been read
             if (!ok) break;
@@ -460,55 +500,43 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             ok = all_wait(&sh.out, parity);
             if (!ok) break;
             tmem_fence_after_sync();
-            uint32_t near[16], far[16];
-            tmem_load_16(tmem + kNear + lanes + r0, near);
-            tmem_load_16(tmem + kFar + lanes + r0, far);
-            if (any_odd && used)
-                for (int t = 0; t < m; ++t)
-                {
-                    const float x = __bfloat162float(v[(t0 + t) * p.v.token + b]);
-                    if (isfinite(x)) continue;
-                    const __nv_bfloat16 *w = reinterpret_cast<const __nv_bfloat16 *>(smem + L::kWeights);
+            const float *come = sh.come + r0 + (reverse ? kChunk - m : 0);
+            char *row = out + static_cast<int64_t>(chunk_of(c) * kChunk + r0) * step;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
+            for (int h = 0; h < 16; h += 8)
+            {
+                uint32_t near[8], far[8];
+                tmem_load_8(tmem + kNear + lanes + r0 + h, near);
+                tmem_load_8(tmem + kFar + lanes + r0 + h, far);
+                if (h == 8)
+                {
+                    tmem_fence_before_sync();
+                    warp_arrive(&sh.out_free);
+                }
+                if (__builtin_expect(odd >= 0 && odd < kChunk, 0))
+                {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (reverse ? r0 + h + i <= odd : r0 + h + i >= odd) near[i] = 0x7fffffffu;
+                }
+                const int rows = used ? m - r0 - h : 0;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2)
+                {
+                    const float2 o = fma2(make_float2(come[h + i], come[h + i + 1]), make_float2(__uint_as_float(far[i]), __uint_as_float(far[i + 1])),
+                                          mul2(make_float2(out_scale, out_scale), make_float2(__uint_as_float(near[i]), __uint_as_float(near[i + 1]))));
+                    char *to = row + static_cast<uint64_t>(step) * (h + i), *after = row + static_cast<uint64_t>(step) * (h + i + 1);
+                    if (SUMS)
                     {
-                        const int r = r0 + i, at = r * 64 + ((t / 8) ^ (r & 7)) * 8 + t % 8;
-                        if (reverse ? t >= r : t <= r)
-                            near[i] = __float_as_uint(__uint_as_float(near[i]) + (__bfloat162float(w[at]) + __bfloat162float(w[kBox / 2 + at])) * x);
+                        if (i < rows) *reinterpret_cast<float *>(to) = o.x;
+                        if (i + 1 < rows) *reinterpret_cast<float *>(after) = o.y;
                     }
-                }
-            tmem_fence_before_sync();
-            mbar_arrive(&sh.out_free);
-            if (!used) continue;
-            float o[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-            {
-                const int r = r0 + i;
-                const float come = sh.power[r >= m ? 0 : reverse ? m - 1 - r : r + 1];
-                o[i] = out_scale * fmaf(come, __uint_as_float(far[i]), __uint_as_float(near[i]));
-            }
-            const int64_t at = (t0 + r0) * p.out.token + b;
-            if (p.sums)
-            {
-                float *to = rows_of<float>(p.out, a, item.sequence, head) + at;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (r0 + i < m) to[i * p.out.token] = o[i];
-            }
-            else
-            {
-                __nv_bfloat16 *to = rows_of<__nv_bfloat16>(p.out, a, item.sequence, head) + at;
-                if (r0 + 16 <= m)
-                {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) to[i * p.out.token] = __float2bfloat16_rn(o[i]);
-                }
-                else
-                {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (r0 + i < m) to[i * p.out.token] = __float2bfloat16_rn(o[i]);
+                    else
+                    {
+                        const uint32_t both = pack_bf16(o);
+                        if (i < rows) *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(both);
+                        if (i + 1 < rows) *reinterpret_cast<uint16_t *>(after) = static_cast<uint16_t>(both >> 16);
+                    }
                 }
             }
         }
@@ -530,7 +558,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     }
     tmem_fence_before_sync();
     __syncthreads();
-    if (warp == kStateWarps + kOperandWarps) tmem_free(tmem, kColumns);
+    if (warp == kIssueWarp) tmem_free(tmem, kColumns);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -576,16 +604,40 @@ bool make_map(CUtensorMap *map, const AttentionArgs &a, const TokenRows &r, int 
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NQ, int NV>
-int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStream_t stream)
+template <int NQ, int NV, bool SUMS>
+int launch_as(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStream_t stream)
 {
     const char *name = "acro_b200_linear_attention";
-    cudaError_t status = cudaFuncSetAttribute(attention_mma_kernel<NQ, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<NQ, NV>::kDynamic);
+    cudaError_t status = cudaFuncSetAttribute(attention_mma_kernel<NQ, NV, SUMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<NQ, NV>::kDynamic);
     if (status != cudaSuccess) return fail_cuda(status, name);
     const int64_t grid = a.items * a.heads;
     if (grid > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 segments x heads");
-    attention_mma_kernel<NQ, NV><<<dim3(static_cast<unsigned>(grid), a.passes), kBlock, Layout<NQ, NV>::kDynamic, stream>>>(a, maps, states_only);
+    attention_mma_kernel<NQ, NV, SUMS><<<dim3(static_cast<unsigned>(grid), a.passes), kBlock, Layout<NQ, NV>::kDynamic, stream>>>(a, maps, states_only);
     return launch_status(name);
+}
+
+template <int NQ, int NV>
+int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStream_t stream)
+{
+    // one launch per kind of output: passes of the gradient write rows of sums when key and value heads are shared
+    int status = ACRO_B200_OK;
+    AttentionArgs part = a;
+    Maps of = maps;
+    for (int first = 0; first < a.passes && status == ACRO_B200_OK; first += part.passes)
+    {
+        part.passes = 0;
+        while (first + part.passes < a.passes && (states_only || a.pass[first + part.passes].sums == a.pass[first].sums))
+        {
+            part.pass[part.passes] = a.pass[first + part.passes];
+            of.q[part.passes] = maps.q[first + part.passes];
+            of.k[part.passes] = maps.k[first + part.passes];
+            of.v[part.passes] = maps.v[first + part.passes];
+            ++part.passes;
+        }
+        status = a.pass[first].sums && !states_only ? launch_as<NQ, NV, true>(part, of, states_only, stream)
+                                                    : launch_as<NQ, NV, false>(part, of, states_only, stream);
+    }
+    return status;
 }
 
 }
@@ -600,7 +652,7 @@ bool attention_mma_supported(const AttentionArgs &a)
     for (int i = 0; i < a.passes; ++i)
     {
         const AttentionPass &p = a.pass[i];
-        if (p.dq > 128 || p.dv > 128 || !rows_fit(a, p.q) || !rows_fit(a, p.k) || !rows_fit(a, p.v)) return false;
+        if (p.dq > 128 || p.dv > 128 || p.out.token < 0 || p.out.token > (1 << 29) || !rows_fit(a, p.q) || !rows_fit(a, p.k) || !rows_fit(a, p.v)) return false;
     }
     return true;
 }

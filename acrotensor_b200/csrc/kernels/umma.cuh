@@ -6,7 +6,7 @@
 // writes it so.  The same tile serves as an operand whose contracted index runs along the rows' columns ("by columns", K-major: rows
 // are M or N) or along the rows ("by rows", MN-major: columns are M or N).
 //
-// Rules kept by every user: one thread issues the products and their commits; A and B are both bf16; waits are bounded.
+// Rules kept by every user: one thread (the elected lane of one warp) issues the products and their commits; A and B are both bf16; waits are bounded.
 #ifndef ACRO_B200_KERNELS_UMMA_CUH
 #define ACRO_B200_KERNELS_UMMA_CUH
 
@@ -34,6 +34,22 @@ __host__ __device__ constexpr uint32_t umma_shape(int n, bool a_by_rows, bool b_
 {
     return 1u << 4 | 1u << 7 | 1u << 10 | static_cast<uint32_t>(a_by_rows) << 15 | static_cast<uint32_t>(b_by_rows) << 16 |
            static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(128 >> 4) << 24;
+}
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_lane()
+{
+    uint32_t one;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(one)
+        :
+        : "memory");
+    return one != 0;
 }
 
 // D[128 lanes][n columns] (+)= A (16 columns) * B, A and B in shared memory.
@@ -86,6 +102,16 @@ __device__ __forceinline__ void tmem_load_16(uint32_t addr, uint32_t (&r)[16])
                  "tcgen05.wait::ld.sync.aligned;"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// 8 columns of this thread's lane.
+__device__ __forceinline__ void tmem_load_8(uint32_t addr, uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(addr)
                  : "memory");
 }
