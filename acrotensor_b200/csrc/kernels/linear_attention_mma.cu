@@ -2,10 +2,10 @@
 //
 // A CTA walks one segment of one head in chunks of 64 tokens (r, s: tokens of the chunk; a: columns of q and k; b: of v):
 //   scores  P[r][s]     = Q[r][a] K[s][a]                            M = r (64 of 128 lanes used)
-//   near    O'[b][r]    = V[s][b] P~[r][s]                           P~: scores times powers of the decay, zero where masked
+//   near    O'[b][r]    = V[s][b] P~[r][s]                           P~: scores times powers of the decay and the scales, zero where masked
 //   far     O"[b][r]    = S[b][a] Q[r][a]                            S: the state before the chunk, A operand in tensor memory
-//   change  D[b][a]     = V[s][b] K~[s][a]                           K~: rows of K times what the decay leaves of them
-//   out[r][b] = out_scale (O' + come_r O"),   S <- lam^m S + state_scale D
+//   change  D[b][a]     = V[s][b] K~[s][a]                           K~: rows of K times what the decay leaves of them and the state's scale
+//   out[r][b] = O' + out_scale come_r O",   S <- lam^m S + D
 // The transposed forms put b on the 128 lanes: the state stays in registers (fp32), one row of S^T per thread and half its columns,
 // and becomes an A operand by a store into tensor memory, without a way through shared memory.
 //
@@ -55,10 +55,10 @@ struct Layout
 
 struct Shared
 {
-    float power[kChunk + 4];                // lam^n
-    float weight[2 * kChunk];               // of tokens kChunk - i apart, times the state's scale; zero for those not seen
-    float come[2 * kChunk];                 // what the state before a whole chunk has kept at row r, times the output's scale (backward in
-                                            // time the rows of a shorter chunk stand behind one another at its end)
+    float left[kChunk + 4];                 // lam^n times the state's scale: what is left of a token that n tokens follow
+    float weight[2 * kChunk];               // of tokens kChunk - i apart, times both scales; zero for those not seen
+    alignas(16) float come[2][kChunk];      // what is left at row r of the state before a whole chunk, and before one of length % kChunk
+                                            // tokens, times the output's scale
     int odd[kRing];
     uint32_t tmem;
     uint64_t full[4], checked[4], scores, scaled, weights, state, far, out, out_free, change, change_free, drained;
@@ -123,7 +123,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t *bar)
     if (threadIdx.x % 32 == 0) mbar_arrive(bar);
 }
 
-__device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+__device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_asleep(bar, parity)); }
 
 template <int NQ, int NV, bool SUMS>
 __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ Maps maps, bool states_only)
@@ -146,12 +146,13 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     const double g = decay_log<float>(a.log_decay, head);
+    const int length = static_cast<int>(item.end - item.begin);
     if (threadIdx.x < 2 * kChunk)
     {
-        const int i = threadIdx.x, near = reverse ? i - kChunk : kChunk - i, come = reverse ? kChunk - 1 - i : i + 1;
-        if (i <= kChunk) sh.power[i] = static_cast<float>(exp(g * i));
-        sh.weight[i] = near >= 0 ? static_cast<float>(exp(g * near) * p.state_scale) : 0.0f;
-        sh.come[i] = come >= 0 ? static_cast<float>(exp(g * come) * p.out_scale) : 0.0f;
+        const int i = threadIdx.x, r = i % kChunk, near = reverse ? i - kChunk : kChunk - i, come = reverse ? (i < kChunk ? kChunk : length % kChunk) - 1 - r : r + 1;
+        if (i <= kChunk) sh.left[i] = static_cast<float>(exp(g * i) * p.state_scale);
+        sh.weight[i] = near >= 0 ? static_cast<float>(exp(g * near) * p.state_scale * p.out_scale) : 0.0f;
+        sh.come[i / kChunk][r] = come >= 0 ? static_cast<float>(exp(g * come) * p.out_scale) : 0.0f;
     }
     if (threadIdx.x < kRing) sh.odd[threadIdx.x] = 0;
     if (threadIdx.x == 0)
@@ -178,7 +179,6 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     __syncthreads();
     tmem_fence_after_sync();
     const uint32_t tmem = sh.tmem;
-    const int length = static_cast<int>(item.end - item.begin);
     const int chunks = (length + kChunk - 1) / kChunk;
     const auto chunk_of = [&](int c) { return reverse ? chunks - 1 - c : c; };
     const auto tokens_of = [&](int c) { return min(kChunk, length - chunk_of(c) * kChunk); };
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                     const int piece = i * 128 + id, r = piece / 8 % kChunk;
                     uint4 x = *reinterpret_cast<const uint4 *>(stage + L::kK + piece * 16);
                     if (r >= m) x = make_uint4(0, 0, 0, 0);     // whatever stands behind the last token
-                    const float w = sh.power[r >= m ? 0 : reverse ? r + 1 : m - 1 - r];
+                    const float w = sh.left[r >= m ? 0 : reverse ? r + 1 : m - 1 - r];
                     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
                     uint32_t part[3][4];
 #pragma unroll
@@ -342,18 +342,25 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             // Rows of V behind the last token become zeros.  So do its infinities and NaN, because a masked weight times one of them would
             // be NaN: where there are any, the rows and states that they do meet get them from the state warps.
             if (id == 0) sh.odd[(c + kRing / 2) % kRing] = 0;
-            bool odd = false;
-#pragma unroll 1
+            uint32_t largest = 0;           // of the magnitudes' bits, in either half
+#pragma unroll 2
             for (int i = 0; i < NV * 4; ++i)
             {
-                const int piece = i * 128 + id, r = piece / 8 % kChunk;
+                const int piece = i * 128 + id;
                 uint4 *at = reinterpret_cast<uint4 *>(stage + L::kV + piece * 16);
+                if (piece / 8 % kChunk >= m) *at = make_uint4(0, 0, 0, 0);
                 const uint4 x = *at;
-                if (r >= m) *at = make_uint4(0, 0, 0, 0);
-                else if (odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w))
+                largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+            }
+            const bool odd = odd_pair(largest);
+            if (__builtin_expect(odd, 0))
+            {
+#pragma unroll 1
+                for (int i = 0; i < NV * 4; ++i)
                 {
+                    uint4 *at = reinterpret_cast<uint4 *>(stage + L::kV + (i * 128 + id) * 16);
+                    const uint4 x = *at;
                     *at = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w));
-                    odd = true;
                 }
             }
             if (odd) sh.odd[c % kRing] = 1;
@@ -367,8 +374,10 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             const int r = warp % 4 * 32 + lane;
             const unsigned first = reverse ? r : 0, seen = reverse ? m - 1 - r : r;     // columns first .. first + seen
             const bool none = reverse && r >= m;
+            // one of the four warps holds a block that no row sees: its zeros stay from the first chunk
+            const bool blank = c > 0 && (reverse ? half * 32 < warp % 4 * 32 : half * 32 > warp % 4 * 32);
 #pragma unroll 1
-            for (int i = half * 4; i < half * 4 + 4; ++i)
+            for (int i = half * 4; i < half * 4 + 4 && !blank; ++i)
             {
                 uint32_t x[8], high[4], low[4];
                 tmem_load_8(tmem + kScores + (static_cast<uint32_t>(warp % 4 * 32) << 16) + i * 8, x);
@@ -438,7 +447,6 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             warp_arrive(&sh.state);
         };
         if (!states_only) publish();
-        const float state_scale = static_cast<float>(p.state_scale), out_scale = static_cast<float>(p.out_scale);
         // rows of `out` are a 32-bit number of bytes apart
         const uint32_t step = static_cast<uint32_t>(p.out.token) * (SUMS ? 4u : 2u);
         char *out = reinterpret_cast<char *>(SUMS ? static_cast<void *>(rows_of<float>(p.out, a, item.sequence, head) + item.begin * p.out.token + b)
@@ -470,8 +478,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                 for (int i = 0; i < 16; i += 2)
                 {
                     const float2 was = make_float2(s[j + i], s[j + i + 1]);
-                    const float2 now = fma2(keeps, was, fma2(rests, was, mul2(make_float2(state_scale, state_scale),
-                                                                              make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])))));
+                    const float2 now = fma2(keeps, was, fma2(rests, was, make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]))));
                     s[j + i] = now.x;
                     s[j + i + 1] = now.y;
                 }
@@ -500,7 +507,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             ok = all_wait(&sh.out, parity);
             if (!ok) break;
             tmem_fence_after_sync();
-            const float *come = sh.come + r0 + (reverse ? kChunk - m : 0);
+            const float *come = sh.come[m < kChunk] + r0;
             char *row = out + static_cast<int64_t>(chunk_of(c) * kChunk + r0) * step;
 #pragma unroll
             for (int h = 0; h < 16; h += 8)
@@ -523,8 +530,8 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < 8; i += 2)
                 {
-                    const float2 o = fma2(make_float2(come[h + i], come[h + i + 1]), make_float2(__uint_as_float(far[i]), __uint_as_float(far[i + 1])),
-                                          mul2(make_float2(out_scale, out_scale), make_float2(__uint_as_float(near[i]), __uint_as_float(near[i + 1]))));
+                    const float2 o = fma2(*reinterpret_cast<const float2 *>(come + h + i), make_float2(__uint_as_float(far[i]), __uint_as_float(far[i + 1])),
+                                          make_float2(__uint_as_float(near[i]), __uint_as_float(near[i + 1])));
                     char *to = row + static_cast<uint64_t>(step) * (h + i), *after = row + static_cast<uint64_t>(step) * (h + i + 1);
                     if (SUMS)
                     {

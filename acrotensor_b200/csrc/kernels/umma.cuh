@@ -87,6 +87,29 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar)
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// mbar_wait for warps that wait for much of their time: a try may suspend the thread for up to a millisecond, so that the waiting
+// warps leave the issue slots to the others.  Bounded like mbar_wait (about a second).
+__device__ __forceinline__ bool mbar_wait_asleep(uint64_t *bar, uint32_t parity)
+{
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long start = clock64();
+    do
+    {
+        uint32_t done;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(parity), "r"(1000000u)
+            : "memory");
+        if (done) return true;
+    } while (clock64() - start < kMbarWaitLimitCycles);
+    return false;
+}
+
 // One box of a four-dimensional array (column, head, token, sequence).
 __device__ __forceinline__ void box_load(void *smem, const CUtensorMap *map, int column, int head, int token, int sequence, uint64_t *bar)
 {
