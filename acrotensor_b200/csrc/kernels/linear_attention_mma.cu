@@ -64,50 +64,44 @@ struct Shared
     uint64_t full[4], checked[4], scores, scaled, weights, state, far, out, out_free, change, change_free, drained;
 };
 
-// Two neighbouring fp32 values in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-    float2 d;
-    asm("{\n"
-        ".reg .b64 x, y, z, w;\n"
-        "mov.b64 x, {%2, %3};\n"
-        "mov.b64 y, {%4, %5};\n"
-        "mov.b64 z, {%6, %7};\n"
-        "fma.rn.f32x2 w, x, y, z;\n"
-        "mov.b64 {%0, %1}, w;\n"
-        "}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
-{
-    float2 d;
-    asm("{\n"
-        ".reg .b64 x, y, w;\n"
-        "mov.b64 x, {%2, %3};\n"
-        "mov.b64 y, {%4, %5};\n"
-        "mul.rn.f32x2 w, x, y;\n"
-        "mov.b64 {%0, %1}, w;\n"
-        "}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
+// Two neighbouring fp32 values in a 64-bit register: one instruction for both.
+typedef unsigned long long Two;
 
-__device__ __forceinline__ uint32_t pack_bf16(float2 x)
+__device__ __forceinline__ Two two(float x, float y)
+{
+    Two d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ Two two(uint32_t x, uint32_t y) { return two(__uint_as_float(x), __uint_as_float(y)); }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
+{
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b)
+{
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float first_of(Two x) { return __uint_as_float(static_cast<uint32_t>(x)); }
+__device__ __forceinline__ float second_of(Two x) { return __uint_as_float(static_cast<uint32_t>(x >> 32)); }
+
+__device__ __forceinline__ uint32_t pack_bf16(Two x)
 {
     uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x.y), "f"(x.x));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(second_of(x)), "f"(first_of(x)));
     return r;
 }
-__device__ __forceinline__ float2 unpack_bf16(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
+__device__ __forceinline__ Two unpack_bf16(uint32_t x) { return two(x << 16, x & 0xffff0000u); }
 
 // The next bf16 part of x: returns it and leaves the remainder.  (Of an infinity the remainder is NaN: sums that meet one are not finite.)
-__device__ __forceinline__ uint32_t take_part(float2 &x)
+__device__ __forceinline__ uint32_t take_part(Two &x)
 {
     const uint32_t part = pack_bf16(x);
-    x = fma2(unpack_bf16(part), make_float2(-1.0f, -1.0f), x);
+    asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(unpack_bf16(part)));
     return part;
 }
 
@@ -326,7 +320,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                     {
-                        float2 y = mul2(unpack_bf16(in[j]), make_float2(w, w));
+                        Two y = mul2(unpack_bf16(in[j]), two(w, w));
                         part[0][j] = take_part(y);
                         part[1][j] = take_part(y);
                         part[2][j] = pack_bf16(y);
@@ -385,10 +379,9 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                 {
-                    float2 z = mul2(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), make_float2(weight[2 * j], weight[2 * j + 1]));
                     // not a product with a zero: the score may be an infinity or NaN of another token
-                    if (i * 8 + 2 * j - first > seen) z.x = 0;
-                    if (i * 8 + 2 * j + 1 - first > seen) z.y = 0;
+                    const uint32_t y0 = i * 8 + 2 * j - first > seen ? 0u : x[2 * j], y1 = i * 8 + 2 * j + 1 - first > seen ? 0u : x[2 * j + 1];
+                    Two z = mul2(two(y0, y1), two(weight[2 * j], weight[2 * j + 1]));
                     high[j] = take_part(z);
                     low[j] = pack_bf16(z);
                 }
@@ -408,7 +401,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         const int b = warp % 4 * 32 + lane, part = warp / 4, d0 = part * PART, r0 = part * 16;
         const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
         const bool used = b < p.dv;
-        float s[PART];
+        Two s[PART / 2];
         const int64_t size = static_cast<int64_t>(p.dq) * p.dv;
         {
             const float *from = nullptr;
@@ -423,8 +416,17 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                 }
             }
 #pragma unroll
-            for (int j = 0; j < PART; ++j)
-                s[j] = from != nullptr && used && d0 + j < p.dq ? (turned ? from[b * p.dq + d0 + j] : from[static_cast<int64_t>(d0 + j) * p.dv + b]) : 0.0f;
+            for (int j = 0; j < PART; j += 2)
+            {
+                float x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                {
+                    const int d = d0 + j + e;
+                    x[e] = from != nullptr && used && d < p.dq ? (turned ? from[b * p.dq + d] : from[static_cast<int64_t>(d) * p.dv + b]) : 0.0f;
+                }
+                s[j / 2] = two(x[0], x[1]);
+            }
         }
         const auto publish = [&]() {
             // the state as the A operand of the next chunk: two bf16 parts, pairs of columns
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                 {
-                    float2 x = make_float2(s[j + 2 * i], s[j + 2 * i + 1]);
+                    Two x = s[j / 2 + i];
                     high[i] = take_part(x);
                     low[i] = pack_bf16(x);
                 }
@@ -468,20 +470,14 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             ok = all_wait(&sh.change, parity);
             if (!ok) break;
             tmem_fence_after_sync();
-            const float2 keeps = make_float2(keep, keep), rests = make_float2(rest, rest);
+            const Two keeps = two(keep, keep), rests = two(rest, rest);
 #pragma unroll
             for (int j = 0; j < PART; j += 16)
             {
                 uint32_t x[16];
                 tmem_load_16(tmem + kDelta + lanes + d0 + j, x);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                {
-                    const float2 was = make_float2(s[j + i], s[j + i + 1]);
-                    const float2 now = fma2(keeps, was, fma2(rests, was, make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]))));
-                    s[j + i] = now.x;
-                    s[j + i + 1] = now.y;
-                }
+                for (int i = 0; i < 16; i += 2) s[(j + i) / 2] = fma2(keeps, s[(j + i) / 2], fma2(rests, s[(j + i) / 2], two(x[i], x[i + 1])));
             }
             tmem_fence_before_sync();
             warp_arrive(&sh.change_free);
@@ -496,7 +492,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                     if (!isfinite(__bfloat162float(v[t * p.v.token]))) odd = reverse ? t : min(odd, t);
                 if (odd >= 0 && odd < kChunk)
 #pragma unroll
-                    for (int j = 0; j < PART; ++j) s[j] = __int_as_float(0x7fffffff);
+                    for (int j = 0; j < PART / 2; ++j) s[j] = ~0ull;
             }
             if (states_only) continue;
             ok = all_wait(&sh.far, parity);         // the old state has been read
@@ -527,24 +523,27 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                         if (reverse ? r0 + h + i <= odd : r0 + h + i >= odd) near[i] = 0x7fffffffu;
                 }
                 const int rows = used ? m - r0 - h : 0;
+                const auto write = [&](bool whole) {
 #pragma unroll
-                for (int i = 0; i < 8; i += 2)
-                {
-                    const float2 o = fma2(*reinterpret_cast<const float2 *>(come + h + i), make_float2(__uint_as_float(far[i]), __uint_as_float(far[i + 1])),
-                                          make_float2(__uint_as_float(near[i]), __uint_as_float(near[i + 1])));
-                    char *to = row + static_cast<uint64_t>(step) * (h + i), *after = row + static_cast<uint64_t>(step) * (h + i + 1);
-                    if (SUMS)
+                    for (int i = 0; i < 8; i += 2)
                     {
-                        if (i < rows) *reinterpret_cast<float *>(to) = o.x;
-                        if (i + 1 < rows) *reinterpret_cast<float *>(after) = o.y;
-                    }
-                    else
-                    {
+                        const Two o = fma2(*reinterpret_cast<const Two *>(come + h + i), two(far[i], far[i + 1]), two(near[i], near[i + 1]));
+                        char *to = row + static_cast<uint64_t>(step) * (h + i), *after = row + static_cast<uint64_t>(step) * (h + i + 1);
                         const uint32_t both = pack_bf16(o);
-                        if (i < rows) *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(both);
-                        if (i + 1 < rows) *reinterpret_cast<uint16_t *>(after) = static_cast<uint16_t>(both >> 16);
+                        if (whole || i < rows)
+                        {
+                            if (SUMS) *reinterpret_cast<float *>(to) = first_of(o);
+                            else *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(both);
+                        }
+                        if (whole || i + 1 < rows)
+                        {
+                            if (SUMS) *reinterpret_cast<float *>(after) = second_of(o);
+                            else *reinterpret_cast<uint16_t *>(after) = static_cast<uint16_t>(both >> 16);
+                        }
                     }
-                }
+                };
+                if (rows >= 8) write(true);
+                else if (rows > 0) write(false);
             }
         }
         if (!ok && lane == 0) *a.wait_flag = 1;
@@ -560,7 +559,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         {
 #pragma unroll
             for (int j = 0; j < PART; ++j)
-                if (d0 + j < p.dq) to[turned ? b * p.dq + d0 + j : static_cast<int64_t>(d0 + j) * p.dv + b] = s[j];
+                if (d0 + j < p.dq) to[turned ? b * p.dq + d0 + j : static_cast<int64_t>(d0 + j) * p.dv + b] = j % 2 ? second_of(s[j / 2]) : first_of(s[j / 2]);
         }
     }
     tmem_fence_before_sync();
