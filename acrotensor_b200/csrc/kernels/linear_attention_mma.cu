@@ -30,9 +30,8 @@ namespace
 constexpr int kChunk = 64;
 constexpr int kBox = kChunk * 128;          // bytes of 64 rows of 64 columns
 // Warps 0 .. 15 keep the state and write `out` (a quarter of the state's columns and of the chunk's rows each, for 32 lanes).
-// Warps 16 .. 23 make operands: those on tensor memory lanes 0 .. 63 the weights, the others K~.  Warp 26 issues copies and products (24 and 25 idle: so the
-// issuing warp shares a scheduler, and its instruction cache, with the short loop of K~ and not with the weights').
-constexpr int kStateWarps = 16, kOperandWarps = 8, kIssueWarp = 26, kBlock = (kIssueWarp + 1) * 32;
+// Warps 16 .. 23 make operands: those on tensor memory lanes 0 .. 63 the weights, the others K~.  Warp 24 issues copies and products.
+constexpr int kStateWarps = 16, kOperandWarps = 8, kIssueWarp = kStateWarps + kOperandWarps, kBlock = (kIssueWarp + 1) * 32;
 constexpr int kRing = 16;                   // slots of the flags that tell of non-finite values; operand warps run at most 5 chunks ahead
 
 // Columns of tensor memory.
@@ -61,7 +60,7 @@ struct Shared
                                             // tokens, times the output's scale
     int odd[kRing];
     uint32_t tmem;
-    uint64_t full[4], checked[4], scores, scaled, weights, state, far, out, out_free, change, change_free, drained;
+    uint64_t full[4], ready[4], scores, weights, state, out, out_free, change, change_free, drained;
 };
 
 // Two neighbouring fp32 values in a 64-bit register: one instruction for both.
@@ -137,7 +136,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     Shared &sh = *reinterpret_cast<Shared *>(smem + L::kTables);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x / 32), 0), lane = threadIdx.x % 32;
 
     const double g = decay_log<float>(a.log_decay, head);
     const int length = static_cast<int>(item.end - item.begin);
@@ -154,14 +153,12 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         for (int i = 0; i < L::kStages; ++i)
         {
             mbar_init(&sh.full[i], 1);
-            mbar_init(&sh.checked[i], kOperandWarps / 2);
+            mbar_init(&sh.ready[i], kOperandWarps);
         }
         mbar_init(&sh.scores, 1);
-        mbar_init(&sh.far, 1);
         mbar_init(&sh.out, 1);
         mbar_init(&sh.change, 1);
         mbar_init(&sh.drained, 1);
-        mbar_init(&sh.scaled, kOperandWarps / 2);
         mbar_init(&sh.weights, kOperandWarps / 2);
         mbar_init(&sh.state, kStateWarps);
         mbar_init(&sh.out_free, kStateWarps);
@@ -172,7 +169,8 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     tmem_fence_before_sync();
     __syncthreads();
     tmem_fence_after_sync();
-    const uint32_t tmem = sh.tmem;
+    // All columns are allocated, so the allocation starts at column zero and addresses are constants.
+    constexpr uint32_t tmem = 0;
     const int chunks = (length + kChunk - 1) / kChunk;
     const auto chunk_of = [&](int c) { return reverse ? chunks - 1 - c : c; };
     const auto tokens_of = [&](int c) { return min(kChunk, length - chunk_of(c) * kChunk); };
@@ -180,39 +178,42 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
 
     if (warp == kIssueWarp)
     {
-        // The whole warp walks the loop, one lane issues: addresses and descriptors stay in uniform registers.
+        // The whole warp walks the loop; only the products and copies themselves are one lane's, by predicate and not by a branch, so
+        // that addresses and descriptors stay in uniform registers (a product costs 30 to 60 cycles of issue less than with a branch).
         const int stage_bytes = states_only ? (NQ + NV) * kBox : L::kStage;
         const int hq = head / p.q.group, hk = head / p.k.group, hv = head / p.v.group, n = a.offsets == nullptr ? static_cast<int>(item.sequence) : 0;
+        const uint32_t leader = elect_lane();
         const auto load = [&](int c) {
             unsigned char *stage = smem + c % L::kStages * L::kStage;
             uint64_t *bar = &sh.full[c % L::kStages];
             const int t = static_cast<int>(item.begin) + chunk_of(c) * kChunk;
-            if (!elect_lane()) return;
-            mbar_arrive_expect_tx(bar, stage_bytes);
-#pragma unroll
-            for (int i = 0; i < NQ; ++i)
+            if (leader)
             {
-                if (!states_only) box_load(stage + L::kQ + i * kBox, &maps.q[pass], i * kBoxColumns, hq, t, n, bar);
-                box_load(stage + L::kK + i * kBox, &maps.k[pass], i * kBoxColumns, hk, t, n, bar);
-            }
+                mbar_arrive_expect_tx(bar, stage_bytes);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) box_load(stage + L::kV + i * kBox, &maps.v[pass], i * kBoxColumns, hv, t, n, bar);
+                for (int i = 0; i < NQ; ++i)
+                {
+                    if (!states_only) box_load(stage + L::kQ + i * kBox, &maps.q[pass], i * kBoxColumns, hq, t, n, bar);
+                    box_load(stage + L::kK + i * kBox, &maps.k[pass], i * kBoxColumns, hk, t, n, bar);
+                }
+#pragma unroll
+                for (int i = 0; i < NV; ++i) box_load(stage + L::kV + i * kBox, &maps.v[pass], i * kBoxColumns, hv, t, n, bar);
+            }
+            __syncwarp();
         };
         int loaded = 0;
         for (; loaded < min(chunks, L::kStages - 1); ++loaded) load(loaded);
         const uint32_t base = smem_addr(smem);
-        const uint32_t by_columns = umma_shape(kChunk, false, false), near_shape = umma_shape(kChunk, true, false),
-                       change_shape = umma_shape(NQ * 64, true, true);
+        constexpr uint32_t by_columns = umma_shape(kChunk, false, false), near_shape = umma_shape(kChunk, true, false),
+                           change_shape = umma_shape(NQ * 64, true, true);
         const uint64_t scaled = umma_operand(base + L::kScaled, kBox, 1024), weights = umma_operand(base + L::kWeights, 16, 1024);
         // descriptors count in units of 16 bytes
         const auto issue_scores = [&](int c) {
             const uint32_t stage = base + c % L::kStages * L::kStage;
             const uint64_t q = umma_operand(stage + L::kQ, 16, 1024), k = umma_operand(stage + L::kK, 16, 1024);
-            if (!elect_lane()) return;
 #pragma unroll
-            for (int i = 0; i < NQ * 4; ++i)
-                umma(tmem + kScores, q + (i / 4 * kBox + i % 4 * 32) / 16, k + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, i > 0);
-            umma_commit(&sh.scores);
+            for (int i = 0; i < NQ * 4; ++i) umma(leader, kScores, q + (i / 4 * kBox + i % 4 * 32) / 16, k + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, i > 0);
+            umma_commit(leader, &sh.scores);
         };
         int c = 0;
         if (!states_only && chunks > 0)
@@ -225,60 +226,47 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         {
             const uint32_t stage = base + c % L::kStages * L::kStage, parity = c & 1;
             const uint64_t q = umma_operand(stage + L::kQ, 16, 1024), v = umma_operand(stage + L::kV, NV == 2 ? kBox : 0, 1024);
-            ok = (!states_only || all_wait(&sh.full[c % L::kStages], c / L::kStages & 1)) && (c == 0 || all_wait(&sh.change_free, parity ^ 1)) &&
-                 all_wait(&sh.checked[c % L::kStages], c / L::kStages & 1) && all_wait(&sh.scaled, parity);
+            // `ready` comes after `full`
+            ok = (c == 0 || all_wait(&sh.change_free, parity ^ 1)) && all_wait(&sh.ready[c % L::kStages], c / L::kStages & 1);
             if (!ok) break;
             tmem_fence_after_sync();
-            if (elect_lane())
-            {
 #pragma unroll
-                for (int part = 0; part < 3; ++part)
+            for (int part = 0; part < 3; ++part)
 #pragma unroll
-                    for (int k = 0; k < kChunk / 16; ++k)
-                        umma(tmem + kDelta, v + k * 2048 / 16, scaled + (part * NQ * kBox + k * 2048) / 16, change_shape, part + k > 0);
-                umma_commit(&sh.change);
-            }
-            __syncwarp();
+                for (int k = 0; k < kChunk / 16; ++k)
+                    umma(leader, kDelta, v + k * 2048 / 16, scaled + (part * NQ * kBox + k * 2048) / 16, change_shape, part + k > 0);
+            umma_commit(leader, &sh.change);
             if (states_only)
             {
                 // the previous chunk's stage is free: its change is complete (its reader was waited for above)
                 if (loaded < chunks) load(loaded++);
                 continue;
             }
-            ok = all_wait(&sh.state, parity) && (c == 0 || all_wait(&sh.out_free, parity ^ 1));
+            // the previous chunk's results have been read, and before that its end state was published
+            ok = c == 0 ? all_wait(&sh.state, 0) : all_wait(&sh.out_free, parity ^ 1);
             if (!ok) break;
-            // so is it here: all of the previous chunk's products were waited for by the readers of their results
-            if (loaded < chunks) load(loaded++);
             tmem_fence_after_sync();
-            if (elect_lane())
-            {
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int i = 0; i < NQ * 4; ++i)
-                        umma_tmem(tmem + kFar, tmem + (part ? kStateLow : kStateHigh) + i * 8, q + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, part + i > 0);
-                umma_commit(&sh.far);
-            }
-            __syncwarp();
+                for (int i = 0; i < NQ * 4; ++i)
+                    umma_tmem(leader, kFar, (part ? kStateLow : kStateHigh) + i * 8, q + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, part + i > 0);
+            // all of the previous chunk's products were waited for by the readers of their results: its stage is free
+            if (loaded < chunks) load(loaded++);
             ok = all_wait(&sh.weights, parity);
             if (!ok) break;
             tmem_fence_after_sync();
-            if (elect_lane())
-            {
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int k = 0; k < kChunk / 16; ++k)
-                        umma(tmem + kNear, v + k * 2048 / 16, weights + (part * kBox + k * 32) / 16, near_shape, part + k > 0);
-                umma_commit(&sh.out);
-            }
-            __syncwarp();
+                for (int k = 0; k < kChunk / 16; ++k)
+                    umma(leader, kNear, v + k * 2048 / 16, weights + (part * kBox + k * 32) / 16, near_shape, part + k > 0);
+            umma_commit(leader, &sh.out);
             if (c + 1 < chunks)
             {
                 ok = all_wait(&sh.full[(c + 1) % L::kStages], (c + 1) / L::kStages & 1);
                 if (!ok) break;
                 issue_scores(c + 1);
-                __syncwarp();
             }
         }
         if (!ok)
@@ -286,12 +274,11 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             if (lane == 0) *a.wait_flag = 1;
             // copies and products of this CTA that are still in flight
             for (int i = c; i < loaded; ++i) all_wait(&sh.full[i % L::kStages], i / L::kStages & 1);
-            if (elect_lane()) umma_commit(&sh.drained);
-            __syncwarp();
+            umma_commit(leader, &sh.drained);
             all_wait(&sh.drained, 0);
         }
     }
-    else if (warp >= kStateWarps && warp < kStateWarps + kOperandWarps)
+    else if (warp >= kStateWarps)
     {
         const bool scores = warp % 4 < 2;
         const int half = (warp - kStateWarps) / 4;
@@ -330,7 +317,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                         *reinterpret_cast<uint4 *>(smem + L::kScaled + k * NQ * kBox + piece * 16) = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
                 }
                 fence_proxy_async();
-                warp_arrive(&sh.scaled);
+                warp_arrive(&sh.ready[c % L::kStages]);
                 continue;
             }
             // Rows of V behind the last token become zeros.  So do its infinities and NaN, because a masked weight times one of them would
@@ -359,7 +346,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             }
             if (odd) sh.odd[c % kRing] = 1;
             fence_proxy_async();
-            warp_arrive(&sh.checked[c % L::kStages]);      // one barrier per stage: these warps may be a few chunks ahead
+            warp_arrive(&sh.ready[c % L::kStages]);        // one barrier per stage: these warps may be a few chunks ahead
             if (states_only) continue;
             // the previous chunk's weights have been read when its results have
             ok = all_wait(&sh.scores, parity) && (c == 0 || all_wait(&sh.out_free, parity ^ 1));
@@ -395,7 +382,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         }
         if (!ok && lane == 0) *a.wait_flag = 1;
     }
-    else if (warp < kStateWarps)
+    else
     {
         // this thread's row of the transposed state, and which quarter of its columns
         const int b = warp % 4 * 32 + lane, part = warp / 4, d0 = part * PART, r0 = part * 16;
@@ -445,10 +432,13 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                 tmem_store_8(tmem + kStateLow + lanes + (d0 + j) / 2, low);
             }
             tmem_wait_stores();
+        };
+        if (!states_only)
+        {
+            publish();
             tmem_fence_before_sync();
             warp_arrive(&sh.state);
-        };
-        if (!states_only) publish();
+        }
         // rows of `out` are a 32-bit number of bytes apart
         const uint32_t step = static_cast<uint32_t>(p.out.token) * (SUMS ? 4u : 2u);
         char *out = reinterpret_cast<char *>(SUMS ? static_cast<void *>(rows_of<float>(p.out, a, item.sequence, head) + item.begin * p.out.token + b)
@@ -495,14 +485,10 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                     for (int j = 0; j < PART / 2; ++j) s[j] = ~0ull;
             }
             if (states_only) continue;
-            ok = all_wait(&sh.far, parity);         // the old state has been read
+            ok = all_wait(&sh.out, parity);         // the old state has been read, too
             if (!ok) break;
             tmem_fence_after_sync();
             publish();
-
-            ok = all_wait(&sh.out, parity);
-            if (!ok) break;
-            tmem_fence_after_sync();
             const float *come = sh.come[m < kChunk] + r0;
             char *row = out + static_cast<int64_t>(chunk_of(c) * kChunk + r0) * step;
 #pragma unroll
@@ -564,7 +550,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     }
     tmem_fence_before_sync();
     __syncthreads();
-    if (warp == kIssueWarp) tmem_free(tmem, kColumns);
+    if (warp == kIssueWarp) tmem_free(sh.tmem, kColumns);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,

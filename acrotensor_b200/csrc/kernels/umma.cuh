@@ -36,8 +36,8 @@ __host__ __device__ constexpr uint32_t umma_shape(int n, bool a_by_rows, bool b_
            static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(128 >> 4) << 24;
 }
 
-// True in one lane of a converged warp.
-__device__ __forceinline__ bool elect_lane()
+// One in one lane of a converged warp (the leader below), zero in the others.
+__device__ __forceinline__ uint32_t elect_lane()
 {
     uint32_t one;
     asm volatile(
@@ -49,37 +49,45 @@ __device__ __forceinline__ bool elect_lane()
         : "=r"(one)
         :
         : "memory");
-    return one != 0;
+    return one;
 }
 
-// D[128 lanes][n columns] (+)= A (16 columns) * B, A and B in shared memory.
-__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add)
+// D[128 lanes][n columns] (+)= A (16 columns) * B, A and B in shared memory; executed by the leader, walked through by its whole warp.
+__device__ __forceinline__ void umma(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add)
 {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, q;\n"
         "setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+        "setp.ne.u32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add)), "r"(leader)
         : "memory");
 }
 
 // The same with A in tensor memory: lane = row of A, a 32-bit column holds two neighbouring entries of the contracted index.
-__device__ __forceinline__ void umma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add)
+__device__ __forceinline__ void umma_tmem(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add)
 {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, q;\n"
         "setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+        "setp.ne.u32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add)), "r"(leader)
         : "memory");
 }
 
-// One arrival on `bar` when every product this thread has issued so far is complete.
-__device__ __forceinline__ void umma_commit(uint64_t *bar)
+// One arrival on `bar` when every product the leader has issued so far is complete.
+__device__ __forceinline__ void umma_commit(uint32_t leader, uint64_t *bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+    asm volatile(
+        "{\n"
+        ".reg .pred q;\n"
+        "setp.ne.u32 q, %1, 0;\n"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+        "}\n" ::"r"(smem_addr(bar)), "r"(leader)
+        : "memory");
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar)
