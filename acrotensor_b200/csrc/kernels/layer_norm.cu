@@ -4,13 +4,17 @@
 //   g = dy w,  dx = rstd (g - sum(g)/W - xhat sum(g xhat)/W),  dw_f = sum_rows dy xhat,  db_f = sum_rows dy
 //
 // Both are bound by HBM: 2 and 3 elements moved per entry against about ten operations.  So a row is read once, stays in
-// registers between its moments and its result, and leaves once.  A row belongs to a group of G threads (whole warps); a CTA
-// holds 256/G groups when rows are short.  The variance is the mean square of the centred entries (a second walk over the
-// registers), not a difference of moments, which cancels for rows far from zero.
+// registers between its moments and its result, and leaves once.  A row belongs to a group of G threads (a power of two up to a warp,
+// or whole warps); a CTA holds several groups when rows are short.  Groups walk over rows and load the next row's
+// bytes before they work on one.  Elements are worked on in pairs, with weight and bias in registers, and a group has a barrier of its
+// own: a row per CTA of 512 threads, element by element, stood at 34 % of the copy rate in bf16 (24 instructions an element).  A ring
+// of rows in shared memory (asynchronous copies, 2 to 4 rows ahead) was slower in every shape but one.  The variance is the mean square of the centred entries (a second walk over the registers), not a
+// difference of moments, which cancels for rows far from zero.
 //
-// The gradient's column sums run over all rows: a thread owns the same columns of every row that its group takes (rows r,
-// r + groups, ...), so the sums over those rows stay in its registers; a group leaves one row of partial sums, and a second
-// kernel adds the groups' rows in ascending order.  No atomics: the same bits on every run on one device.
+// The gradient's column sums run over all rows: a thread owns the same columns of every row that its group takes, so the sums over
+// those rows stay in its registers (in shared memory beyond 16 columns a thread); the groups of a CTA are added in ascending order, a CTA
+// leaves one row of partial sums, and a second kernel adds these in ascending order.  No atomics: the same bits on every run on
+// one device.
 #include "element.cuh"
 
 #include <algorithm>
@@ -20,8 +24,7 @@ using namespace acro_b200_detail;
 namespace
 {
 
-constexpr int kMaxThreads = 512;       // of one group; 32 columns a thread and two sums a column fit the registers of 512 threads
-constexpr int kColumnsMax = 32;        // columns of one thread
+constexpr int kMaxThreads = 512;       // of one group
 constexpr int kWideThreads = 512;
 
 struct NormArgs
@@ -29,31 +32,32 @@ struct NormArgs
     const void *x, *w, *b, *dy;
     void *y;                            // the result, or dx
     void *mean, *rstd;                  // written by the forward pass (or null), read by the gradient
-    void *partial;                      // gradient: [groups][2][width] sums
+    void *partial;                      // gradient: [CTAs][2][width] sums
     int64_t rows, width, x_stride, y_stride, dy_stride;
     double eps;
     int group;                          // threads of one row
 };
 
-// Sum over the threads of a row's group; `slot` is the group's own part of shared memory (one entry per warp), written and
-// read between two barriers of the whole CTA.  Every thread of the CTA calls it.
+// Sum over the threads of a row's group, each of whom calls it.  `slot`: the group's own part of shared memory, one entry per warp.  Two
+// sums in a row use different slots: then everybody has read the one before the last when a barrier lets the next be written.
 template <int N, class A>
 __device__ __forceinline__ void group_sum(A (&v)[N], A *slot, int group)
 {
+    const int within = group < 32 ? group : 32;
+    for (int o = within / 2; o > 0; o >>= 1)
+    {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
     const int warps = group / 32;
-    if (warps == 1) return;
+    if (warps <= 1) return;
     const int warp = (threadIdx.x % group) / 32;
-    __syncthreads();                    // the previous sum's entries have been read
     if (threadIdx.x % 32 == 0)
     {
 #pragma unroll
         for (int i = 0; i < N; ++i) slot[warp * N + i] = v[i];
     }
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / group), "r"(group) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0;
     for (int k = 0; k < warps; ++k)
@@ -63,99 +67,70 @@ __device__ __forceinline__ void group_sum(A (&v)[N], A *slot, int group)
     }
 }
 
-// The columns of thread `lane` of a group of `group` threads: packs lane, lane + group, ... of VEC columns.
-template <class T, int VEC, int COLS, class A>
-__device__ __forceinline__ void load_row(A (&v)[COLS], const T *row, int lane, int group, int64_t width, A missing)
-{
-    Pack<T, VEC> p[COLS / VEC];
-#pragma unroll
-    for (int k = 0; k < COLS / VEC; ++k)
-    {
-        const int64_t c = (static_cast<int64_t>(k) * group + lane) * VEC;
-        if (c < width) p[k] = *reinterpret_cast<const Pack<T, VEC> *>(row + c);
-    }
-#pragma unroll
-    for (int k = 0; k < COLS / VEC; ++k)
-    {
-        const bool there = (static_cast<int64_t>(k) * group + lane) * VEC < width;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[k * VEC + j] = there ? static_cast<A>(widen(p[k].x[j])) : missing;
-    }
-}
-
-template <class T, int VEC, int COLS, class A>
-__device__ __forceinline__ void store_row(const A (&v)[COLS], T *row, int lane, int group, int64_t width)
-{
-#pragma unroll
-    for (int k = 0; k < COLS / VEC; ++k)
-    {
-        const int64_t c = (static_cast<int64_t>(k) * group + lane) * VEC;
-        if (c >= width) continue;
-        Pack<T, VEC> p;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) p.x[j] = narrow<T>(v[k * VEC + j]);
-        *reinterpret_cast<Pack<T, VEC> *>(row + c) = p;
-    }
-}
-
-template <class T, int VEC, int COLS>
-__global__ void __launch_bounds__(kMaxThreads) norm_kernel(NormArgs a)
+// THREADS: the largest CTA (256 when rows are short enough: twice the registers a thread).
+template <class T, int VEC, int COLS, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_kernel(NormArgs a)
 {
     using A = typename Element<T>::Acc;
-    __shared__ A slots[kMaxThreads / 32];
-    const int groups = blockDim.x / a.group, mine = threadIdx.x / a.group, lane = threadIdx.x % a.group;
-    A *slot = slots + mine * (a.group / 32);
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * groups + mine;
-    const bool there = row < a.rows;
-    const A inv = A(1) / static_cast<A>(a.width);
-    A x[COLS];
-    if (there) load_row<T, VEC, COLS>(x, static_cast<const T *>(a.x) + row * a.x_stride, lane, a.group, a.width, A(0));
-    else
-#pragma unroll
-        for (int i = 0; i < COLS; ++i) x[i] = 0;
-    A s[1] = {0};
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) s[0] += x[i];
-    group_sum(s, slot, a.group);
-    const A mean = s[0] * inv;
-    s[0] = 0;
-#pragma unroll
-    for (int k = 0; k < COLS / VEC; ++k)
+    using P = typename PairOf<A>::type;
+    using Row = RowPart<T, VEC, COLS>;
+    __shared__ A slots[2][THREADS / 32];
+    const int groups = blockDim.x / a.group, mine = threadIdx.x / a.group, lane = threadIdx.x % a.group, width = static_cast<int>(a.width);
+    const int slot = mine * (a.group / 32);
+    const A inv = A(1) / static_cast<A>(width);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+    int64_t base = static_cast<int64_t>(blockIdx.x) * groups;
+    // the thread's columns of weight and bias stay in registers (one and zero where there are none)
+    Row next, weight, bias;
+    const auto fetch = [&](int64_t row) {
+        if (row < a.rows) next.load(static_cast<const T *>(a.x) + row * a.x_stride, lane, a.group, width);
+    };
+    fetch(base + mine);
+    if (a.w != nullptr) weight.load(static_cast<const T *>(a.w), lane, a.group, width);
+    else weight.fill(narrow2<T>(two(A(1), A(1))));
+    if (a.b != nullptr) bias.load(static_cast<const T *>(a.b), lane, a.group, width);
+    else bias.fill(narrow2<T>(two(A(0), A(0))));
+    for (; base < a.rows; base += step)
     {
-        if ((static_cast<int64_t>(k) * a.group + lane) * VEC >= a.width) continue;
+        const int64_t row = base + mine;
+        const bool there = row < a.rows;
+        P x[COLS / 2], sum = two(A(0), A(0));
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
+        for (int k = 0; k < COLS / 2; ++k)
         {
-            x[k * VEC + j] -= mean;
-            s[0] += x[k * VEC + j] * x[k * VEC + j];
+            x[k] = widen2<T>(next.pair[k]);
+            sum = add2(sum, x[k]);
         }
-    }
-    group_sum(s, slot, a.group);
-    const A rstd = A(1) / sqrt(s[0] * inv + static_cast<A>(a.eps));
-    if (!there) return;
-    if (lane == 0)
-    {
-        if (a.mean != nullptr) static_cast<A *>(a.mean)[row] = mean;
-        if (a.rstd != nullptr) static_cast<A *>(a.rstd)[row] = rstd;
-    }
+        fetch(row + step);
+        A s[1] = {first_of(sum) + second_of(sum)};
+        group_sum(s, slots[0] + slot, a.group);
+        const A mean = s[0] * inv;
+        const P means = two(mean, mean);
+        sum = two(A(0), A(0));
 #pragma unroll
-    for (int k = 0; k < COLS / VEC; ++k)
-    {
-        const int64_t c = (static_cast<int64_t>(k) * a.group + lane) * VEC;
-        if (c >= a.width) continue;
-        Pack<T, VEC> w, b;
-        if (a.w != nullptr) w = *reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.w) + c);
-        if (a.b != nullptr) b = *reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.b) + c);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
+        for (int k = 0; k < COLS / 2; ++k)
         {
-            A v = x[k * VEC + j] * rstd;
-            if (a.w != nullptr) v *= widen(w.x[j]);
-            if (a.b != nullptr) v += widen(b.x[j]);
-            x[k * VEC + j] = v;
+            const bool one = Row::column(k, 0, lane, a.group) < width, other = Row::column(k, 1, lane, a.group) < width;
+            x[k] = sub2(x[k], means);
+            if (VEC == 1 && !other) x[k] = two(first_of(x[k]), A(0));
+            if (!one) x[k] = two(A(0), A(0));
+            sum = fma2(x[k], x[k], sum);
         }
+        s[0] = first_of(sum) + second_of(sum);
+        group_sum(s, slots[1] + slot, a.group);
+        const A rstd = A(1) / sqrt(s[0] * inv + static_cast<A>(a.eps));
+        if (!there) continue;
+        if (lane == 0)
+        {
+            if (a.mean != nullptr) static_cast<A *>(a.mean)[row] = mean;
+            if (a.rstd != nullptr) static_cast<A *>(a.rstd)[row] = rstd;
+        }
+        const P scale = two(rstd, rstd);
+        Row out;
+#pragma unroll
+        for (int k = 0; k < COLS / 2; ++k) out.pair[k] = narrow2<T>(fma2(mul2(x[k], scale), widen2<T>(weight.pair[k]), widen2<T>(bias.pair[k])));
+        out.store(static_cast<T *>(a.y) + row * a.y_stride, lane, a.group, width);
     }
-    store_row<T, VEC, COLS>(x, static_cast<T *>(a.y) + row * a.y_stride, lane, a.group, a.width);
 }
 
 // Rows wider than a group's registers hold: three walks over the row, the later two mostly from L2.
@@ -163,13 +138,13 @@ template <class T>
 __global__ void __launch_bounds__(kWideThreads) norm_wide_kernel(NormArgs a)
 {
     using A = typename Element<T>::Acc;
-    __shared__ A slot[kWideThreads / 32];
+    __shared__ A slots[2][kWideThreads / 32];
     const int64_t row = blockIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
     const A inv = A(1) / static_cast<A>(a.width);
     A s[1] = {0};
     for (int64_t c = threadIdx.x; c < a.width; c += kWideThreads) s[0] += widen(x[c]);
-    group_sum(s, slot, kWideThreads);
+    group_sum(s, slots[0], kWideThreads);
     const A mean = s[0] * inv;
     s[0] = 0;
     for (int64_t c = threadIdx.x; c < a.width; c += kWideThreads)
@@ -177,7 +152,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_kernel(NormArgs a)
         const A d = widen(x[c]) - mean;
         s[0] += d * d;
     }
-    group_sum(s, slot, kWideThreads);
+    group_sum(s, slots[1], kWideThreads);
     const A rstd = A(1) / sqrt(s[0] * inv + static_cast<A>(a.eps));
     if (threadIdx.x == 0)
     {
@@ -194,72 +169,133 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_kernel(NormArgs a)
     }
 }
 
-template <class T, int VEC, int COLS>
-__global__ void __launch_bounds__(kMaxThreads) norm_gradient_kernel(NormArgs a)
+// Up to 16 columns a thread the column sums are registers; beyond that each thread keeps its own in shared memory (sums[2][width],
+// touched by their owner alone until the end).
+template <class T, int VEC, int COLS, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_gradient_kernel(NormArgs a)
 {
     using A = typename Element<T>::Acc;
-    __shared__ A slots[2 * kMaxThreads / 32];
-    const int groups = blockDim.x / a.group, mine = threadIdx.x / a.group, lane = threadIdx.x % a.group;
-    A *slot = slots + mine * (a.group / 32) * 2;
-    const A inv = A(1) / static_cast<A>(a.width);
-    A dw[COLS], db[COLS];
+    using P = typename PairOf<A>::type;
+    using Row = RowPart<T, VEC, COLS>;
+    constexpr bool kRegisters = COLS <= 16;
+    constexpr int kSums = kRegisters ? COLS / 2 : 1;
+    __shared__ A slots[2][2 * THREADS / 32];
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    // pair k of thread t at entry k * threads + t (dw, then db), or [2][width] when groups are added up
+    P *own = reinterpret_cast<P *>(dynamic);
+    A *sums = reinterpret_cast<A *>(own);
+    const int groups = blockDim.x / a.group, mine = threadIdx.x / a.group, lane = threadIdx.x % a.group, width = static_cast<int>(a.width);
+    const int slot = mine * (a.group / 32) * 2;
+    int turn = 0;
+    const A inv = A(1) / static_cast<A>(width);
+    P dw[kSums], db[kSums];
 #pragma unroll
-    for (int i = 0; i < COLS; ++i) dw[i] = db[i] = 0;
+    for (int k = 0; k < kSums; ++k) dw[k] = db[k] = two(A(0), A(0));
+    if constexpr (!kRegisters)
+    {
+#pragma unroll
+        for (int k = 0; k < COLS; ++k) own[k * blockDim.x + threadIdx.x] = two(A(0), A(0));
+    }
     const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * groups; base < a.rows; base += step)
+    int64_t base = static_cast<int64_t>(blockIdx.x) * groups;
+    Row next_x, next_g, weight;
+    A next_mean = 0, next_rstd = 0;
+    const auto fetch = [&](int64_t row) {
+        if (row >= a.rows) return;
+        next_x.load(static_cast<const T *>(a.x) + row * a.x_stride, lane, a.group, width);
+        next_g.load(static_cast<const T *>(a.dy) + row * a.dy_stride, lane, a.group, width);
+        next_mean = static_cast<const A *>(a.mean)[row];
+        next_rstd = static_cast<const A *>(a.rstd)[row];
+    };
+    fetch(base + mine);
+    if (a.w != nullptr) weight.load(static_cast<const T *>(a.w), lane, a.group, width);
+    else weight.fill(narrow2<T>(two(A(1), A(1))));
+    for (; base < a.rows; base += step)
     {
         const int64_t row = base + mine;
         const bool there = row < a.rows;
-        A x[COLS], g[COLS], s[2] = {0, 0}, rstd = 0;
+        P x[COLS / 2], g[COLS / 2], sum_g = two(A(0), A(0)), sum_gx = sum_g;
+        const A rstd = next_rstd;
         if (there)
         {
-            load_row<T, VEC, COLS>(x, static_cast<const T *>(a.x) + row * a.x_stride, lane, a.group, a.width, A(0));
-            load_row<T, VEC, COLS>(g, static_cast<const T *>(a.dy) + row * a.dy_stride, lane, a.group, a.width, A(0));
-            const A mean = static_cast<const A *>(a.mean)[row];
-            rstd = static_cast<const A *>(a.rstd)[row];
+            const P means = two(next_mean, next_mean), scale = two(rstd, rstd);
 #pragma unroll
-            for (int k = 0; k < COLS / VEC; ++k)
+            for (int k = 0; k < COLS / 2; ++k)
             {
-                const int64_t c = (static_cast<int64_t>(k) * a.group + lane) * VEC;
-                if (c >= a.width) continue;
-                Pack<T, VEC> w;
-                if (a.w != nullptr) w = *reinterpret_cast<const Pack<T, VEC> *>(static_cast<const T *>(a.w) + c);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
+                // columns behind the width have dy = 0 and weigh nothing
+                const P dy = widen2<T>(next_g.pair[k]);
+                x[k] = mul2(sub2(widen2<T>(next_x.pair[k]), means), scale);
+                if constexpr (kRegisters)
                 {
-                    const int i = k * VEC + j;
-                    x[i] = (x[i] - mean) * rstd;
-                    db[i] += g[i];
-                    dw[i] += g[i] * x[i];
-                    if (a.w != nullptr) g[i] *= widen(w.x[j]);
-                    s[0] += g[i];
-                    s[1] += g[i] * x[i];
+                    db[k] = add2(db[k], dy);
+                    dw[k] = fma2(dy, x[k], dw[k]);
                 }
+                else
+                {
+                    P &w = own[k * blockDim.x + threadIdx.x], &b = own[(COLS / 2 + k) * blockDim.x + threadIdx.x];
+                    w = fma2(dy, x[k], w);
+                    b = add2(b, dy);
+                }
+                g[k] = mul2(dy, widen2<T>(weight.pair[k]));
+                sum_g = add2(sum_g, g[k]);
+                sum_gx = fma2(g[k], x[k], sum_gx);
             }
         }
-        group_sum(s, slot, a.group);
+        fetch(row + step);
+        A s[2] = {first_of(sum_g) + second_of(sum_g), first_of(sum_gx) + second_of(sum_gx)};
+        group_sum(s, slots[turn] + slot, a.group);
+        turn ^= 1;
         if (there)
         {
-            s[0] *= inv;
-            s[1] *= inv;
+            const P mean_g = two(s[0] * inv, s[0] * inv), mean_gx = two(-s[1] * inv, -s[1] * inv), scale = two(rstd, rstd);
+            Row out;
 #pragma unroll
-            for (int i = 0; i < COLS; ++i) x[i] = rstd * (g[i] - s[0] - x[i] * s[1]);
-            store_row<T, VEC, COLS>(x, static_cast<T *>(a.y) + row * a.y_stride, lane, a.group, a.width);
+            for (int k = 0; k < COLS / 2; ++k) out.pair[k] = narrow2<T>(mul2(scale, fma2(x[k], mean_gx, sub2(g[k], mean_g))));
+            out.store(static_cast<T *>(a.y) + row * a.y_stride, lane, a.group, width);
         }
     }
     if (a.partial == nullptr) return;
-    A *out = static_cast<A *>(a.partial) + (static_cast<int64_t>(blockIdx.x) * groups + mine) * 2 * a.width;
-#pragma unroll
-    for (int k = 0; k < COLS / VEC; ++k)
+    A *out = static_cast<A *>(a.partial) + static_cast<int64_t>(blockIdx.x) * 2 * width;
+    if constexpr (!kRegisters)
     {
-        const int64_t c = (static_cast<int64_t>(k) * a.group + lane) * VEC;
-        if (c >= a.width) continue;
+        // rows this wide have one group: the columns are this thread's alone
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
+        for (int k = 0; k < COLS / 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                const int c = Row::column(k, e, lane, a.group);
+                if (c >= width) continue;
+                const P w = own[k * blockDim.x + threadIdx.x], b = own[(COLS / 2 + k) * blockDim.x + threadIdx.x];
+                out[c] = e ? second_of(w) : first_of(w);
+                out[width + c] = e ? second_of(b) : first_of(b);
+            }
+        return;
+    }
+    else
+    {
+        // the groups' sums, one group after the other
+        for (int one = 0; one < groups; ++one)
         {
-            out[c + j] = dw[k * VEC + j];
-            out[a.width + c + j] = db[k * VEC + j];
+            if (mine == one)
+            {
+                A *to = groups == 1 ? out : sums;
+#pragma unroll
+                for (int k = 0; k < kSums; ++k)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                    {
+                        const int c = Row::column(k, e, lane, a.group);
+                        if (c >= width) continue;
+                        const A w = e ? second_of(dw[k]) : first_of(dw[k]), b = e ? second_of(db[k]) : first_of(db[k]);
+                        to[c] = one == 0 ? w : to[c] + w;
+                        to[width + c] = one == 0 ? b : to[width + c] + b;
+                    }
+            }
+            __syncthreads();
         }
+        if (groups > 1)
+            for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) out[c] = sums[c];
     }
 }
 
@@ -308,19 +344,20 @@ __global__ void __launch_bounds__(256) norm_columns_wide_kernel(NormArgs a)
     out[a.width + c] = db;
 }
 
-// out[c] = sum over the parts, in ascending order within each of the 16 threads of a column and then over those threads.
+// out[c] = sum over the parts, in ascending order within each of the 32 threads of a column and then over those threads.
 template <class A>
-__global__ void __launch_bounds__(512) norm_combine_kernel(const A *partial, A *dw, A *db, int parts, int64_t width)
+__global__ void __launch_bounds__(1024) norm_combine_kernel(const A *partial, A *dw, A *db, int parts, int64_t width)
 {
-    __shared__ A sums[16][33];
+    __shared__ A sums[32][33];
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;      // over 2 * width: the sums of dw, then those of db
     A s = 0;
     if (c < 2 * width)
-        for (int p = threadIdx.y; p < parts; p += 16) s += partial[static_cast<int64_t>(p) * 2 * width + c];
+#pragma unroll 8
+        for (int p = threadIdx.y; p < parts; p += 32) s += partial[static_cast<int64_t>(p) * 2 * width + c];
     sums[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y != 0 || c >= 2 * width) return;
-    for (int k = 1; k < 16; ++k) s += sums[k][threadIdx.x];
+    for (int k = 1; k < 32; ++k) s += sums[k][threadIdx.x];
     if (c < width)
     {
         if (dw != nullptr) dw[c] = s;
@@ -335,58 +372,96 @@ struct Shape
     int groups() const { return threads / group; }
 };
 
-// Columns a thread: 8, 16 or 32 of them, by whether a group of at most 512 threads then covers the row.
-Shape norm_shape(int type, int64_t width, bool vectors)
+int sms() { return sm_count() > 0 ? sm_count() : 148; }
+
+// Columns a thread: as many as give it 64 bytes of a row (the gradient, which reads two rows: 32), at least 8, as long as the threads
+// then still fill the GPU; fewer for few rows, down to 8; more when 512 threads would not cover the row.  (16384 x 4096 in bf16, 8 / 16 / 32
+// columns: forward 99 / 68 / 58 us, gradient 126 / 93 us; in fp32 the gradient takes 157 / 168 us with 8 / 16.)
+Shape norm_shape(int type, int64_t rows, int64_t width, bool vectors, bool gradient)
 {
     Shape s;
     s.vec = vectors ? static_cast<int>(16 / element_bytes(type)) : 1;
-    s.cols = width <= 8 * kMaxThreads ? 8 : width <= 16 * kMaxThreads ? 16 : 32;
-    if (width > static_cast<int64_t>(kColumnsMax) * kMaxThreads) s.cols = 0;
-    if (s.cols == 0)
+    const int most = type == ACRO_B200_F64 ? 16 : 32;
+    s.cols = std::max(8, static_cast<int>((gradient ? 32 : 64) / element_bytes(type)));
+    while (s.cols > 8 && rows * width / s.cols < static_cast<int64_t>(sms()) * 512) s.cols /= 2;
+    while (s.cols < most && width > static_cast<int64_t>(s.cols) * kMaxThreads) s.cols *= 2;
+    if (width > static_cast<int64_t>(s.cols) * kMaxThreads)
     {
+        s.cols = 0;
         s.group = s.threads = kWideThreads;
         return s;
     }
-    s.group = static_cast<int>((width + s.cols - 1) / s.cols + 31) / 32 * 32;
+    const int lanes = static_cast<int>((width + s.cols - 1) / s.cols);
+    s.group = 1;
+    while (s.group < lanes && s.group < 32) s.group *= 2;
+    if (lanes > 32) s.group = (lanes + 31) / 32 * 32;
     s.threads = s.group <= 128 ? 256 / s.group * s.group : s.group;
     return s;
 }
 
-// CTAs of the gradient (and of the wide rows' column sums): enough to fill the GPU, few enough that their partial sums stay
-// small against the rows.
-int gradient_parts(int64_t rows, const Shape &s)
+// CTAs that walk over the rows: as many as are resident at once, and no more than rows need.
+int norm_grid(int64_t rows, const Shape &s, int per_sm)
 {
-    const int sms = sm_count() > 0 ? sm_count() : 148;
-    const int64_t most = static_cast<int64_t>(sms) * (s.cols == 0 ? 1 : std::max(1, 1024 / s.threads));
-    const int64_t need = s.cols == 0 ? rows : (rows + s.groups() - 1) / s.groups();
+    const int64_t most = static_cast<int64_t>(sms()) * std::max(1, per_sm), need = (rows + s.groups() - 1) / s.groups();
     return static_cast<int>(std::max<int64_t>(1, std::min(most, need)));
 }
 
-template <class T, int VEC>
-void launch_norm(const Shape &s, const NormArgs &a, bool gradient, int grid, cudaStream_t stream)
+// Rows of partial sums: the gradient's CTAs (512 threads an SM: 768 and 1024 were slower in every shape measured), or the slabs of rows
+// of the wide rows' column sums.
+int gradient_parts(int64_t rows, const Shape &s)
 {
-    if (gradient)
+    if (s.cols == 0) return static_cast<int>(std::min<int64_t>(rows, sms()));
+    return norm_grid(rows, s, 512 / s.threads);
+}
+
+template <class T, int VEC, int COLS, int THREADS>
+int launch(const Shape &s, const NormArgs &a, bool gradient, cudaStream_t stream)
+{
+    const char *name = gradient ? "acro_b200_layer_norm_backward" : "acro_b200_layer_norm";
+    if (!gradient)
     {
-        if (s.cols == 8) norm_gradient_kernel<T, VEC, 8><<<grid, s.threads, 0, stream>>>(a);
-        else if (s.cols == 16) norm_gradient_kernel<T, VEC, 16><<<grid, s.threads, 0, stream>>>(a);
-        else norm_gradient_kernel<T, VEC, 32><<<grid, s.threads, 0, stream>>>(a);
+        int resident = 1;
+        const cudaError_t status = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, norm_kernel<T, VEC, COLS, THREADS>, s.threads, 0);
+        if (status != cudaSuccess) return fail_cuda(status, name);
+        norm_kernel<T, VEC, COLS, THREADS><<<norm_grid(a.rows, s, resident), s.threads, 0, stream>>>(a);
+        return launch_status(name);
     }
-    else
+    // gradients of 32 columns a thread have CTAs of more than 256 threads
+    if constexpr (COLS <= 16 || THREADS > 256)
     {
-        if (s.cols == 8) norm_kernel<T, VEC, 8><<<grid, s.threads, 0, stream>>>(a);
-        else if (s.cols == 16) norm_kernel<T, VEC, 16><<<grid, s.threads, 0, stream>>>(a);
-        else norm_kernel<T, VEC, 32><<<grid, s.threads, 0, stream>>>(a);
+        const int smem = COLS > 16 ? COLS * s.threads * 2 * static_cast<int>(sizeof(typename Element<T>::Acc))
+                                   : s.groups() > 1 ? 2 * static_cast<int>(a.width * sizeof(typename Element<T>::Acc)) : 0;
+        cudaError_t status = cudaFuncSetAttribute(norm_gradient_kernel<T, VEC, COLS, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (status != cudaSuccess) return fail_cuda(status, name);
+        norm_gradient_kernel<T, VEC, COLS, THREADS><<<gradient_parts(a.rows, s), s.threads, smem, stream>>>(a);
     }
+    return launch_status(name);
+}
+
+template <class T, int VEC>
+int launch_norm(const Shape &s, const NormArgs &a, bool gradient, cudaStream_t stream)
+{
+    if (s.threads <= 256)
+    {
+        if (s.cols == 8) return launch<T, VEC, 8, 256>(s, a, gradient, stream);
+        if (s.cols == 16) return launch<T, VEC, 16, 256>(s, a, gradient, stream);
+        if constexpr (sizeof(T) == 2) return launch<T, VEC, 32, 256>(s, a, gradient, stream);
+    }
+    if (s.cols == 8) return launch<T, VEC, 8, 512>(s, a, gradient, stream);
+    if (s.cols == 16) return launch<T, VEC, 16, 512>(s, a, gradient, stream);
+    if constexpr (sizeof(T) < 8) return launch<T, VEC, 32, 512>(s, a, gradient, stream);
+    return fail_unsupported("layer norm: no kernel for this shape");
 }
 
 template <class T>
 int forward_of(const Shape &s, const NormArgs &a, cudaStream_t stream)
 {
-    const int64_t grid = s.cols == 0 ? a.rows : (a.rows + s.groups() - 1) / s.groups();
-    if (s.cols == 0) norm_wide_kernel<T><<<static_cast<unsigned>(grid), kWideThreads, 0, stream>>>(a);
-    else if (s.vec == 1) launch_norm<T, 1>(s, a, false, static_cast<int>(grid), stream);
-    else launch_norm<T, 16 / sizeof(T)>(s, a, false, static_cast<int>(grid), stream);
-    return launch_status("acro_b200_layer_norm");
+    if (s.cols == 0)
+    {
+        norm_wide_kernel<T><<<static_cast<unsigned>(a.rows), kWideThreads, 0, stream>>>(a);
+        return launch_status("acro_b200_layer_norm");
+    }
+    return s.vec == 1 ? launch_norm<T, 1>(s, a, false, stream) : launch_norm<T, 16 / sizeof(T)>(s, a, false, stream);
 }
 
 template <class T>
@@ -394,19 +469,20 @@ int gradient_of(const Shape &s, const NormArgs &a, void *dw, void *db, cudaStrea
 {
     using A = typename Element<T>::Acc;
     const int parts = gradient_parts(a.rows, s);
-    int rows_of_sums = parts * s.groups();
     if (s.cols == 0)
     {
         norm_gradient_wide_kernel<T><<<static_cast<unsigned>(a.rows), kWideThreads, 0, stream>>>(a);
         if (a.partial != nullptr)
             norm_columns_wide_kernel<T><<<dim3(static_cast<unsigned>((a.width + 255) / 256), parts), 256, 0, stream>>>(a);
-        rows_of_sums = parts;
     }
-    else if (s.vec == 1) launch_norm<T, 1>(s, a, true, parts, stream);
-    else launch_norm<T, 16 / sizeof(T)>(s, a, true, parts, stream);
+    else
+    {
+        const int status = s.vec == 1 ? launch_norm<T, 1>(s, a, true, stream) : launch_norm<T, 16 / sizeof(T)>(s, a, true, stream);
+        if (status != ACRO_B200_OK) return status;
+    }
     if (a.partial != nullptr)
-        norm_combine_kernel<A><<<static_cast<unsigned>((2 * a.width + 31) / 32), dim3(32, 16), 0, stream>>>(
-            static_cast<const A *>(a.partial), static_cast<A *>(dw), static_cast<A *>(db), rows_of_sums, a.width);
+        norm_combine_kernel<A><<<static_cast<unsigned>((2 * a.width + 31) / 32), dim3(32, 32), 0, stream>>>(
+            static_cast<const A *>(a.partial), static_cast<A *>(dw), static_cast<A *>(db), parts, a.width);
     return launch_status("acro_b200_layer_norm_backward");
 }
 
@@ -445,7 +521,7 @@ int acro_b200_layer_norm(int type, const void *x, int64_t x_stride, const void *
     if (x == y && x_stride != y_stride) return fail_invalid("acro_b200_layer_norm: in place, but with different row strides");
     if (!on_current_device(x) || !on_current_device(y)) return fail_invalid("acro_b200_layer_norm: a pointer is not memory of the current device");
     NormArgs a = {x, weight, bias, nullptr, y, mean, rstd, nullptr, rows, width, x_stride, y_stride, 0, eps, 0};
-    const Shape s = norm_shape(type, width, packs_fit(type, width, {x, weight, bias, y}, {x_stride, y_stride}));
+    const Shape s = norm_shape(type, rows, width, packs_fit(type, width, {x, weight, bias, y}, {x_stride, y_stride}), false);
     a.group = s.group;
     cudaStream_t st = as_stream(stream);
     if (type == ACRO_B200_F64) return forward_of<double>(s, a, st);
@@ -456,14 +532,9 @@ int acro_b200_layer_norm(int type, const void *x, int64_t x_stride, const void *
 size_t acro_b200_layer_norm_backward_scratch_bytes(int type, int64_t rows, int64_t width)
 {
     if (shape_fault(type, rows, width) != nullptr || rows == 0) return 0;
-    size_t most = 0;
-    for (int vectors = 0; vectors < 2; ++vectors)
-    {
-        const Shape s = norm_shape(type, width, vectors != 0);
-        const size_t sums = static_cast<size_t>(gradient_parts(rows, s)) * (s.cols == 0 ? 1 : s.groups());
-        most = std::max(most, sums * 2 * static_cast<size_t>(width) * statistic_bytes(type));
-    }
-    return most;
+    // independent of whether packs of 16 bytes will fit
+    const Shape s = norm_shape(type, rows, width, true, true);
+    return static_cast<size_t>(gradient_parts(rows, s)) * 2 * static_cast<size_t>(width) * statistic_bytes(type);
 }
 
 int acro_b200_layer_norm_backward(int type, const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const void *weight, const void *mean,
@@ -490,10 +561,10 @@ int acro_b200_layer_norm_backward(int type, const void *dy, int64_t dy_stride, c
         return fail_invalid(std::string(name) + "in place, but with different row strides");
     if (!on_current_device(dy) || !on_current_device(x) || !on_current_device(dx))
         return fail_invalid(std::string(name) + "a pointer is not memory of the current device");
-    const Shape s = norm_shape(type, width, packs_fit(type, width, {x, weight, dy, dx}, {x_stride, dy_stride, dx_stride}));
+    const Shape s = norm_shape(type, rows, width, packs_fit(type, width, {x, weight, dy, dx}, {x_stride, dy_stride, dx_stride}), true);
     const bool sums = dweight != nullptr || dbias != nullptr;
     if (sums && s.cols == 0 && (dx == x || dx == dy))
-        return fail_invalid(std::string(name) + "rows wider than 16384 cannot be overwritten in place (their column sums are a second walk)");
+        return fail_invalid(std::string(name) + "rows wider than 16384 (fp64: 8192) cannot be overwritten in place (their column sums are a second walk)");
     if (sums && (scratch == nullptr || scratch_bytes < acro_b200_layer_norm_backward_scratch_bytes(type, rows, width)))
         return fail_invalid(std::string(name) + "scratch is smaller than acro_b200_layer_norm_backward_scratch_bytes");
     if (sums && (!aligned16(scratch) || !on_current_device(scratch)))

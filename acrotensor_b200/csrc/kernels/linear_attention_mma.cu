@@ -63,44 +63,11 @@ struct Shared
     uint64_t full[4], ready[4], scores, weights, state, out, out_free, change, change_free, drained;
 };
 
-// Two neighbouring fp32 values in a 64-bit register: one instruction for both.
-typedef unsigned long long Two;
-
-__device__ __forceinline__ Two two(float x, float y)
-{
-    Two d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-    return d;
-}
-__device__ __forceinline__ Two two(uint32_t x, uint32_t y) { return two(__uint_as_float(x), __uint_as_float(y)); }
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
-{
-    Two d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b)
-{
-    Two d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float first_of(Two x) { return __uint_as_float(static_cast<uint32_t>(x)); }
-__device__ __forceinline__ float second_of(Two x) { return __uint_as_float(static_cast<uint32_t>(x >> 32)); }
-
-__device__ __forceinline__ uint32_t pack_bf16(Two x)
-{
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(second_of(x)), "f"(first_of(x)));
-    return r;
-}
-__device__ __forceinline__ Two unpack_bf16(uint32_t x) { return two(x << 16, x & 0xffff0000u); }
-
 // The next bf16 part of x: returns it and leaves the remainder.  (Of an infinity the remainder is NaN: sums that meet one are not finite.)
 __device__ __forceinline__ uint32_t take_part(Two &x)
 {
     const uint32_t part = pack_bf16(x);
-    asm("sub.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(unpack_bf16(part)));
+    x = sub2(x, unpack_bf16(part));
     return part;
 }
 

@@ -467,7 +467,7 @@ int acro_b200_layer_norm(int type, const void *x, int64_t x_stride, const void *
 /* Gradients for dy: with xhat = (x - mean) rstd and g = dy weight,
  *     dx = rstd (g - sum(g)/width - xhat sum(g xhat)/width),  dweight = sum over the rows of dy xhat,  dbias = sum over the rows of dy
  * (the column sums are what reduce_batch computes for one operand; here they leave with the same walk over the rows).  dweight
- * and dbias are of the type of sums, may be NULL; without both, scratch may be NULL.  dx may be dy or x up to a width of 16384.
+ * and dbias are of the type of sums, may be NULL; without both, scratch may be NULL.  dx may be dy or x up to a width of 16384 (fp64: 8192).
  * Fixed summation orders: the same bits on every run on one device. */
 size_t acro_b200_layer_norm_backward_scratch_bytes(int type, int64_t rows, int64_t width);
 int acro_b200_layer_norm_backward(int type, const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, const void *weight, const void *mean,
