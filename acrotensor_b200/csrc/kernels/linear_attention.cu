@@ -11,11 +11,7 @@ namespace
 
 constexpr int kThreads = 256;
 constexpr int kMaxHead = 256;           // columns of a head
-
-// Sizes of the pass for one type of sums: CHUNK tokens at a time, SLICE columns of v (of the state) per CTA.
-template <class A> struct PassTile;
-template <> struct PassTile<float> { static constexpr int kChunk = 64, kSlice = 64; };
-template <> struct PassTile<double> { static constexpr int kChunk = 32, kSlice = 32; };
+constexpr int kJoin = 8;                // segments whose states a thread of the join has in flight
 
 // Rows of shared memory are read in 16-byte packs: an odd number of packs a row keeps 8 consecutive rows in different banks.
 template <class A>
@@ -26,12 +22,13 @@ __host__ __device__ constexpr int padded(int columns)
     return (packs | 1) * n;
 }
 
-template <class A>
+// The pass works on CHUNK tokens at a time and SLICE columns of v (of the state) per CTA.
+template <class A, int CHUNK, int SLICE>
 size_t pass_smem_bytes(int dq)
 {
-    constexpr int C = PassTile<A>::kChunk, SV = PassTile<A>::kSlice;
     const int rows = (dq + 16 / sizeof(A) * 16 - 1) / (16 / sizeof(A) * 16) * (16 / sizeof(A) * 16);
-    return sizeof(A) * (C * static_cast<size_t>(padded<A>(dq) + std::max(padded<A>(dq), padded<A>(C))) + C * SV + static_cast<size_t>(rows) * SV + C + 1);
+    return sizeof(A) * (CHUNK * static_cast<size_t>(padded<A>(dq) + std::max(padded<A>(dq), padded<A>(CHUNK))) + CHUNK * SLICE +
+                        static_cast<size_t>(rows) * SLICE + CHUNK + 1);
 }
 
 template <class A> struct alignas(16) Vec { A x[16 / sizeof(A)]; };
@@ -39,45 +36,82 @@ template <class A> struct alignas(16) Vec { A x[16 / sizeof(A)]; };
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 __device__ __forceinline__ bool not_finite(double x) { return (__double2hiint(x) & 0x7ff00000) == 0x7ff00000; }
 
-// acc[i][j] += sum_(s < n) P[ty + 16 i][s] V[s][tx TN + j]; with GUARD only over the s that row ty + 16 i sees, because a product
+// Rows 0 .. rows-1 of `to` (columns 0 .. width-1, a multiple of a pack of sums) from m rows of `from` with `columns` columns; zeros where
+// there is nothing.  `packs`: rows start on 16-byte boundaries and columns are a multiple of a pack of elements.  Returns whether
+// this thread met an infinity or NaN.
+template <class T>
+__device__ __forceinline__ bool stage_rows(typename Element<T>::Acc *to, int ld, int width, const T *from, int64_t stride, int rows, int m, int columns,
+                                           bool packs)
+{
+    using A = typename Element<T>::Acc;
+    constexpr int N = 16 / sizeof(A);
+    const int each = width / N;
+    bool odd = false;
+    for (int i = threadIdx.x; i < rows * each; i += kThreads)
+    {
+        const int r = i / each, c = (i - r * each) * N;
+        const T *at = from + r * stride + c;
+        Vec<A> x;
+        if (r < m && packs && c < columns)
+        {
+            const Pack<T, N> p = load_pack<T, N>(at);
+#pragma unroll
+            for (int k = 0; k < N; ++k) x.x[k] = widen(p.x[k]);
+        }
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < N; ++k) x.x[k] = r < m && c + k < columns ? static_cast<A>(widen(at[k])) : A(0);
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) odd |= not_finite(x.x[k]);
+        *reinterpret_cast<Vec<A> *>(to + r * ld + c) = x;
+    }
+    return odd;
+}
+
+// acc[i][j] += sum_(s < n) P[ty + 16 i][s] V[s][column j of tx]; with GUARD only over the s that row ty + 16 i sees, because a product
 // of a masked zero with an infinity or NaN of another token would be NaN.
-template <class A, int TM, int TN, int SV, bool GUARD>
-__device__ __forceinline__ void product(A (&acc)[TM][TN], const A *p, int ldp, const A *v, int n, int ty, int tx, bool reverse)
+template <class A, int TM, int NP, int SV, bool GUARD>
+__device__ __forceinline__ void product(A (&acc)[TM][NP][16 / sizeof(A)], const A *p, int ldp, const A *v, int n, int ty, int tx, bool reverse)
 {
     constexpr int VN = 16 / sizeof(A);
+#pragma unroll 1
     for (int s = 0; s < n; s += VN)
     {
-        Vec<A> row[TM], col[VN];
+        Vec<A> row[TM];
 #pragma unroll
         for (int i = 0; i < TM; ++i) row[i] = *reinterpret_cast<const Vec<A> *>(p + (ty + 16 * i) * ldp + s);
 #pragma unroll
-        for (int k = 0; k < VN; ++k) col[k] = *reinterpret_cast<const Vec<A> *>(v + (s + k) * SV + tx * TN);
-#pragma unroll
         for (int k = 0; k < VN; ++k)
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+            for (int q = 0; q < NP; ++q)
             {
-                if (GUARD && (reverse ? s + k < ty + 16 * i : s + k > ty + 16 * i)) continue;
+                const Vec<A> col = *reinterpret_cast<const Vec<A> *>(v + (s + k) * SV + (q * 16 + tx) * VN);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] += row[i].x[k] * col[k].x[j];
+                for (int i = 0; i < TM; ++i)
+                {
+                    if (GUARD && (reverse ? s + k < ty + 16 * i : s + k > ty + 16 * i)) continue;
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) acc[i][q][j] += row[i].x[k] * col.x[j];
+                }
             }
     }
 }
 
-// The pass for every type and head size: sums of products in the type of sums on the ordinary cores, a chunk of Q, K and V, the
-// scores and the state in shared memory, register tiles of 4 x 4 (2 x 2 in 64 bits) per thread.  Bound by those cores (0.75 of
-// its operations are multiply-adds), not by HBM.
-template <class T>
-__global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs a, int slices, bool states_only)
+// The pass for every type and head size: sums of products in the type of sums on the ordinary cores, a chunk of Q, K and V, the scores
+// and the state in shared memory, register tiles per thread (4 x 4 of a chunk of 64 tokens and 64 columns; 2 x 8 of 32 tokens and 128
+// columns; in 64 bits 2 x 2).  Bound by those cores and by their reads of shared memory, not by HBM.
+template <class T, int C, int SV>
+__global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_constant__ AttentionArgs a, int slices, bool states_only)
 {
     using A = typename Element<T>::Acc;
-    constexpr int C = PassTile<A>::kChunk, SV = PassTile<A>::kSlice, VN = 16 / sizeof(A), TM = C / 16, TN = SV / 16;
-    static_assert(TN == VN, "a thread's columns are one pack");
+    constexpr int VN = 16 / sizeof(A), TM = C / 16, NP = SV / 16 / VN;
     const AttentionPass &p = a.pass[blockIdx.y];
     const int head = blockIdx.x % a.heads, slice = blockIdx.x / a.heads % slices;
     const int c0 = slice * SV;
     if (c0 >= p.dv) return;
-    const int64_t item_index = blockIdx.x / (static_cast<int64_t>(a.heads) * slices);
+    const int64_t item_index = blockIdx.x / (a.heads * slices);
     const bool reverse = p.reverse != 0;
     const SegmentItem item = find_item(a, item_index, reverse);
     if (item.sequence < 0) return;
@@ -85,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs 
     if (states_only && (!cut || item.last)) return;
 
     extern __shared__ __align__(16) unsigned char smem_bytes[];
-    const int ld = padded<A>(p.dq), ldp = padded<A>(C), cols = min(SV, p.dv - c0);
+    const int ld = padded<A>(p.dq), ldp = padded<A>(C), cols = min(SV, p.dv - c0), width = (p.dq + VN - 1) / VN * VN;
     const int state_rows = (p.dq + VN * 16 - 1) / (VN * 16) * (VN * 16);
     A *sq = reinterpret_cast<A *>(smem_bytes), *sp = sq, *sk = sq + C * max(ld, ldp), *sv = sk + C * ld, *st = sv + C * SV, *power = st + state_rows * SV;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
@@ -110,35 +144,24 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs 
     {
         const int d = i / SV, c = i % SV;
         A x = 0;
-        if (from != nullptr && d < p.dq && c < cols) x = turned ? from[static_cast<int64_t>(c0 + c) * p.dq + d] : from[static_cast<int64_t>(d) * p.dv + c0 + c];
+        if (from != nullptr && d < p.dq && c < cols) x = turned ? from[(c0 + c) * p.dq + d] : from[d * p.dv + c0 + c];
         st[i] = x;
     }
     const T *q = rows_of<const T>(p.q, a, item.sequence, head), *k = rows_of<const T>(p.k, a, item.sequence, head),
-            *v = rows_of<const T>(p.v, a, item.sequence, head);
+            *v = rows_of<const T>(p.v, a, item.sequence, head) + c0;
+    const bool packs = p.packs != 0;
+    const A scale = static_cast<A>(p.state_scale), out_scale = static_cast<A>(p.out_scale);
 
-    const int64_t chunks = (item.end - item.begin + C - 1) / C;
-    for (int64_t index = 0; index < chunks; ++index)
+    const int chunks = static_cast<int>((item.end - item.begin + C - 1) / C);
+    for (int index = 0; index < chunks; ++index)
     {
-        const int64_t t0 = item.begin + (reverse ? chunks - 1 - index : index) * C;
+        const int64_t t0 = item.begin + static_cast<int64_t>(reverse ? chunks - 1 - index : index) * C;
         const int m = static_cast<int>(min(static_cast<int64_t>(C), item.end - t0));
         __syncthreads();
         // rows behind the chunk's last token and columns behind the head's last one are zeros
-        bool odd = false;
-        for (int i = threadIdx.x; i < C * ld; i += kThreads)
-        {
-            const int r = i / ld, d = i % ld;
-            const bool there = r < m && d < p.dq;
-            if (!states_only) sq[i] = there ? widen(q[(t0 + r) * p.q.token + d]) : A(0);
-            sk[i] = there ? widen(k[(t0 + r) * p.k.token + d]) : A(0);
-        }
-        for (int i = threadIdx.x; i < C * SV; i += kThreads)
-        {
-            const int r = i / SV, c = i % SV;
-            const A x = r < m && c < cols ? static_cast<A>(widen(v[(t0 + r) * p.v.token + c0 + c])) : A(0);
-            sv[i] = x;
-            odd |= not_finite(x);
-        }
-        odd = __syncthreads_or(odd) != 0;
+        if (!states_only) stage_rows<T>(sq, ld, width, q + t0 * p.q.token, p.q.token, C, m, p.dq, packs);
+        stage_rows<T>(sk, ld, width, k + t0 * p.k.token, p.k.token, C, m, p.dq, packs);
+        const bool odd = __syncthreads_or(stage_rows<T>(sv, SV, SV, v + t0 * p.v.token, p.v.token, C, m, cols, packs)) != 0;
         if (!states_only)
         {
             A acc[TM][TM];
@@ -146,6 +169,7 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs 
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < TM; ++j) acc[i][j] = 0;
+#pragma unroll 2
             for (int d = 0; d < p.dq; d += VN)
             {
                 Vec<A> x[TM], y[TM];
@@ -162,12 +186,14 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs 
 #pragma unroll
                         for (int j = 0; j < TM; ++j) acc[i][j] += x[i].x[n] * y[j].x[n];
             }
-            A near[TM][TN], far[TM][TN];
+            A near[TM][NP][VN], far[TM][NP][VN];
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) near[i][j] = far[i][j] = 0;
-            product<A, TM, TN, SV, false>(far, sq, ld, st, p.dq, ty, tx, reverse);
+                for (int n = 0; n < NP; ++n)
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) near[i][n][j] = far[i][n][j] = 0;
+            product<A, TM, NP, SV, false>(far, sq, ld, st, p.dq, ty, tx, reverse);
             __syncthreads();            // the scores take Q's place
 #pragma unroll
             for (int i = 0; i < TM; ++i)
@@ -175,62 +201,76 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs 
                 for (int j = 0; j < TM; ++j)
                 {
                     const int r = ty + 16 * i, s = tx + 16 * j, n = reverse ? s - r : r - s;
-                    sp[r * ldp + s] = n < 0 ? A(0) : acc[i][j] * power[n] * static_cast<A>(p.state_scale);
+                    sp[r * ldp + s] = n < 0 ? A(0) : acc[i][j] * power[n] * scale;
                 }
             __syncthreads();
-            if (odd) product<A, TM, TN, SV, true>(near, sp, ldp, sv, C, ty, tx, reverse);
-            else product<A, TM, TN, SV, false>(near, sp, ldp, sv, C, ty, tx, reverse);
+            if (odd) product<A, TM, NP, SV, true>(near, sp, ldp, sv, C, ty, tx, reverse);
+            else product<A, TM, NP, SV, false>(near, sp, ldp, sv, C, ty, tx, reverse);
 #pragma unroll
             for (int i = 0; i < TM; ++i)
             {
                 const int r = ty + 16 * i;
                 if (r >= m) continue;
                 const A come = power[reverse ? m - 1 - r : r + 1];
+                const int64_t at = (t0 + r) * p.out.token + c0;
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
-                {
-                    const int c = tx * TN + j;
-                    if (c >= cols) continue;
-                    const A o = static_cast<A>(p.out_scale) * (near[i][j] + come * far[i][j]);
-                    const int64_t at = (t0 + r) * p.out.token + c0 + c;
-                    if (p.sums) rows_of<A>(p.out, a, item.sequence, head)[at] = o;
-                    else rows_of<T>(p.out, a, item.sequence, head)[at] = narrow<T>(o);
-                }
+                for (int n = 0; n < NP; ++n)
+#pragma unroll
+                    for (int j = 0; j < VN; ++j)
+                    {
+                        const int c = (n * 16 + tx) * VN + j;
+                        if (c >= cols) continue;
+                        const A o = out_scale * (near[i][n][j] + come * far[i][n][j]);
+                        if (p.sums) rows_of<A>(p.out, a, item.sequence, head)[at + c] = o;
+                        else rows_of<T>(p.out, a, item.sequence, head)[at + c] = narrow<T>(o);
+                    }
             }
             __syncthreads();
         }
-        for (int i = threadIdx.x; i < C * SV; i += kThreads)
+        for (int i = threadIdx.x; i < C * SV / VN; i += kThreads)
         {
-            const int r = i / SV;
-            if (r < m) sv[i] *= power[reverse ? r + 1 : m - 1 - r] * static_cast<A>(p.state_scale);
+            const int r = i / (SV / VN);
+            if (r >= m) continue;
+            const A w = power[reverse ? r + 1 : m - 1 - r] * scale;
+            Vec<A> &x = reinterpret_cast<Vec<A> *>(sv)[i];
+#pragma unroll
+            for (int j = 0; j < VN; ++j) x.x[j] *= w;
         }
         __syncthreads();
         // what is left of the state after m tokens, to twice the digits: the rounding of one factor would come back in every chunk
         const double exact = exp(g * m);
         const A keep = static_cast<A>(exact), rest = static_cast<A>(exact - static_cast<double>(keep));
-        for (int d = ty * VN; d < state_rows; d += 16 * VN)
+        for (int d = ty * VN; d < p.dq; d += 16 * VN)
         {
-            A acc[VN][TN];
+            A acc[VN][NP][VN];
 #pragma unroll
             for (int i = 0; i < VN; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = 0;
-            if (d < p.dq)
-                for (int s = 0; s < m; ++s)
+                for (int n = 0; n < NP; ++n)
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) acc[i][n][j] = 0;
+#pragma unroll 2
+            for (int s = 0; s < m; ++s)
+            {
+                const Vec<A> x = *reinterpret_cast<const Vec<A> *>(sk + s * ld + d);
+#pragma unroll
+                for (int n = 0; n < NP; ++n)
                 {
-                    const Vec<A> x = *reinterpret_cast<const Vec<A> *>(sk + s * ld + d), y = *reinterpret_cast<const Vec<A> *>(sv + s * SV + tx * TN);
+                    const Vec<A> y = *reinterpret_cast<const Vec<A> *>(sv + s * SV + (n * 16 + tx) * VN);
 #pragma unroll
                     for (int i = 0; i < VN; ++i)
 #pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] += x.x[i] * y.x[j];
+                        for (int j = 0; j < VN; ++j) acc[i][n][j] += x.x[i] * y.x[j];
                 }
+            }
 #pragma unroll
             for (int i = 0; i < VN; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
+                for (int n = 0; n < NP; ++n)
                 {
-                    A &s = st[(d + i) * SV + tx * TN + j];
-                    s = keep * s + (rest * s + acc[i][j]);
+                    Vec<A> &s = *reinterpret_cast<Vec<A> *>(st + (d + i) * SV + (n * 16 + tx) * VN);
+#pragma unroll
+                    for (int j = 0; j < VN; ++j) s.x[j] = keep * s.x[j] + (rest * s.x[j] + acc[i][n][j]);
                 }
         }
     }
@@ -247,44 +287,51 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(AttentionArgs 
     for (int i = threadIdx.x; i < p.dq * SV; i += kThreads)
     {
         const int d = i / SV, c = i % SV;
-        if (c < cols) to[turned ? static_cast<int64_t>(c0 + c) * p.dq + d : static_cast<int64_t>(d) * p.dv + c0 + c] = st[i];
+        if (c < cols) to[turned ? (c0 + c) * p.dq + d : d * p.dv + c0 + c] = st[i];
     }
 }
 
 // Turns the segments' own states into the states that they start from: one thread per entry of a state, walking a sequence's
-// segments in the order of time.
+// segments in the order of time, a few loads ahead (144 segments of 128 x 128: 5 us; with the decay's power taken in every step and one
+// load at a time it was 89).
 template <class A>
-__global__ void __launch_bounds__(kThreads) attention_join_kernel(AttentionArgs a)
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionArgs a)
 {
-    __shared__ int64_t total;
+    __shared__ unsigned long long total;
+    __shared__ double left[2];
     const AttentionPass &p = a.pass[blockIdx.z];
     const int head = blockIdx.x % a.heads;
     const int64_t n = blockIdx.x / a.heads;
     const bool reverse = p.reverse != 0;
-    int64_t begin = 0, end = a.tokens, first = n * segments_of(a.tokens, a.segment);
+    int64_t begin = 0, end = a.tokens;
+    if (a.offsets != nullptr) packed_range(a, n, &begin, &end);
+    const int64_t count = segments_of(end - begin, a.segment);
+    if (count <= 1) return;
+    // only the sequence's last segment is shorter; what it leaves matters backward in time alone
+    if (threadIdx.x < 2) left[threadIdx.x] = exp(decay_log<A>(a.log_decay, head) * static_cast<double>(threadIdx.x == 0 ? a.segment : end - begin - (count - 1) * a.segment));
+    if (threadIdx.x == 2) total = 0;
+    __syncthreads();
+    int64_t first = n * count;
     if (a.offsets != nullptr)
     {
-        packed_range(a, n, &begin, &end);
-        if (threadIdx.x == 0) total = 0;
-        __syncthreads();
-        int64_t before = 0;
+        unsigned long long before = 0;
         for (int64_t i = threadIdx.x; i < n; i += kThreads)
         {
             int64_t b, e;
             packed_range(a, i, &b, &e);
             before += segments_of(e - b, a.segment);
         }
-        if (before > 0) atomicAdd(reinterpret_cast<unsigned long long *>(&total), static_cast<unsigned long long>(before));
+        if (before > 0) atomicAdd(&total, before);
         __syncthreads();
-        first = total;
+        first = static_cast<int64_t>(total);
     }
-    const int64_t count = segments_of(end - begin, a.segment);
-    if (count <= 1 || first + count > a.items) return;     // more segments than rows allow: only with offsets that decrease
+    if (first + count > a.items) return;        // more segments than rows allow: only with offsets that decrease
     const int64_t state = state_of(a.slots, n, a.state_count, a.bad_index);
     if (state < 0) return;
-    const double g = decay_log<A>(a.log_decay, head);
-    const int64_t size = static_cast<int64_t>(p.dq) * p.dv;
-    for (int64_t i = static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x; i < size; i += static_cast<int64_t>(gridDim.y) * kThreads)
+    const double whole = left[0], tail = left[1];
+    const int size = p.dq * p.dv;
+    const int64_t step = static_cast<int64_t>(a.heads) * size;
+    for (int i = blockIdx.y * kThreads + threadIdx.x; i < size; i += gridDim.y * kThreads)
     {
         double run = 0;
         if (p.initial != nullptr)
@@ -292,41 +339,59 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(AttentionArgs 
             const A *from = static_cast<const A *>(p.initial) + (state * a.heads + head) * size;
             run = p.turned ? from[i % p.dv * p.dq + i / p.dv] : from[i];
         }
-#pragma unroll 4
-        for (int64_t k = 0; k < count; ++k)
+        A *states = static_cast<A *>(p.segment_states) + (first * a.heads + head) * size + i;
+        for (int64_t k0 = 0; k0 < count; k0 += kJoin)
         {
-            const int64_t at = reverse ? count - 1 - k : k;
-            A *s = static_cast<A *>(p.segment_states) + ((first + at) * a.heads + head) * size + i;
-            const int64_t length = min(a.segment, end - begin - at * a.segment);
-            const A own = k + 1 < count ? *s : A(0);
-            *s = static_cast<A>(run);
-            run = exp(g * static_cast<double>(length)) * run + own;
+            A own[kJoin];
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k)
+                if (k0 + k + 1 < count) own[k] = states[(reverse ? count - 1 - k0 - k : k0 + k) * step];
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k)
+            {
+                if (k0 + k >= count) break;
+                const int64_t at = reverse ? count - 1 - k0 - k : k0 + k;
+                states[at * step] = static_cast<A>(run);
+                if (k0 + k + 1 < count) run = (at == count - 1 ? tail : whole) * run + own[k];
+            }
         }
     }
 }
 
+struct ShareArgs
+{
+    const void *sums[2];
+    TokenRows out[2];
+    int32_t columns[2];
+};
+
 // out[row, h, c] = sum over the query heads of head h, in ascending order: the gradients of shared keys and values.
 template <class T>
-__global__ void __launch_bounds__(kThreads) attention_share_kernel(AttentionArgs a, const typename Element<T>::Acc *sums, TokenRows out, int heads, int group,
-                                                                   int columns)
+__global__ void __launch_bounds__(kThreads) attention_share_kernel(const __grid_constant__ AttentionArgs a, ShareArgs both, int heads, int group)
 {
     using A = typename Element<T>::Acc;
+    const A *sums = static_cast<const A *>(both.sums[blockIdx.y]);
+    const TokenRows out = both.out[blockIdx.y];
+    const int columns = both.columns[blockIdx.y];
     int64_t begin = 0, end = a.sequences * a.tokens;
     if (a.offsets != nullptr)
     {
         begin = min(max(a.offsets[0], int64_t(0)), a.tokens);
         end = min(max(a.offsets[a.sequences], int64_t(0)), a.tokens);
     }
-    const int64_t each = static_cast<int64_t>(heads) * columns, total = (end - begin) * each;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads)
+    for (int64_t row = begin + blockIdx.x; row < end; row += gridDim.x)
     {
-        const int64_t row = begin + i / each;
-        const int h = static_cast<int>(i % each / columns), c = static_cast<int>(i % columns);
-        const A *from = sums + (row * heads * group + static_cast<int64_t>(h) * group) * columns + c;
-        A s = from[0];
-        for (int k = 1; k < group; ++k) s += from[static_cast<int64_t>(k) * columns];
         const int64_t n = a.offsets == nullptr ? row / a.tokens : 0, t = a.offsets == nullptr ? row % a.tokens : row;
-        static_cast<T *>(out.data)[n * out.sequence + t * out.token + h * out.head + c] = narrow<T>(s);
+        const A *from = sums + row * heads * group * columns;
+        T *to = static_cast<T *>(out.data) + n * out.sequence + t * out.token;
+        for (int i = threadIdx.x; i < heads * columns; i += kThreads)
+        {
+            const int h = i / columns, c = i % columns;
+            const A *x = from + h * group * columns + c;
+            A s = x[0];
+            for (int k = 1; k < group; ++k) s += x[k * columns];
+            to[h * out.head + c] = narrow<T>(s);
+        }
     }
 }
 
@@ -451,19 +516,30 @@ std::string head_fault(const acro_b200_linear_attention_desc *d)
     return "";
 }
 
-// Tokens of a segment.  With at least half as many (sequence, head) pairs as SMs the pairs alone fill the GPU (a cut reads k
-// and v twice); fewer are cut so that segments x heads come to about one per SM.  Packed sequences are treated as one axis of
-// all their rows, since their lengths are not known here.
-int64_t segment_tokens(const acro_b200_linear_attention_desc &d, bool packed)
+// Tokens of a segment.  A cut of the sequences into `wanted` segments each makes the GPU's waves of CTAs shorter, and costs a second
+// walk over k and v (about 0.6 of the main pass on either path) and the join (as long as 6 chunks of 64 tokens): the cheapest number
+// is taken.  `resident`: CTAs an SM holds (tensor-core pass: 1; the other: 2 at least).  Packed sequences are treated as one axis of all
+// their rows, since their lengths are not known here.
+int64_t segment_tokens(const acro_b200_linear_attention_desc &d, bool packed, bool tensor_cores, int passes)
 {
-    const int64_t sms = sm_count() > 0 ? sm_count() : 148;
-    const int64_t whole = (d.tokens + kSegmentQuantum - 1) / kSegmentQuantum * kSegmentQuantum;
-    const int64_t pairs = (packed ? 1 : std::max<int64_t>(1, d.sequences)) * d.q_heads;
-    const int64_t wanted = std::max<int64_t>(1, sms / pairs);
-    int64_t segment = (d.tokens + wanted - 1) / wanted;
-    segment = (segment + kSegmentQuantum - 1) / kSegmentQuantum * kSegmentQuantum;
-    segment = std::max<int64_t>(segment, 4 * kSegmentQuantum);
-    return std::max<int64_t>(kSegmentQuantum, std::min(segment, whole));
+    const int64_t slots = (sm_count() > 0 ? sm_count() : 148) * (tensor_cores ? 1 : 2);
+    const int64_t whole = std::max<int64_t>(1, (d.tokens + kSegmentQuantum - 1) / kSegmentQuantum) * kSegmentQuantum;
+    const int64_t pairs = (packed ? 1 : std::max<int64_t>(1, d.sequences)) * d.q_heads * passes;
+    const int64_t shortest = kSegmentQuantum * (tensor_cores ? 4 : 1);
+    int64_t best = whole;
+    double cost = static_cast<double>((pairs + slots - 1) / slots) * whole;
+    for (int64_t wanted = 2; wanted <= slots / pairs + 1 && whole / wanted >= shortest; ++wanted)
+    {
+        const int64_t segment = ((d.tokens + wanted - 1) / wanted + kSegmentQuantum - 1) / kSegmentQuantum * kSegmentQuantum;
+        const int64_t each = (d.tokens + segment - 1) / segment;
+        const double c = 1.6 * static_cast<double>((pairs * each + slots - 1) / slots) * segment + 6 * 64;
+        if (c < cost)
+        {
+            cost = c;
+            best = segment;
+        }
+    }
+    return best;
 }
 
 int64_t item_bound(const acro_b200_linear_attention_desc &d, bool packed, int64_t segment)
@@ -477,11 +553,17 @@ bool may_cut(const acro_b200_linear_attention_desc &d, int64_t segment) { return
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t states_bytes(const acro_b200_linear_attention_desc &d, bool packed)
+// For whichever path the arrays will turn out to allow.
+size_t states_bytes(const acro_b200_linear_attention_desc &d, bool packed, int passes)
 {
-    const int64_t segment = segment_tokens(d, packed);
-    if (!may_cut(d, segment)) return 0;
-    return round256(static_cast<size_t>(item_bound(d, packed, segment)) * d.q_heads * d.dk * d.dv * statistic_bytes(d.type));
+    size_t most = 0;
+    for (int tensor_cores = 0; tensor_cores < 2; ++tensor_cores)
+    {
+        const int64_t segment = segment_tokens(d, packed, tensor_cores != 0, passes);
+        if (may_cut(d, segment) && (tensor_cores == 0 || d.type == ACRO_B200_BF16))
+            most = std::max(most, round256(static_cast<size_t>(item_bound(d, packed, segment)) * d.q_heads * d.dk * d.dv * statistic_bytes(d.type)));
+    }
+    return most;
 }
 
 size_t shared_bytes(const acro_b200_linear_attention_desc &d, bool packed, int columns)
@@ -503,51 +585,81 @@ std::string array_fault(const acro_b200_token_array *x, int64_t columns, int hea
     return "";
 }
 
+// Do the pass's operands come in packs of 16 bytes of sums?
 template <class T>
-int run_pass(const AttentionArgs &a, bool states_only, cudaStream_t stream)
+bool rows_in_packs(const AttentionPass &p)
 {
-    using A = typename Element<T>::Acc;
+    constexpr int n = 16 / sizeof(typename Element<T>::Acc);
+    const auto fits = [](const TokenRows &r, int columns) {
+        return reinterpret_cast<uintptr_t>(r.data) % (n * sizeof(T)) == 0 && r.sequence % n == 0 && r.token % n == 0 && r.head % n == 0 && columns % n == 0;
+    };
+    return fits(p.q, p.dq) && fits(p.k, p.dq) && fits(p.v, p.dv);
+}
+
+template <class T, int C, int SV>
+int run_pass_tiled(const AttentionArgs &all, bool states_only, cudaStream_t stream)
+{
+    AttentionArgs a = all;
     int slices = 1;
     size_t smem = 0;
     for (int i = 0; i < a.passes; ++i)
     {
-        slices = std::max(slices, (a.pass[i].dv + PassTile<A>::kSlice - 1) / PassTile<A>::kSlice);
-        smem = std::max(smem, pass_smem_bytes<A>(a.pass[i].dq));
+        a.pass[i].packs = rows_in_packs<T>(a.pass[i]);
+        slices = std::max(slices, (a.pass[i].dv + SV - 1) / SV);
+        smem = std::max(smem, pass_smem_bytes<typename Element<T>::Acc, C, SV>(a.pass[i].dq));
     }
-    cudaError_t status = cudaFuncSetAttribute(attention_pass_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = cudaFuncSetAttribute(attention_pass_kernel<T, C, SV>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_linear_attention");
     const int64_t grid = a.items * a.heads * slices;
     if (grid > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 segments x heads");
-    attention_pass_kernel<T><<<dim3(static_cast<unsigned>(grid), a.passes), kThreads, smem, stream>>>(a, slices, states_only);
+    attention_pass_kernel<T, C, SV><<<dim3(static_cast<unsigned>(grid), a.passes), kThreads, smem, stream>>>(a, slices, states_only);
     return launch_status("acro_b200_linear_attention");
 }
 
-int run_pass_of(int type, const AttentionArgs &a, bool states_only, cudaStream_t stream)
+// The scores are made anew for every slice of v's columns, so heads of more than 64 columns take slices of 128, with half the tokens a
+// chunk to make room.
+template <class T>
+int run_pass(const AttentionArgs &a, bool states_only, cudaStream_t stream)
 {
+    if constexpr (sizeof(T) == 8) return run_pass_tiled<T, 32, 32>(a, states_only, stream);
+    else
+    {
+        int widest = 0;
+        for (int i = 0; i < a.passes; ++i) widest = std::max(widest, a.pass[i].dv);
+        return widest <= 64 ? run_pass_tiled<T, 64, 64>(a, states_only, stream) : run_pass_tiled<T, 32, 128>(a, states_only, stream);
+    }
+}
+
+int run_pass_of(int type, const AttentionArgs &a, bool tensor_cores, bool states_only, cudaStream_t stream)
+{
+    if (tensor_cores) return attention_mma_launch(a, states_only, stream);
     switch (type)
     {
     case ACRO_B200_F64: return run_pass<double>(a, states_only, stream);
     case ACRO_B200_F32: return run_pass<float>(a, states_only, stream);
-    case ACRO_B200_BF16:
-        if (attention_mma_supported(a)) return attention_mma_launch(a, states_only, stream);
-        return run_pass<__nv_bfloat16>(a, states_only, stream);
+    case ACRO_B200_BF16: return run_pass<__nv_bfloat16>(a, states_only, stream);
     default: return run_pass<__half>(a, states_only, stream);
     }
 }
 
-int run_all(int type, const AttentionArgs &a, bool cut, cudaStream_t stream)
+int run_all(const acro_b200_linear_attention_desc &d, AttentionArgs &a, cudaStream_t stream)
 {
-    if (cut)
+    const bool packed = a.offsets != nullptr, tensor_cores = d.type == ACRO_B200_BF16 && attention_mma_supported(a);
+    a.segment = segment_tokens(d, packed, tensor_cores, a.passes);
+    a.items = item_bound(d, packed, a.segment);
+    if (may_cut(d, a.segment))
     {
-        int status = run_pass_of(type, a, true, stream);
+        int status = run_pass_of(d.type, a, tensor_cores, true, stream);
         if (status != ACRO_B200_OK) return status;
-        const dim3 grid(static_cast<unsigned>(a.sequences * a.heads), 16, a.passes);
-        if (type == ACRO_B200_F64) attention_join_kernel<double><<<grid, kThreads, 0, stream>>>(a);
+        int64_t entries = 0;
+        for (int i = 0; i < a.passes; ++i) entries = std::max<int64_t>(entries, static_cast<int64_t>(a.pass[i].dq) * a.pass[i].dv);
+        const dim3 grid(static_cast<unsigned>(a.sequences * a.heads), static_cast<unsigned>(std::min<int64_t>(16, (entries + kThreads - 1) / kThreads)), a.passes);
+        if (d.type == ACRO_B200_F64) attention_join_kernel<double><<<grid, kThreads, 0, stream>>>(a);
         else attention_join_kernel<float><<<grid, kThreads, 0, stream>>>(a);
         status = launch_status("acro_b200_linear_attention");
         if (status != ACRO_B200_OK) return status;
     }
-    return run_pass_of(type, a, false, stream);
+    return run_pass_of(d.type, a, tensor_cores, false, stream);
 }
 
 int common_args(const acro_b200_linear_attention_desc &d, const void *log_decay, const int64_t *offsets, AttentionArgs *a)
@@ -559,8 +671,6 @@ int common_args(const acro_b200_linear_attention_desc &d, const void *log_decay,
     a->state_count = d.sequences;
     a->sequences = d.sequences;
     a->tokens = d.tokens;
-    a->segment = segment_tokens(d, offsets != nullptr);
-    a->items = item_bound(d, offsets != nullptr, a->segment);
     a->bad_index = bad_index_flag_device_ptr();
     a->wait_flag = wait_flag_device_ptr();
     if (a->bad_index == nullptr || a->wait_flag == nullptr) return fail_cuda(cudaErrorUnknown, "acro_b200_linear_attention (device flag)");
@@ -575,7 +685,7 @@ extern "C" {
 size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
 {
     if (!head_fault(desc).empty()) return 0;
-    return states_bytes(*desc, packed != 0);
+    return states_bytes(*desc, packed != 0, 1);
 }
 
 int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -600,7 +710,7 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
     if (fault.empty() && slots != nullptr && state_count < 0) fault = "negative state_count";
     if (fault.empty() && slots == nullptr && state_count != d.sequences && (initial_state != nullptr || final_state != nullptr))
         fault = "without slots there is one state per sequence";
-    const size_t need = states_bytes(d, packed);
+    const size_t need = states_bytes(d, packed, 1);
     if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
         fault = "scratch is smaller than acro_b200_linear_attention_scratch_bytes or not 16-byte aligned";
     if (fault.empty() && need > 0 && !on_current_device(scratch)) fault = "scratch is not memory of the current device";
@@ -632,7 +742,7 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
     p.initial = initial_state;
     p.final = final_state;
     p.segment_states = scratch;
-    return run_all(d.type, a, need > 0, as_stream(stream));
+    return run_all(d, a, as_stream(stream));
 }
 
 int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -711,7 +821,7 @@ int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc,
 size_t acro_b200_linear_attention_backward_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
 {
     if (!head_fault(desc).empty()) return 0;
-    return 3 * states_bytes(*desc, packed != 0) + shared_bytes(*desc, packed != 0, desc->dk) + shared_bytes(*desc, packed != 0, desc->dv);
+    return 3 * states_bytes(*desc, packed != 0, 3) + shared_bytes(*desc, packed != 0, desc->dk) + shared_bytes(*desc, packed != 0, desc->dv);
 }
 
 int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -753,7 +863,7 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     const int group = d.q_heads / d.kv_heads;
     const TokenRows rq = rows_from(rows ? *q : none, 1), rk = rows_from(rows ? *k : none, group), rv = rows_from(rows ? *v : none, group),
                     ro = rows_from(rows ? *dout : none, 1);
-    const size_t states = states_bytes(d, packed);
+    const size_t states = states_bytes(d, packed, 3);
     unsigned char *at = static_cast<unsigned char *>(scratch);
     a.passes = 3;
     for (int i = 0; i < 3; ++i)
@@ -784,36 +894,28 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     {
         a.pass[1].out = rows_from(rows ? *dk : none, 1);
         a.pass[2].out = rows_from(rows ? *dv : none, 1);
-        return run_all(d.type, a, states > 0, as_stream(stream));
+        return run_all(d, a, as_stream(stream));
     }
     // a row of sums per query head, added up afterwards
-    void *sums[2];
-    const int columns[2] = {d.dk, d.dv};
+    ShareArgs both = {{nullptr, nullptr}, {rows_from(rows ? *dk : none, 1), rows_from(rows ? *dv : none, 1)}, {d.dk, d.dv}};
     for (int i = 0; i < 2; ++i)
     {
-        sums[i] = at;
-        at += shared_bytes(d, packed, columns[i]);
-        const int64_t row = static_cast<int64_t>(d.q_heads) * columns[i];
-        a.pass[1 + i].out = {sums[i], row * d.tokens, row, columns[i], 1};
+        both.sums[i] = at;
+        const int64_t row = static_cast<int64_t>(d.q_heads) * both.columns[i];
+        a.pass[1 + i].out = {at, row * d.tokens, row, both.columns[i], 1};
         a.pass[1 + i].sums = 1;
+        at += shared_bytes(d, packed, both.columns[i]);
     }
     cudaStream_t st = as_stream(stream);
-    status = run_all(d.type, a, states > 0, st);
+    status = run_all(d, a, st);
     if (status != ACRO_B200_OK || !rows) return status;
-    for (int i = 0; i < 2; ++i)
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((packed ? 1 : d.sequences) * d.tokens, 148 * 16)), 2);
+    switch (d.type)
     {
-        const TokenRows out = rows_from(i == 0 ? *dk : *dv, 1);
-        const int64_t entries = (packed ? 1 : d.sequences) * d.tokens * d.kv_heads * columns[i];
-        const unsigned grid = static_cast<unsigned>(std::min<int64_t>((entries + kThreads - 1) / kThreads, 148 * 16));
-        switch (d.type)
-        {
-        case ACRO_B200_F64: attention_share_kernel<double><<<grid, kThreads, 0, st>>>(a, static_cast<double *>(sums[i]), out, d.kv_heads, group, columns[i]); break;
-        case ACRO_B200_F32: attention_share_kernel<float><<<grid, kThreads, 0, st>>>(a, static_cast<float *>(sums[i]), out, d.kv_heads, group, columns[i]); break;
-        case ACRO_B200_BF16:
-            attention_share_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, static_cast<float *>(sums[i]), out, d.kv_heads, group, columns[i]);
-            break;
-        default: attention_share_kernel<__half><<<grid, kThreads, 0, st>>>(a, static_cast<float *>(sums[i]), out, d.kv_heads, group, columns[i]);
-        }
+    case ACRO_B200_F64: attention_share_kernel<double><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group); break;
+    case ACRO_B200_F32: attention_share_kernel<float><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group); break;
+    case ACRO_B200_BF16: attention_share_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group); break;
+    default: attention_share_kernel<__half><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group);
     }
     return launch_status("acro_b200_linear_attention_backward");
 }

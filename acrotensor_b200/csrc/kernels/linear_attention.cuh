@@ -37,6 +37,7 @@ struct AttentionPass
     int32_t dq, dv;                     // columns of q and k; of v and out
     int32_t reverse;                    // backward in time
     int32_t turned;                     // the user's states are [dv][dq]: read and written transposed
+    int32_t packs;                      // q, k and v can be read in packs of 16 bytes of sums (set by the launch)
     int32_t sums;                       // out is in the type of sums (one row per query head, to be added up), not the element type
     double state_scale, out_scale;      // on k v^T as it enters the state, on q^T S; their product on (q.k) v
     const void *initial;                // state a sequence starts from, or null: zero

@@ -10,6 +10,8 @@ and reported by ``acro_b200_device_status()``.
 
 The formulas stand in include/acro_b200.h; acro::TensorEngine has the same operators for fp64 tensors (``TensorEngine.LinearAttention``).
 """
+import threading
+
 from ._lib import LinearAttentionDesc, TokenArray, check, lib
 
 _TYPES = {"float64": 0, "float32": 1, "bfloat16": 2, "float16": 3}
@@ -77,11 +79,42 @@ def _scratch(scratch, need):
         return None, 0
     if scratch is None:
         raise ValueError("this call needs %d bytes of scratch" % need)
-    _contiguous("scratch", scratch)
     n = scratch.element_size()
+    if len(scratch.shape) != 1 or (scratch.shape[0] > 1 and scratch.stride()[0] != 1):
+        _contiguous("scratch", scratch)
     for d in scratch.shape:
         n *= d
     return scratch.data_ptr(), n
+
+
+class _Plan:
+    """What a call's shapes, strides and types come to, checked: everything but the addresses.  Kept per thread, since a call fills the
+    addresses in."""
+    __slots__ = ("desc", "rows", "count", "need", "extra")
+
+
+_local = threading.local()
+_PLANS = 1024               # kept per thread
+
+
+def _known(key):
+    plans = getattr(_local, "plans", None)
+    if plans is None:
+        plans = _local.plans = {}
+    return plans.get(key)
+
+
+def _keep(key, desc, rows, count=0, need=0, extra=None):
+    plan = _Plan()
+    plan.desc, plan.rows, plan.count, plan.need, plan.extra = desc, rows, count, need, extra
+    if len(_local.plans) >= _PLANS:
+        _local.plans.clear()
+    _local.plans[key] = plan
+    return plan
+
+
+def _form(x):
+    return None if x is None else (x.shape, x.stride(), x.dtype)
 
 
 def _attention_desc(q, k, v, scale, offsets, step=False):
@@ -125,8 +158,12 @@ def _check_states(desc, sums, log_decay, slots, **states):
 
 def linear_attention_scratch_bytes(q, k, v, offsets=None):
     """Bytes of scratch :func:`linear_attention` needs for arrays of these shapes."""
-    desc, _ = _attention_desc(q, k, v, 1.0, offsets)
-    return lib().acro_b200_linear_attention_scratch_bytes(desc, offsets is not None)
+    key = (5, _form(q), _form(k), _form(v), _form(offsets))
+    plan = _known(key)
+    if plan is None:
+        desc, _ = _attention_desc(q, k, v, 1.0, offsets)
+        plan = _keep(key, None, None, need=lib().acro_b200_linear_attention_scratch_bytes(desc, offsets is not None))
+    return plan.need
 
 
 def linear_attention(out, q, k, v, log_decay, scale=1.0, offsets=None, initial_state=None, final_state=None, slots=None, scratch=None, stream=None):
@@ -136,15 +173,20 @@ def linear_attention(out, q, k, v, log_decay, scale=1.0, offsets=None, initial_s
     sequence n in the rows offsets[n] .. offsets[n+1]-1.  k and v may have fewer heads (a divisor of q's).  States are
     [sequences, heads, dk, dv]; with ``slots`` (int32 per sequence, negative: not there) [any number, heads, dk, dv].  ``final_state`` may be
     ``initial_state``.  ``scratch``: any contiguous array of :func:`linear_attention_scratch_bytes` bytes."""
-    desc, lead = _attention_desc(q, k, v, scale, offsets)
-    _same_type(q.dtype, out=out)
-    _shape("out", out, tuple(q.shape[:-1]) + (desc.dv,))
-    count = _check_states(desc, _type(q, "q")[1], log_decay, slots, initial_state=initial_state, final_state=final_state)
-    need = lib().acro_b200_linear_attention_scratch_bytes(desc, offsets is not None)
-    at, have = _scratch(scratch, need)
-    check(lib().acro_b200_linear_attention(desc, _rows("q", q, lead), _rows("k", k, lead), _rows("v", v, lead), _rows("out", out, lead),
-                                           log_decay.data_ptr(), _pointer(offsets), _pointer(initial_state), _pointer(final_state), _pointer(slots),
-                                           count, at, have, _stream(stream)))
+    key = (0, scale, _form(q), _form(k), _form(v), _form(out), _form(log_decay), _form(offsets), _form(initial_state), _form(final_state), _form(slots))
+    plan = _known(key)
+    if plan is None:
+        desc, lead = _attention_desc(q, k, v, scale, offsets)
+        _same_type(q.dtype, out=out)
+        _shape("out", out, tuple(q.shape[:-1]) + (desc.dv,))
+        count = _check_states(desc, _type(q, "q")[1], log_decay, slots, initial_state=initial_state, final_state=final_state)
+        need = lib().acro_b200_linear_attention_scratch_bytes(desc, offsets is not None)
+        plan = _keep(key, desc, tuple(_rows(n, x, lead) for n, x in (("q", q), ("k", k), ("v", v), ("out", out))), count, need)
+    rq, rk, rv, ro = plan.rows
+    rq.data, rk.data, rv.data, ro.data = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    at, have = _scratch(scratch, plan.need)
+    check(lib().acro_b200_linear_attention(plan.desc, rq, rk, rv, ro, log_decay.data_ptr(), _pointer(offsets), _pointer(initial_state),
+                                           _pointer(final_state), _pointer(slots), plan.count, at, have, _stream(stream)))
 
 
 def linear_attention_step(out, state_out, q, k, v, log_decay, state_in, scale=1.0, slots=None, stream=None):
@@ -152,38 +194,57 @@ def linear_attention_step(out, state_out, q, k, v, log_decay, state_in, scale=1.
 
     q, k [requests, heads, dk], v, out [requests, heads, dv]; states [requests, heads, dk, dv], or with ``slots`` (int32 per request,
     negative: not there) [any number, heads, dk, dv].  ``state_out`` may be ``state_in``."""
-    desc, lead = _attention_desc(q, k, v, scale, None, step=True)
-    _same_type(q.dtype, out=out)
-    _shape("out", out, (desc.sequences, desc.q_heads, desc.dv))
-    count = _check_states(desc, _type(q, "q")[1], log_decay, slots, state_in=state_in, state_out=state_out)
-    check(lib().acro_b200_linear_attention_step(desc, _rows("q", q, lead), _rows("k", k, lead), _rows("v", v, lead), _rows("out", out, lead),
-                                                log_decay.data_ptr(), state_in.data_ptr(), state_out.data_ptr(), _pointer(slots), count,
-                                                _stream(stream)))
+    key = (1, scale, _form(q), _form(k), _form(v), _form(out), _form(log_decay), _form(state_in), _form(state_out), _form(slots))
+    plan = _known(key)
+    if plan is None:
+        desc, lead = _attention_desc(q, k, v, scale, None, step=True)
+        _same_type(q.dtype, out=out)
+        _shape("out", out, (desc.sequences, desc.q_heads, desc.dv))
+        if state_in is None or state_out is None:
+            raise ValueError("a step needs states")
+        count = _check_states(desc, _type(q, "q")[1], log_decay, slots, state_in=state_in, state_out=state_out)
+        plan = _keep(key, desc, tuple(_rows(n, x, lead) for n, x in (("q", q), ("k", k), ("v", v), ("out", out))), count)
+    rq, rk, rv, ro = plan.rows
+    rq.data, rk.data, rv.data, ro.data = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    check(lib().acro_b200_linear_attention_step(plan.desc, rq, rk, rv, ro, log_decay.data_ptr(), state_in.data_ptr(), state_out.data_ptr(),
+                                                _pointer(slots), plan.count, _stream(stream)))
 
 
 def linear_attention_backward_scratch_bytes(q, k, v, offsets=None):
     """Bytes of scratch :func:`linear_attention_backward` needs for arrays of these shapes."""
-    desc, _ = _attention_desc(q, k, v, 1.0, offsets)
-    return lib().acro_b200_linear_attention_backward_scratch_bytes(desc, offsets is not None)
+    key = (6, _form(q), _form(k), _form(v), _form(offsets))
+    plan = _known(key)
+    if plan is None:
+        desc, _ = _attention_desc(q, k, v, 1.0, offsets)
+        plan = _keep(key, None, None, need=lib().acro_b200_linear_attention_backward_scratch_bytes(desc, offsets is not None))
+    return plan.need
 
 
 def linear_attention_backward(dq, dk, dv, dout, q, k, v, log_decay, scale=1.0, offsets=None, initial_state=None, d_final_state=None,
                               d_initial_state=None, scratch=None, stream=None):
     """Gradients of :func:`linear_attention` for ``dout`` (and ``d_final_state``) with respect to q, k, v (and the initial state).  The
     decays are constants of the layer and get none.  Shapes as there; states [sequences, heads, dk, dv]."""
-    desc, lead = _attention_desc(q, k, v, scale, offsets)
-    _same_type(q.dtype, dout=dout, dq=dq, dk=dk, dv=dv)
-    _shape("dout", dout, tuple(q.shape[:-1]) + (desc.dv,))
-    for name, x, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        _shape(name, x, tuple(like.shape))
-    _check_states(desc, _type(q, "q")[1], log_decay, None, initial_state=initial_state, d_final_state=d_final_state,
-                  d_initial_state=d_initial_state)
-    need = lib().acro_b200_linear_attention_backward_scratch_bytes(desc, offsets is not None)
-    at, have = _scratch(scratch, need)
+    key = (2, scale, _form(q), _form(k), _form(v), _form(dout), _form(dq), _form(dk), _form(dv), _form(log_decay), _form(offsets), _form(initial_state),
+           _form(d_final_state), _form(d_initial_state))
+    plan = _known(key)
+    if plan is None:
+        desc, lead = _attention_desc(q, k, v, scale, offsets)
+        _same_type(q.dtype, dout=dout, dq=dq, dk=dk, dv=dv)
+        _shape("dout", dout, tuple(q.shape[:-1]) + (desc.dv,))
+        for name, x, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+            _shape(name, x, tuple(like.shape))
+        _check_states(desc, _type(q, "q")[1], log_decay, None, initial_state=initial_state, d_final_state=d_final_state,
+                      d_initial_state=d_initial_state)
+        need = lib().acro_b200_linear_attention_backward_scratch_bytes(desc, offsets is not None)
+        arrays = (("q", q), ("k", k), ("v", v), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv))
+        plan = _keep(key, desc, tuple(_rows(n, x, lead) for n, x in arrays), 0, need)
+    rows = plan.rows
+    for r, x in zip(rows, (q, k, v, dout, dq, dk, dv)):
+        r.data = x.data_ptr()
+    at, have = _scratch(scratch, plan.need)
     check(lib().acro_b200_linear_attention_backward(
-        desc, _rows("q", q, lead), _rows("k", k, lead), _rows("v", v, lead), _rows("dout", dout, lead), log_decay.data_ptr(), _pointer(offsets),
-        _pointer(initial_state), _pointer(d_final_state), _rows("dq", dq, lead), _rows("dk", dk, lead), _rows("dv", dv, lead),
-        _pointer(d_initial_state), at, have, _stream(stream)))
+        plan.desc, rows[0], rows[1], rows[2], rows[3], log_decay.data_ptr(), _pointer(offsets), _pointer(initial_state), _pointer(d_final_state),
+        rows[4], rows[5], rows[6], _pointer(d_initial_state), at, have, _stream(stream)))
 
 
 def _matrix(name, x):
@@ -208,13 +269,18 @@ def _matrix(name, x):
 def layer_norm(out, x, weight=None, bias=None, eps=1e-5, mean=None, rstd=None, stream=None):
     """``out = (x - mean) rstd weight + bias`` over the last dim of x, rstd = 1 / sqrt(variance + eps).  weight and bias (both may be None)
     are of x's type; mean and rstd (if given) receive the row statistics, as the gradient wants them.  ``out`` may be ``x``."""
-    code, sums, _ = _type(x, "x")
-    _same_type(x.dtype, out=out, weight=weight, bias=bias)
-    _shape("out", out, tuple(x.shape))
-    rows, width, x_stride = _matrix("x", x)
-    y_stride = _matrix("out", out)[2]
-    _row_arrays(rows, sums, mean=mean, rstd=rstd)
-    _column_arrays(width, weight=weight, bias=bias)
+    key = (3, _form(x), _form(out), _form(weight), _form(bias), _form(mean), _form(rstd))
+    plan = _known(key)
+    if plan is None:
+        code, sums, _ = _type(x, "x")
+        _same_type(x.dtype, out=out, weight=weight, bias=bias)
+        _shape("out", out, tuple(x.shape))
+        rows, width, x_stride = _matrix("x", x)
+        y_stride = _matrix("out", out)[2]
+        _row_arrays(rows, sums, mean=mean, rstd=rstd)
+        _column_arrays(width, weight=weight, bias=bias)
+        plan = _keep(key, None, None, extra=(code, x_stride, y_stride, rows, width))
+    code, x_stride, y_stride, rows, width = plan.extra
     check(lib().acro_b200_layer_norm(code, x.data_ptr(), x_stride, _pointer(weight), _pointer(bias), out.data_ptr(), y_stride, _pointer(mean),
                                      _pointer(rstd), rows, width, eps, _stream(stream)))
 
@@ -240,23 +306,34 @@ def _column_arrays(width, **arrays):
 
 def layer_norm_backward_scratch_bytes(x):
     """Bytes of scratch :func:`layer_norm_backward` needs for an array of this shape."""
-    rows, width, _ = _matrix("x", x)
-    return lib().acro_b200_layer_norm_backward_scratch_bytes(_type(x, "x")[0], rows, width)
+    key = (7, _form(x))
+    plan = _known(key)
+    if plan is None:
+        rows, width, _ = _matrix("x", x)
+        plan = _keep(key, None, None, need=lib().acro_b200_layer_norm_backward_scratch_bytes(_type(x, "x")[0], rows, width))
+    return plan.need
 
 
 def layer_norm_backward(dx, dweight, dbias, dout, x, mean, rstd, weight=None, scratch=None, stream=None):
     """Gradients of :func:`layer_norm`: dx, and (unless None) dweight and dbias, the sums over all rows, in the type of sums.  mean and
     rstd are the forward pass's.  ``scratch`` is needed for dweight and dbias only.  ``dx`` may be ``dout`` or ``x``."""
-    code, sums, _ = _type(x, "x")
-    _same_type(x.dtype, dx=dx, dout=dout, weight=weight)
-    _shape("dx", dx, tuple(x.shape))
-    _shape("dout", dout, tuple(x.shape))
-    rows, width, x_stride = _matrix("x", x)
-    _row_arrays(rows, sums, mean=mean, rstd=rstd)
-    _of_type(sums, dweight=dweight, dbias=dbias)
-    _column_arrays(width, weight=weight, dweight=dweight, dbias=dbias)
-    need = 0 if dweight is None and dbias is None else lib().acro_b200_layer_norm_backward_scratch_bytes(code, rows, width)
-    at, have = _scratch(scratch, need)
-    check(lib().acro_b200_layer_norm_backward(code, dout.data_ptr(), _matrix("dout", dout)[2], x.data_ptr(), x_stride, _pointer(weight),
-                                              mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _matrix("dx", dx)[2], _pointer(dweight),
-                                              _pointer(dbias), rows, width, at, have, _stream(stream)))
+    key = (4, _form(x), _form(dx), _form(dout), _form(mean), _form(rstd), _form(weight), _form(dweight), _form(dbias))
+    plan = _known(key)
+    if plan is None:
+        code, sums, _ = _type(x, "x")
+        _same_type(x.dtype, dx=dx, dout=dout, weight=weight)
+        _shape("dx", dx, tuple(x.shape))
+        _shape("dout", dout, tuple(x.shape))
+        rows, width, x_stride = _matrix("x", x)
+        if mean is None or rstd is None:
+            raise ValueError("the gradient needs the mean and rstd of the forward pass")
+        _row_arrays(rows, sums, mean=mean, rstd=rstd)
+        _of_type(sums, dweight=dweight, dbias=dbias)
+        _column_arrays(width, weight=weight, dweight=dweight, dbias=dbias)
+        need = 0 if dweight is None and dbias is None else lib().acro_b200_layer_norm_backward_scratch_bytes(code, rows, width)
+        plan = _keep(key, None, None, need=need, extra=(code, x_stride, _matrix("dout", dout)[2], _matrix("dx", dx)[2], rows, width))
+    code, x_stride, dy_stride, dx_stride, rows, width = plan.extra
+    at, have = _scratch(scratch, plan.need)
+    check(lib().acro_b200_layer_norm_backward(code, dout.data_ptr(), dy_stride, x.data_ptr(), x_stride, _pointer(weight), mean.data_ptr(),
+                                              rstd.data_ptr(), dx.data_ptr(), dx_stride, _pointer(dweight), _pointer(dbias), rows, width, at, have,
+                                              _stream(stream)))
