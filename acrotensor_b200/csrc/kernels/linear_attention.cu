@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
 }
 
 // Turns the segments' own states into the states that they start from: one thread per entry of a state, walking a sequence's
-// segments in the order of time, a few loads ahead (144 segments of 128 x 128: 5 us; with the decay's power taken in every step and one
-// load at a time it was 89).
+// segments in the order of time, 16 loads ahead (with the decay's power taken in every step and one load at a time 144 segments of
+// 128 x 128 took 89 us).
 template <class A>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionArgs a)
 {
@@ -331,28 +331,48 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
     const double whole = left[0], tail = left[1];
     const int size = p.dq * p.dv;
     const int64_t step = static_cast<int64_t>(a.heads) * size;
-    for (int i = blockIdx.y * kThreads + threadIdx.x; i < size; i += gridDim.y * kThreads)
+    const int stride = gridDim.y * kThreads;
+    for (int i0 = blockIdx.y * kThreads + threadIdx.x; i0 < size; i0 += 2 * stride)
     {
-        double run = 0;
-        if (p.initial != nullptr)
+        const bool both = i0 + stride < size;
+        const int entry[2] = {i0, both ? i0 + stride : i0};
+        double run[2] = {0, 0};
+        A *states[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
         {
-            const A *from = static_cast<const A *>(p.initial) + (state * a.heads + head) * size;
-            run = p.turned ? from[i % p.dv * p.dq + i / p.dv] : from[i];
+            const int i = entry[e];
+            if (p.initial != nullptr)
+            {
+                const A *from = static_cast<const A *>(p.initial) + (state * a.heads + head) * size;
+                run[e] = p.turned ? from[i % p.dv * p.dq + i / p.dv] : from[i];
+            }
+            states[e] = static_cast<A *>(p.segment_states) + (first * a.heads + head) * size + i;
         }
-        A *states = static_cast<A *>(p.segment_states) + (first * a.heads + head) * size + i;
         for (int64_t k0 = 0; k0 < count; k0 += kJoin)
         {
-            A own[kJoin];
+            A own[2][kJoin];
 #pragma unroll
             for (int k = 0; k < kJoin; ++k)
-                if (k0 + k + 1 < count) own[k] = states[(reverse ? count - 1 - k0 - k : k0 + k) * step];
+                if (k0 + k + 1 < count)
+                {
+                    const int64_t at = (reverse ? count - 1 - k0 - k : k0 + k) * step;
+                    own[0][k] = states[0][at];
+                    own[1][k] = states[1][at];
+                }
 #pragma unroll
             for (int k = 0; k < kJoin; ++k)
             {
                 if (k0 + k >= count) break;
                 const int64_t at = reverse ? count - 1 - k0 - k : k0 + k;
-                states[at * step] = static_cast<A>(run);
-                if (k0 + k + 1 < count) run = (at == count - 1 ? tail : whole) * run + own[k];
+                states[0][at * step] = static_cast<A>(run[0]);
+                if (both) states[1][at * step] = static_cast<A>(run[1]);
+                if (k0 + k + 1 < count)
+                {
+                    const double left_over = at == count - 1 ? tail : whole;
+                    run[0] = left_over * run[0] + own[0][k];
+                    run[1] = left_over * run[1] + own[1][k];
+                }
             }
         }
     }
@@ -653,7 +673,7 @@ int run_all(const acro_b200_linear_attention_desc &d, AttentionArgs &a, cudaStre
         if (status != ACRO_B200_OK) return status;
         int64_t entries = 0;
         for (int i = 0; i < a.passes; ++i) entries = std::max<int64_t>(entries, static_cast<int64_t>(a.pass[i].dq) * a.pass[i].dv);
-        const dim3 grid(static_cast<unsigned>(a.sequences * a.heads), static_cast<unsigned>(std::min<int64_t>(16, (entries + kThreads - 1) / kThreads)), a.passes);
+        const dim3 grid(static_cast<unsigned>(a.sequences * a.heads), static_cast<unsigned>(std::min<int64_t>(32, (entries + 2 * kThreads - 1) / (2 * kThreads))), a.passes);
         if (d.type == ACRO_B200_F64) attention_join_kernel<double><<<grid, kThreads, 0, stream>>>(a);
         else attention_join_kernel<float><<<grid, kThreads, 0, stream>>>(a);
         status = launch_status("acro_b200_linear_attention");

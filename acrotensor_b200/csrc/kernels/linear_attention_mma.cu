@@ -11,7 +11,9 @@
 //
 // Precision: accumulators and the state are fp32.  The operands that are not inputs are sums of bf16 parts: P~ and S two parts (an
 // error of 2^-18 of an entry, 2^-9 of what the result's own rounding to bf16 loses), K~ three (2^-26), because the final state is an
-// fp32 result and collects every chunk's change.
+// fp32 result and collects every chunk's change.  The small parts are multiplied first: the tensor cores' additions lose up to a step of the
+// sum so far, so fewer of them happen at its full size; and no sum of theirs spans more than a chunk (spanning a segment of 58 cost the
+// final state a digit).
 //
 // Bound: by HBM 128 KB a chunk at 128 columns, about 2850 cycles of an SM at its share of 6.5 TB/s; the products take 1800 cycles of
 // the tensor pipe, the conversions about 2000 issue slots of the four schedulers, shared memory (operands of the products included)
@@ -86,7 +88,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t *bar)
 __device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_asleep(bar, parity)); }
 
 template <int NQ, int NV, bool SUMS>
-__global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ Maps maps, bool states_only)
+__global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ Maps maps)
 {
     using L = Layout<NQ, NV>;
     constexpr int PART = NQ * 16;               // columns of the state per thread
@@ -98,7 +100,6 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     const SegmentItem item = find_item(a, item_index, reverse);
     if (item.sequence < 0) return;
     const bool cut = segments_of(item.sequence_end - item.sequence_begin, a.segment) > 1;
-    if (states_only && (!cut || item.last)) return;
 
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -147,7 +148,6 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     {
         // The whole warp walks the loop; only the products and copies themselves are one lane's, by predicate and not by a branch, so
         // that addresses and descriptors stay in uniform registers (a product costs 30 to 60 cycles of issue less than with a branch).
-        const int stage_bytes = states_only ? (NQ + NV) * kBox : L::kStage;
         const int hq = head / p.q.group, hk = head / p.k.group, hv = head / p.v.group, n = a.offsets == nullptr ? static_cast<int>(item.sequence) : 0;
         const uint32_t leader = elect_lane();
         const auto load = [&](int c) {
@@ -156,11 +156,11 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             const int t = static_cast<int>(item.begin) + chunk_of(c) * kChunk;
             if (leader)
             {
-                mbar_arrive_expect_tx(bar, stage_bytes);
+                mbar_arrive_expect_tx(bar, L::kStage);
 #pragma unroll
                 for (int i = 0; i < NQ; ++i)
                 {
-                    if (!states_only) box_load(stage + L::kQ + i * kBox, &maps.q[pass], i * kBoxColumns, hq, t, n, bar);
+                    box_load(stage + L::kQ + i * kBox, &maps.q[pass], i * kBoxColumns, hq, t, n, bar);
                     box_load(stage + L::kK + i * kBox, &maps.k[pass], i * kBoxColumns, hk, t, n, bar);
                 }
 #pragma unroll
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             umma_commit(leader, &sh.scores);
         };
         int c = 0;
-        if (!states_only && chunks > 0)
+        if (chunks > 0)
         {
             ok = all_wait(&sh.full[0], 0);
             if (ok) issue_scores(0);
@@ -198,36 +198,30 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             if (!ok) break;
             tmem_fence_after_sync();
 #pragma unroll
-            for (int part = 0; part < 3; ++part)
+            for (int part = 2; part >= 0; --part)
 #pragma unroll
                 for (int k = 0; k < kChunk / 16; ++k)
-                    umma(leader, kDelta, v + k * 2048 / 16, scaled + (part * NQ * kBox + k * 2048) / 16, change_shape, part + k > 0);
+                    umma(leader, kDelta, v + k * 2048 / 16, scaled + (part * NQ * kBox + k * 2048) / 16, change_shape, part < 2 || k > 0);
             umma_commit(leader, &sh.change);
-            if (states_only)
-            {
-                // the previous chunk's stage is free: its change is complete (its reader was waited for above)
-                if (loaded < chunks) load(loaded++);
-                continue;
-            }
             // the previous chunk's results have been read, and before that its end state was published
             ok = c == 0 ? all_wait(&sh.state, 0) : all_wait(&sh.out_free, parity ^ 1);
             if (!ok) break;
             tmem_fence_after_sync();
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+            for (int part = 1; part >= 0; --part)
 #pragma unroll
                 for (int i = 0; i < NQ * 4; ++i)
-                    umma_tmem(leader, kFar, (part ? kStateLow : kStateHigh) + i * 8, q + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, part + i > 0);
+                    umma_tmem(leader, kFar, (part ? kStateLow : kStateHigh) + i * 8, q + (i / 4 * kBox + i % 4 * 32) / 16, by_columns, part < 1 || i > 0);
             // all of the previous chunk's products were waited for by the readers of their results: its stage is free
             if (loaded < chunks) load(loaded++);
             ok = all_wait(&sh.weights, parity);
             if (!ok) break;
             tmem_fence_after_sync();
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+            for (int part = 1; part >= 0; --part)
 #pragma unroll
                 for (int k = 0; k < kChunk / 16; ++k)
-                    umma(leader, kNear, v + k * 2048 / 16, weights + (part * kBox + k * 32) / 16, near_shape, part + k > 0);
+                    umma(leader, kNear, v + k * 2048 / 16, weights + (part * kBox + k * 32) / 16, near_shape, part < 1 || k > 0);
             umma_commit(leader, &sh.out);
             if (c + 1 < chunks)
             {
@@ -314,7 +308,6 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             if (odd) sh.odd[c % kRing] = 1;
             fence_proxy_async();
             warp_arrive(&sh.ready[c % L::kStages]);        // one barrier per stage: these warps may be a few chunks ahead
-            if (states_only) continue;
             // the previous chunk's weights have been read when its results have
             ok = all_wait(&sh.scores, parity) && (c == 0 || all_wait(&sh.out_free, parity ^ 1));
             if (!ok) break;
@@ -360,14 +353,11 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         {
             const float *from = nullptr;
             int turned = 0;
-            if (!states_only)
+            if (cut) from = static_cast<const float *>(p.segment_states) + (item_index * a.heads + head) * size;
+            else if (p.initial != nullptr)
             {
-                if (cut) from = static_cast<const float *>(p.segment_states) + (item_index * a.heads + head) * size;
-                else if (p.initial != nullptr)
-                {
-                    from = static_cast<const float *>(p.initial) + (item.state * a.heads + head) * size;
-                    turned = p.turned;
-                }
+                from = static_cast<const float *>(p.initial) + (item.state * a.heads + head) * size;
+                turned = p.turned;
             }
 #pragma unroll
             for (int j = 0; j < PART; j += 2)
@@ -400,12 +390,9 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             }
             tmem_wait_stores();
         };
-        if (!states_only)
-        {
-            publish();
-            tmem_fence_before_sync();
-            warp_arrive(&sh.state);
-        }
+        publish();
+        tmem_fence_before_sync();
+        warp_arrive(&sh.state);
         // rows of `out` are a 32-bit number of bytes apart
         const uint32_t step = static_cast<uint32_t>(p.out.token) * (SUMS ? 4u : 2u);
         char *out = reinterpret_cast<char *>(SUMS ? static_cast<void *>(rows_of<float>(p.out, a, item.sequence, head) + item.begin * p.out.token + b)
@@ -451,7 +438,6 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
 #pragma unroll
                     for (int j = 0; j < PART / 2; ++j) s[j] = ~0ull;
             }
-            if (states_only) continue;
             ok = all_wait(&sh.out, parity);         // the old state has been read, too
             if (!ok) break;
             tmem_fence_after_sync();
@@ -502,8 +488,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         if (!ok && lane == 0) *a.wait_flag = 1;
         float *to = nullptr;
         int turned = 0;
-        if (states_only) to = static_cast<float *>(p.segment_states) + (item_index * a.heads + head) * size;
-        else if (item.last && p.final != nullptr)
+        if (item.last && p.final != nullptr)
         {
             to = static_cast<float *>(p.final) + (item.state * a.heads + head) * size;
             turned = p.turned;
@@ -518,6 +503,194 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
     tmem_fence_before_sync();
     __syncthreads();
     if (warp == kIssueWarp) tmem_free(sh.tmem, kColumns);
+}
+
+// The state that a segment alone would end with: the sum over its tokens of what is left of k v^T at its end.  The weights reach to the
+// segment's end, so no state has to decay: the chunks are walked away from that end with a running factor.  16 warps make K~ (two
+// buffers) and add up the chunks' products (two accumulators); one issues.
+template <int NQ, int NV>
+struct StateLayout
+{
+    static constexpr int kWarps = 17, kBlock = kWarps * 32, kMakers = 512;
+    static constexpr int kStages = NQ == 2 ? 3 : 4;
+    static constexpr int kK = 0, kV = NQ * kBox, kStage = (NQ + NV) * kBox;
+    static constexpr int kScaled = kStages * kStage, kParts = 3 * NQ * kBox;
+    static constexpr int kTables = kScaled + 2 * kParts;
+    static constexpr int kDynamic = kTables + 1024 + 1024;
+    static constexpr uint32_t kColumns = NQ * 128;             // two accumulators
+};
+
+struct StateShared
+{
+    float left[kChunk + 4];
+    uint32_t tmem;
+    uint64_t full[4], ready[2], done[2];
+};
+
+template <int NQ, int NV>
+__global__ void __launch_bounds__(StateLayout<NQ, NV>::kBlock, 1) attention_states_kernel(const __grid_constant__ AttentionArgs a, const __grid_constant__ Maps maps)
+{
+    using L = StateLayout<NQ, NV>;
+    const int pass = blockIdx.y;
+    const AttentionPass &p = a.pass[pass];
+    const int head = blockIdx.x % a.heads;
+    const int64_t item_index = blockIdx.x / a.heads;
+    const bool reverse = p.reverse != 0;
+    const SegmentItem item = find_item(a, item_index, reverse);
+    if (item.sequence < 0 || item.last || segments_of(item.sequence_end - item.sequence_begin, a.segment) == 1) return;
+
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    StateShared &sh = *reinterpret_cast<StateShared *>(smem + L::kTables);
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x / 32), 0), lane = threadIdx.x % 32;
+    const double g = decay_log<float>(a.log_decay, head);
+    if (threadIdx.x <= kChunk) sh.left[threadIdx.x] = static_cast<float>(exp(g * threadIdx.x) * p.state_scale);
+    if (threadIdx.x == 0)
+    {
+        for (int i = 0; i < L::kStages; ++i) mbar_init(&sh.full[i], 1);
+        for (int i = 0; i < 2; ++i)
+        {
+            mbar_init(&sh.ready[i], L::kMakers / 32);
+            mbar_init(&sh.done[i], 1);
+        }
+        fence_mbar_init();
+    }
+    if (warp == 16) tmem_alloc(&sh.tmem, L::kColumns);
+    tmem_fence_before_sync();
+    __syncthreads();
+    tmem_fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    const int length = static_cast<int>(item.end - item.begin), chunks = (length + kChunk - 1) / kChunk;
+    const auto chunk_of = [&](int c) { return reverse ? c : chunks - 1 - c; };      // away from the end, in time
+    bool ok = true;
+
+    if (warp == 16)
+    {
+        const int hk = head / p.k.group, hv = head / p.v.group, n = a.offsets == nullptr ? static_cast<int>(item.sequence) : 0;
+        const uint32_t leader = elect_lane(), base = smem_addr(smem);
+        const auto load = [&](int c) {
+            unsigned char *stage = smem + c % L::kStages * L::kStage;
+            uint64_t *bar = &sh.full[c % L::kStages];
+            const int t = static_cast<int>(item.begin) + chunk_of(c) * kChunk;
+            if (leader)
+            {
+                mbar_arrive_expect_tx(bar, L::kStage);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) box_load(stage + L::kK + i * kBox, &maps.k[pass], i * kBoxColumns, hk, t, n, bar);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) box_load(stage + L::kV + i * kBox, &maps.v[pass], i * kBoxColumns, hv, t, n, bar);
+            }
+            __syncwarp();
+        };
+        int loaded = 0, c = 0;
+        for (; loaded < min(chunks, L::kStages - 1); ++loaded) load(loaded);
+        constexpr uint32_t shape = umma_shape(NQ * 64, true, true);
+#pragma unroll 1
+        for (; c < chunks; ++c)
+        {
+            ok = all_wait(&sh.ready[c & 1], c / 2 & 1);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            const uint64_t v = umma_operand(base + c % L::kStages * L::kStage + L::kV, NV == 2 ? kBox : 0, 1024),
+                           k = umma_operand(base + L::kScaled + (c & 1) * L::kParts, kBox, 1024);
+#pragma unroll
+            for (int part = 2; part >= 0; --part)
+#pragma unroll
+                for (int i = 0; i < kChunk / 16; ++i)
+                    umma(leader, tmem + (c & 1) * NQ * 64, v + i * 2048 / 16, k + (part * NQ * kBox + i * 2048) / 16, shape, part < 2 || i > 0);
+            umma_commit(leader, &sh.done[c & 1]);
+            if (loaded < chunks)
+            {
+                // into the previous chunk's stage
+                if (c > 0) ok = all_wait(&sh.done[(c - 1) & 1], (c - 1) / 2 & 1);
+                if (!ok) break;
+                load(loaded++);
+            }
+        }
+        if (!ok)
+        {
+            if (lane == 0) *a.wait_flag = 1;
+            for (int i = c; i < loaded; ++i) all_wait(&sh.full[i % L::kStages], i / L::kStages & 1);
+        }
+    }
+    else
+    {
+        const double whole = exp(g * kChunk);
+        double factor = 1;
+        const int b = warp % 4 * 32 + lane, d0 = warp / 4 * NQ * 16;
+        Two sum[NQ * 8];
+#pragma unroll
+        for (int j = 0; j < NQ * 8; ++j) sum[j] = two(0.0f, 0.0f);
+        const auto add = [&](int c) {
+#pragma unroll
+            for (int j = 0; j < NQ * 16; j += 16)
+            {
+                uint32_t x[16];
+                tmem_load_16(tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + (c & 1) * NQ * 64 + d0 + j, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[j / 2 + i] = add2(sum[j / 2 + i], two(x[2 * i], x[2 * i + 1]));
+            }
+            tmem_fence_before_sync();
+        };
+        for (int c = 0; c < chunks; ++c)
+        {
+            unsigned char *stage = smem + c % L::kStages * L::kStage, *scaled = smem + L::kScaled + (c & 1) * L::kParts;
+            const int m = min(kChunk, length - chunk_of(c) * kChunk);
+            // the buffer of K~ that this chunk takes was read by the products that were added up last
+            ok = all_wait(&sh.full[c % L::kStages], c / L::kStages & 1);
+            if (!ok) break;
+            const float f = static_cast<float>(factor);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+            {
+                const int piece = i * L::kMakers + threadIdx.x, r = piece / 8 % kChunk;
+                uint4 x = *reinterpret_cast<const uint4 *>(stage + L::kK + piece * 16);
+                if (r >= m) x = make_uint4(0, 0, 0, 0);
+                const float w = sh.left[r >= m ? 0 : reverse ? r + 1 : m - 1 - r] * f;
+                const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                uint32_t part[3][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    Two y = mul2(unpack_bf16(in[j]), two(w, w));
+                    part[0][j] = take_part(y);
+                    part[1][j] = take_part(y);
+                    part[2][j] = pack_bf16(y);
+                }
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    *reinterpret_cast<uint4 *>(scaled + k * NQ * kBox + piece * 16) = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
+            }
+            if (m < kChunk)
+            {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                {
+                    const int piece = i * L::kMakers + threadIdx.x;
+                    if (piece / 8 % kChunk >= m) *reinterpret_cast<uint4 *>(stage + L::kV + piece * 16) = make_uint4(0, 0, 0, 0);
+                }
+            }
+            fence_proxy_async();
+            warp_arrive(&sh.ready[c & 1]);
+            factor *= m == kChunk ? whole : exp(g * m);
+            if (c == 0) continue;
+            ok = all_wait(&sh.done[(c - 1) & 1], (c - 1) / 2 & 1);
+            if (!ok) break;
+            tmem_fence_after_sync();
+            add(c - 1);
+        }
+        if (ok) ok = all_wait(&sh.done[(chunks - 1) & 1], (chunks - 1) / 2 & 1);
+        if (!ok && lane == 0) *a.wait_flag = 1;
+        tmem_fence_after_sync();
+        add(chunks - 1);
+        float *to = static_cast<float *>(p.segment_states) + (item_index * a.heads + head) * (static_cast<int64_t>(p.dq) * p.dv);
+#pragma unroll
+        for (int j = 0; j < NQ * 16; ++j)
+            if (b < p.dv && d0 + j < p.dq) to[(d0 + j) * p.dv + b] = j % 2 ? second_of(sum[j / 2]) : first_of(sum[j / 2]);
+    }
+    tmem_fence_before_sync();
+    __syncthreads();
+    if (warp == 16) tmem_free(tmem, L::kColumns);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -564,20 +737,29 @@ bool make_map(CUtensorMap *map, const AttentionArgs &a, const TokenRows &r, int 
 }
 
 template <int NQ, int NV, bool SUMS>
-int launch_as(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStream_t stream)
+int launch_as(const AttentionArgs &a, const Maps &maps, cudaStream_t stream)
 {
     const char *name = "acro_b200_linear_attention";
     cudaError_t status = cudaFuncSetAttribute(attention_mma_kernel<NQ, NV, SUMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<NQ, NV>::kDynamic);
     if (status != cudaSuccess) return fail_cuda(status, name);
-    const int64_t grid = a.items * a.heads;
-    if (grid > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 segments x heads");
-    attention_mma_kernel<NQ, NV, SUMS><<<dim3(static_cast<unsigned>(grid), a.passes), kBlock, Layout<NQ, NV>::kDynamic, stream>>>(a, maps, states_only);
+    const dim3 grid(static_cast<unsigned>(a.items * a.heads), a.passes);
+    attention_mma_kernel<NQ, NV, SUMS><<<grid, kBlock, Layout<NQ, NV>::kDynamic, stream>>>(a, maps);
     return launch_status(name);
 }
 
 template <int NQ, int NV>
 int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStream_t stream)
 {
+    if (a.items * a.heads > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 segments x heads");
+    if (states_only)
+    {
+        const char *name = "acro_b200_linear_attention";
+        cudaError_t status = cudaFuncSetAttribute(attention_states_kernel<NQ, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, StateLayout<NQ, NV>::kDynamic);
+        if (status != cudaSuccess) return fail_cuda(status, name);
+        const dim3 grid(static_cast<unsigned>(a.items * a.heads), a.passes);
+        attention_states_kernel<NQ, NV><<<grid, StateLayout<NQ, NV>::kBlock, StateLayout<NQ, NV>::kDynamic, stream>>>(a, maps);
+        return launch_status(name);
+    }
     // one launch per kind of output: passes of the gradient write rows of sums when key and value heads are shared
     int status = ACRO_B200_OK;
     AttentionArgs part = a;
@@ -585,7 +767,7 @@ int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStrea
     for (int first = 0; first < a.passes && status == ACRO_B200_OK; first += part.passes)
     {
         part.passes = 0;
-        while (first + part.passes < a.passes && (states_only || a.pass[first + part.passes].sums == a.pass[first].sums))
+        while (first + part.passes < a.passes && a.pass[first + part.passes].sums == a.pass[first].sums)
         {
             part.pass[part.passes] = a.pass[first + part.passes];
             of.q[part.passes] = maps.q[first + part.passes];
@@ -593,8 +775,7 @@ int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStrea
             of.v[part.passes] = maps.v[first + part.passes];
             ++part.passes;
         }
-        status = a.pass[first].sums && !states_only ? launch_as<NQ, NV, true>(part, of, states_only, stream)
-                                                    : launch_as<NQ, NV, false>(part, of, states_only, stream);
+        status = a.pass[first].sums ? launch_as<NQ, NV, true>(part, of, stream) : launch_as<NQ, NV, false>(part, of, stream);
     }
     return status;
 }
