@@ -133,19 +133,19 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
     int turned = 0;
     if (!states_only)
     {
-        if (cut) from = static_cast<const A *>(p.segment_states) + (item_index * a.heads + head) * size;
+        if (cut) from = static_cast<const A *>(p.segment_states) + (item.item * a.heads + head) * size;
         else if (p.initial != nullptr)
         {
             from = static_cast<const A *>(p.initial) + (item.state * a.heads + head) * size;
             turned = p.turned;
         }
     }
+    const int along = turned ? 1 : p.dv, across = turned ? p.dq : 1;
+#pragma unroll 8
     for (int i = threadIdx.x; i < state_rows * SV; i += kThreads)
     {
         const int d = i / SV, c = i % SV;
-        A x = 0;
-        if (from != nullptr && d < p.dq && c < cols) x = turned ? from[(c0 + c) * p.dq + d] : from[d * p.dv + c0 + c];
-        st[i] = x;
+        st[i] = from != nullptr && d < p.dq && c < cols ? from[d * along + (c0 + c) * across] : A(0);
     }
     const T *q = rows_of<const T>(p.q, a, item.sequence, head), *k = rows_of<const T>(p.k, a, item.sequence, head),
             *v = rows_of<const T>(p.v, a, item.sequence, head) + c0;
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
     __syncthreads();
     A *to = nullptr;
     turned = 0;
-    if (states_only) to = static_cast<A *>(p.segment_states) + (item_index * a.heads + head) * size;
+    if (states_only) to = static_cast<A *>(p.segment_states) + (item.item * a.heads + head) * size;
     else if (item.last && p.final != nullptr)
     {
         to = static_cast<A *>(p.final) + (item.state * a.heads + head) * size;

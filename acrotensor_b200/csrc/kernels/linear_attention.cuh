@@ -65,7 +65,7 @@ struct SegmentItem
 {
     int64_t begin, end;                 // tokens of the sequence (of all rows when packed)
     int64_t sequence;                   // -1: no such item, or a sequence that is not there
-    int64_t first_item;                 // the sequence's first item
+    int64_t item;                       // its number in the natural order
     int64_t sequence_begin, sequence_end;
     int64_t state;                      // which of the user's states
     int32_t last;                       // is this the sequence's last item in the order of time?
@@ -105,66 +105,113 @@ __device__ __forceinline__ int64_t state_of(const int32_t *slots, int64_t n, int
     return mine;
 }
 
-// Item `item` of the list of all sequences' segments (in natural order).  Every thread of the CTA (at most 1024, whole warps)
-// calls it and gets the same answer; holds CTA barriers.
-__device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t item, bool reverse)
+// Inclusive sum over the CTA's threads of two counts, before each thread's own the sums of the threads in front of it.  Every thread
+// calls it; holds CTA barriers.
+__device__ __forceinline__ void scan_two(int64_t &x, int64_t &y, int64_t &total_x, int64_t &total_y, int64_t (*sums)[2])
+{
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+    const int64_t own_x = x, own_y = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const int64_t up_x = __shfl_up_sync(0xffffffffu, x, o), up_y = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o)
+        {
+            x += up_x;
+            y += up_y;
+        }
+    }
+    __syncthreads();
+    if (lane == 31)
+    {
+        sums[warp][0] = x;
+        sums[warp][1] = y;
+    }
+    __syncthreads();
+    total_x = total_y = 0;
+    int64_t ahead_x = 0, ahead_y = 0;
+    for (int w = 0; w < warps; ++w)
+    {
+        if (w == warp)
+        {
+            ahead_x = total_x;
+            ahead_y = total_y;
+        }
+        total_x += sums[w][0];
+        total_y += sums[w][1];
+    }
+    x += ahead_x - own_x;
+    y += ahead_y - own_y;
+}
+
+// Item `launched` of the list of all sequences' segments.  Packed sequences put their whole segments in front and their (shorter) last
+// ones behind, so that the long work starts first; states are kept under the natural number, s.item.  Every thread of the CTA (at most
+// 1024, whole warps) calls it and gets the same answer; holds CTA barriers.
+__device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t launched, bool reverse)
 {
     SegmentItem s;
+    int64_t index;
     if (a.offsets == nullptr)
     {
         const int64_t each = segments_of(a.tokens, a.segment);
-        s.sequence = item / each;
-        s.first_item = s.sequence * each;
+        s.sequence = launched / each;
+        index = launched - s.sequence * each;
+        s.item = launched;
         s.sequence_begin = 0;
         s.sequence_end = a.tokens;
     }
     else
     {
-        __shared__ int64_t found[4], warp_sums[33];
+        __shared__ int64_t found[5], sums[32][2];
         if (threadIdx.x == 0) found[0] = -1;
-        int64_t before = 0;
-        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+        // the number of whole segments of all sequences
+        int64_t all = 0;
+        for (int64_t n = threadIdx.x; n < a.sequences; n += blockDim.x)
+        {
+            int64_t b, e;
+            packed_range(a, n, &b, &e);
+            all += (e - b) / a.segment;
+        }
+        int64_t none = 0, whole, nothing;
+        scan_two(all, none, whole, nothing, sums);
+        int64_t before = 0, before_whole = 0;
         for (int64_t base = 0; base < a.sequences; base += blockDim.x)
         {
             const int64_t n = base + threadIdx.x;
-            int64_t b = 0, e = 0, mine = 0;
+            int64_t b = 0, e = 0, start = 0, start_whole = 0;
             if (n < a.sequences)
             {
                 packed_range(a, n, &b, &e);
-                mine = segments_of(e - b, a.segment);
+                start = segments_of(e - b, a.segment);
+                start_whole = (e - b) / a.segment;
             }
-            int64_t sum = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1)
-            {
-                const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += up;
-            }
-            __syncthreads();
-            if (lane == 31) warp_sums[warp] = sum;
-            __syncthreads();
-            int64_t total = 0, ahead = 0;
-            for (int w = 0; w < warps; ++w)
-            {
-                if (w == warp) ahead = total;
-                total += warp_sums[w];
-            }
-            const int64_t start = before + ahead + sum - mine;
-            if (mine > 0 && item >= start && item < start + mine)
+            const int64_t mine = start, mine_whole = start_whole;
+            int64_t total, total_whole;
+            scan_two(start, start_whole, total, total_whole, sums);
+            start += before;
+            start_whole += before_whole;
+            const int64_t start_last = start - start_whole;      // last segments in front of this sequence's: whole ones do not count
+            int64_t which = -1;
+            if (launched < whole && launched >= start_whole && launched < start_whole + mine_whole) which = launched - start_whole;
+            if (launched >= whole && mine > mine_whole && launched - whole == start_last) which = mine_whole;
+            if (which >= 0)
             {
                 found[0] = n;
-                found[1] = start;
+                found[1] = start + which;
                 found[2] = b;
                 found[3] = e;
+                found[4] = which;
             }
             before += total;
-            if (item < before) break;       // the same for every thread
+            before_whole += total_whole;
         }
         __syncthreads();
         s.sequence = found[0];
-        s.first_item = found[1];
+        s.item = found[1];
+        if (s.sequence >= 0 && s.item >= a.items) s.sequence = -1;       // only with offsets that decrease: more segments than rows allow
         s.sequence_begin = found[2];
         s.sequence_end = found[3];
+        index = found[4];
     }
     if (s.sequence < 0) return s;
     s.state = state_of(a.slots, s.sequence, a.state_count, a.bad_index);
@@ -173,7 +220,7 @@ __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t
         s.sequence = -1;
         return s;
     }
-    const int64_t index = item - s.first_item, count = segments_of(s.sequence_end - s.sequence_begin, a.segment);
+    const int64_t count = segments_of(s.sequence_end - s.sequence_begin, a.segment);
     s.begin = s.sequence_begin + index * a.segment;
     s.end = s.begin + a.segment < s.sequence_end ? s.begin + a.segment : s.sequence_end;
     s.first = reverse ? index == count - 1 : index == 0;

@@ -353,24 +353,20 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         {
             const float *from = nullptr;
             int turned = 0;
-            if (cut) from = static_cast<const float *>(p.segment_states) + (item_index * a.heads + head) * size;
+            if (cut) from = static_cast<const float *>(p.segment_states) + (item.item * a.heads + head) * size;
             else if (p.initial != nullptr)
             {
                 from = static_cast<const float *>(p.initial) + (item.state * a.heads + head) * size;
                 turned = p.turned;
             }
+            // one address for all of them, so that the loads go out together
+            const int along = turned ? 1 : p.dv, mine = turned ? b * p.dq : b;
+            const int there = from != nullptr && used ? min(PART, p.dq - d0) : 0;
+            float x[PART];
 #pragma unroll
-            for (int j = 0; j < PART; j += 2)
-            {
-                float x[2];
+            for (int j = 0; j < PART; ++j) x[j] = j < there ? from[mine + (d0 + j) * along] : 0.0f;
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                {
-                    const int d = d0 + j + e;
-                    x[e] = from != nullptr && used && d < p.dq ? (turned ? from[b * p.dq + d] : from[static_cast<int64_t>(d) * p.dv + b]) : 0.0f;
-                }
-                s[j / 2] = two(x[0], x[1]);
-            }
+            for (int j = 0; j < PART; j += 2) s[j / 2] = two(x[j], x[j + 1]);
         }
         const auto publish = [&]() {
             // the state as the A operand of the next chunk: two bf16 parts, pairs of columns
@@ -495,9 +491,10 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         }
         if (to != nullptr && used)
         {
+            const int along = turned ? 1 : p.dv, mine = turned ? b * p.dq : b;
 #pragma unroll
             for (int j = 0; j < PART; ++j)
-                if (d0 + j < p.dq) to[turned ? b * p.dq + d0 + j : static_cast<int64_t>(d0 + j) * p.dv + b] = j % 2 ? second_of(s[j / 2]) : first_of(s[j / 2]);
+                if (d0 + j < p.dq) to[mine + (d0 + j) * along] = j % 2 ? second_of(s[j / 2]) : first_of(s[j / 2]);
         }
     }
     tmem_fence_before_sync();
@@ -683,7 +680,7 @@ __global__ void __launch_bounds__(StateLayout<NQ, NV>::kBlock, 1) attention_stat
         if (!ok && lane == 0) *a.wait_flag = 1;
         tmem_fence_after_sync();
         add(chunks - 1);
-        float *to = static_cast<float *>(p.segment_states) + (item_index * a.heads + head) * (static_cast<int64_t>(p.dq) * p.dv);
+        float *to = static_cast<float *>(p.segment_states) + (item.item * a.heads + head) * (static_cast<int64_t>(p.dq) * p.dv);
 #pragma unroll
         for (int j = 0; j < NQ * 16; ++j)
             if (b < p.dv && d0 + j < p.dq) to[(d0 + j) * p.dv + b] = j % 2 ? second_of(sum[j / 2]) : first_of(sum[j / 2]);
