@@ -523,6 +523,7 @@ __global__ void __launch_bounds__(kThreads) attention_step_kernel(StepArgs a)
 // ---------------------------------------------------------------- host side
 
 constexpr int kSegmentQuantum = 128;    // every kernel's chunk divides it
+constexpr int kPlaneTokens = 128;       // fewer tokens stay on the ordinary cores
 
 std::string head_fault(const acro_b200_linear_attention_desc *d)
 {
@@ -580,7 +581,7 @@ size_t states_bytes(const acro_b200_linear_attention_desc &d, bool packed, int p
     for (int tensor_cores = 0; tensor_cores < 2; ++tensor_cores)
     {
         const int64_t segment = segment_tokens(d, packed, tensor_cores != 0, passes);
-        if (may_cut(d, segment) && (tensor_cores == 0 || d.type == ACRO_B200_BF16))
+        if (may_cut(d, segment) && (tensor_cores == 0 || d.type != ACRO_B200_F64))
             most = std::max(most, round256(static_cast<size_t>(item_bound(d, packed, segment)) * d.q_heads * d.dk * d.dv * statistic_bytes(d.type)));
     }
     return most;
@@ -652,7 +653,7 @@ int run_pass(const AttentionArgs &a, bool states_only, cudaStream_t stream)
 
 int run_pass_of(int type, const AttentionArgs &a, bool tensor_cores, bool states_only, cudaStream_t stream)
 {
-    if (tensor_cores) return attention_mma_launch(a, states_only, stream);
+    if (tensor_cores) return attention_mma_launch(a, type, states_only, stream);
     switch (type)
     {
     case ACRO_B200_F64: return run_pass<double>(a, states_only, stream);
@@ -662,9 +663,33 @@ int run_pass_of(int type, const AttentionArgs &a, bool tensor_cores, bool states
     }
 }
 
-int run_all(const acro_b200_linear_attention_desc &d, AttentionArgs &a, cudaStream_t stream)
+// Do inputs of these sizes go to the tensor cores as planes of bf16 parts?  fp64 has none; bf16 rows of a multiple of eight columns are
+// read as they are (and stay on the other path if they are not aligned).  A few tokens are not worth the planes.
+bool takes_planes(const acro_b200_linear_attention_desc &d)
 {
-    const bool packed = a.offsets != nullptr, tensor_cores = d.type == ACRO_B200_BF16 && attention_mma_supported(a);
+    if (d.type == ACRO_B200_F64 || d.dk > 128 || d.dv > 128 || d.tokens < kPlaneTokens) return false;
+    return d.type != ACRO_B200_BF16 || d.dk % 8 != 0 || d.dv % 8 != 0;
+}
+
+size_t planes_bytes(const acro_b200_linear_attention_desc &d, bool packed, bool gradient)
+{
+    if (!takes_planes(d)) return 0;
+    const int64_t rows = packed ? d.tokens : d.sequences * d.tokens;
+    return attention_planes_bytes(d.type, rows, d.q_heads, d.dk) + attention_planes_bytes(d.type, rows, d.kv_heads, d.dk) +
+           attention_planes_bytes(d.type, rows, d.kv_heads, d.dv) + (gradient ? attention_planes_bytes(d.type, rows, d.q_heads, d.dv) : 0);
+}
+
+// `arrays`: q, k, v (and dout) as the passes use them; `planes`: scratch of planes_bytes.
+int run_all(const acro_b200_linear_attention_desc &d, AttentionArgs &a, const TokenRows *arrays, const int *columns, int count, void *planes,
+            cudaStream_t stream)
+{
+    const bool packed = a.offsets != nullptr, sizes = d.type != ACRO_B200_F64 && attention_mma_sizes(a);
+    const bool direct = sizes && d.type == ACRO_B200_BF16 && attention_mma_direct(a), tensor_cores = direct || (sizes && takes_planes(d));
+    if (tensor_cores && !direct)
+    {
+        const int status = attention_split(a, d.type, arrays, columns, count, planes, stream);
+        if (status != ACRO_B200_OK) return status;
+    }
     a.segment = segment_tokens(d, packed, tensor_cores, a.passes);
     a.items = item_bound(d, packed, a.segment);
     if (may_cut(d, a.segment))
@@ -673,7 +698,8 @@ int run_all(const acro_b200_linear_attention_desc &d, AttentionArgs &a, cudaStre
         if (status != ACRO_B200_OK) return status;
         int64_t entries = 0;
         for (int i = 0; i < a.passes; ++i) entries = std::max<int64_t>(entries, static_cast<int64_t>(a.pass[i].dq) * a.pass[i].dv);
-        const dim3 grid(static_cast<unsigned>(a.sequences * a.heads), static_cast<unsigned>(std::min<int64_t>(32, (entries + 2 * kThreads - 1) / (2 * kThreads))), a.passes);
+        const dim3 grid(static_cast<unsigned>(a.sequences * a.heads), static_cast<unsigned>(std::min<int64_t>(32, (entries + 2 * kThreads - 1) / (2 * kThreads))),
+                        a.passes);
         if (d.type == ACRO_B200_F64) attention_join_kernel<double><<<grid, kThreads, 0, stream>>>(a);
         else attention_join_kernel<float><<<grid, kThreads, 0, stream>>>(a);
         status = launch_status("acro_b200_linear_attention");
@@ -705,7 +731,7 @@ extern "C" {
 size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
 {
     if (!head_fault(desc).empty()) return 0;
-    return states_bytes(*desc, packed != 0, 1);
+    return states_bytes(*desc, packed != 0, 1) + planes_bytes(*desc, packed != 0, false);
 }
 
 int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -730,7 +756,7 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
     if (fault.empty() && slots != nullptr && state_count < 0) fault = "negative state_count";
     if (fault.empty() && slots == nullptr && state_count != d.sequences && (initial_state != nullptr || final_state != nullptr))
         fault = "without slots there is one state per sequence";
-    const size_t need = states_bytes(d, packed, 1);
+    const size_t states = states_bytes(d, packed, 1), need = states + planes_bytes(d, packed, false);
     if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
         fault = "scratch is smaller than acro_b200_linear_attention_scratch_bytes or not 16-byte aligned";
     if (fault.empty() && need > 0 && !on_current_device(scratch)) fault = "scratch is not memory of the current device";
@@ -762,7 +788,9 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
     p.initial = initial_state;
     p.final = final_state;
     p.segment_states = scratch;
-    return run_all(d, a, as_stream(stream));
+    const TokenRows arrays[3] = {p.q, p.k, p.v};
+    const int columns[3] = {d.dk, d.dk, d.dv};
+    return run_all(d, a, arrays, columns, 3, static_cast<unsigned char *>(scratch) + states, as_stream(stream));
 }
 
 int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -841,7 +869,8 @@ int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc,
 size_t acro_b200_linear_attention_backward_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
 {
     if (!head_fault(desc).empty()) return 0;
-    return 3 * states_bytes(*desc, packed != 0, 3) + shared_bytes(*desc, packed != 0, desc->dk) + shared_bytes(*desc, packed != 0, desc->dv);
+    return 3 * states_bytes(*desc, packed != 0, 3) + shared_bytes(*desc, packed != 0, desc->dk) + shared_bytes(*desc, packed != 0, desc->dv) +
+           planes_bytes(*desc, packed != 0, true);
 }
 
 int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -856,11 +885,11 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     const acro_b200_linear_attention_desc &d = *desc;
     if (d.sequences == 0) return ACRO_B200_OK;
     const bool packed = offsets != nullptr, rows = d.tokens > 0;
-    const struct { const acro_b200_token_array *x; int columns, heads; const char *name; } arrays[] = {
+    const struct { const acro_b200_token_array *x; int columns, heads; const char *name; } given[] = {
         {q, d.dk, d.q_heads, "q"}, {k, d.dk, d.kv_heads, "k"}, {v, d.dv, d.kv_heads, "v"}, {dout, d.dv, d.q_heads, "dout"},
         {dq, d.dk, d.q_heads, "dq"}, {dk, d.dk, d.kv_heads, "dk"}, {dv, d.dv, d.kv_heads, "dv"}};
     if (rows)
-        for (const auto &x : arrays)
+        for (const auto &x : given)
             if (fault.empty()) fault = array_fault(x.x, x.columns, x.heads, d.tokens, d.sequences, packed, x.name);
     if (fault.empty() && log_decay == nullptr) fault = "log_decay is a null pointer";
     const size_t need = acro_b200_linear_attention_backward_scratch_bytes(desc, packed);
@@ -910,11 +939,13 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     a.pass[2].q = rk;
     a.pass[2].k = rq;
     a.pass[2].v = ro;
+    const TokenRows arrays[4] = {rq, rk, rv, ro};
+    const int columns[4] = {d.dk, d.dk, d.dv, d.dv};
     if (group == 1)
     {
         a.pass[1].out = rows_from(rows ? *dk : none, 1);
         a.pass[2].out = rows_from(rows ? *dv : none, 1);
-        return run_all(d, a, as_stream(stream));
+        return run_all(d, a, arrays, columns, 4, at, as_stream(stream));
     }
     // a row of sums per query head, added up afterwards
     ShareArgs both = {{nullptr, nullptr}, {rows_from(rows ? *dk : none, 1), rows_from(rows ? *dv : none, 1)}, {d.dk, d.dv}};
@@ -927,7 +958,7 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
         at += shared_bytes(d, packed, both.columns[i]);
     }
     cudaStream_t st = as_stream(stream);
-    status = run_all(d, a, st);
+    status = run_all(d, a, arrays, columns, 4, at, st);
     if (status != ACRO_B200_OK || !rows) return status;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((packed ? 1 : d.sequences) * d.tokens, 148 * 16)), 2);
     switch (d.type)

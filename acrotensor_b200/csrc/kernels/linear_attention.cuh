@@ -242,9 +242,14 @@ __device__ __forceinline__ A decay_log(const void *log_decay, int head)
     return g < A(-1e5) ? A(-1e5) : g;
 }
 
-// The pass on the tcgen05 tensor cores for bf16 (linear_attention_mma.cu), for operands that tiled copies can read.
-bool attention_mma_supported(const AttentionArgs &a);
-int attention_mma_launch(const AttentionArgs &a, bool states_only, cudaStream_t stream);
+// The pass on the tcgen05 tensor cores (linear_attention_mma.cuh).  Its inputs are bf16 rows that tiled copies can read
+// (attention_mma_direct), or the planes of bf16 parts that attention_split makes of any rows of up to 32 bits, in whose place it then
+// puts the planes (attention_planes_bytes for each array, one behind the other).
+bool attention_mma_sizes(const AttentionArgs &a);
+bool attention_mma_direct(const AttentionArgs &a);
+size_t attention_planes_bytes(int type, int64_t rows, int heads, int columns);
+int attention_split(AttentionArgs &a, int type, const TokenRows *arrays, const int *columns, int count, void *planes, cudaStream_t stream);
+int attention_mma_launch(const AttentionArgs &a, int type, bool states_only, cudaStream_t stream);
 
 }
 
