@@ -399,18 +399,19 @@ __global__ void __launch_bounds__(kThreads) attention_share_kernel(const __grid_
         begin = min(max(a.offsets[0], int64_t(0)), a.tokens);
         end = min(max(a.offsets[a.sequences], int64_t(0)), a.tokens);
     }
-    for (int64_t row = begin + blockIdx.x; row < end; row += gridDim.x)
+    const int each = heads * columns, some = max(1, 1024 / each);       // rows at once
+    for (int64_t first = begin + static_cast<int64_t>(blockIdx.x) * some; first < end; first += static_cast<int64_t>(gridDim.x) * some)
     {
-        const int64_t n = a.offsets == nullptr ? row / a.tokens : 0, t = a.offsets == nullptr ? row % a.tokens : row;
-        const A *from = sums + row * heads * group * columns;
-        T *to = static_cast<T *>(out.data) + n * out.sequence + t * out.token;
-        for (int i = threadIdx.x; i < heads * columns; i += kThreads)
+        const int count = static_cast<int>(min(static_cast<int64_t>(some), end - first)) * each;
+#pragma unroll 2
+        for (int i = threadIdx.x; i < count; i += kThreads)
         {
-            const int h = i / columns, c = i % columns;
-            const A *x = from + h * group * columns + c;
+            const int own = i / each, rest = i - own * each, h = rest / columns, c = rest - h * columns;
+            const int64_t row = first + own, n = a.offsets == nullptr ? row / a.tokens : 0, t = row - n * a.tokens;
+            const A *x = sums + (row * heads + h) * group * columns + c;
             A s = x[0];
             for (int k = 1; k < group; ++k) s += x[k * columns];
-            to[h * out.head + c] = narrow<T>(s);
+            static_cast<T *>(out.data)[n * out.sequence + t * out.token + h * out.head + c] = narrow<T>(s);
         }
     }
 }
@@ -960,7 +961,7 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     cudaStream_t st = as_stream(stream);
     status = run_all(d, a, arrays, columns, 4, at, st);
     if (status != ACRO_B200_OK || !rows) return status;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((packed ? 1 : d.sequences) * d.tokens, 148 * 16)), 2);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((packed ? 1 : d.sequences) * d.tokens, 148 * 8)), 2);
     switch (d.type)
     {
     case ACRO_B200_F64: attention_share_kernel<double><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group); break;

@@ -48,12 +48,12 @@ bool make_map(CUtensorMap *map, const AttentionArgs &a, const TokenRows &r, int 
 }
 
 // The bf16 parts of an array, plane by plane: planes[part][sequence][token][head][columns], columns filled up to a multiple of eight
-// with zeros so that tiled copies can read them.  One CTA per row (all heads of a token).
+// with zeros so that tiled copies can read them.  A CTA takes a few rows (all heads of a token), a thread four columns at a time.
 struct SplitArgs
 {
     TokenRows from[4];
     __nv_bfloat16 *to[4];
-    int32_t columns[4], heads[4];
+    int32_t columns[4], heads[4], packs[4];     // packs: four columns can be read at once
     const int64_t *offsets;
     int64_t sequences, tokens;
 };
@@ -61,8 +61,9 @@ struct SplitArgs
 template <class T, int IN>
 __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_constant__ SplitArgs a)
 {
-    const int array = blockIdx.y, columns = a.columns[array], filled = (columns + 7) / 8 * 8, heads = a.heads[array], half = filled / 2;
+    const int array = blockIdx.y, columns = a.columns[array], heads = a.heads[array], quads = (columns + 7) / 8 * 2, each = heads * quads;
     const TokenRows &r = a.from[array];
+    const bool packs = a.packs[array] != 0;
     const int64_t rows = a.offsets == nullptr ? a.sequences * a.tokens : a.tokens;
     int64_t begin = 0, end = rows;
     if (a.offsets != nullptr)
@@ -71,29 +72,47 @@ __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_const
         begin = min(max(a.offsets[0], int64_t(0)), rows);
         end = min(max(a.offsets[a.sequences], int64_t(0)), rows);
     }
-    const int64_t plane = rows * heads * half;
-    for (int64_t row = begin + blockIdx.x; row < end; row += gridDim.x)
+    const int some = max(1, 1024 / each);       // rows at once
+    const int64_t plane = rows * each;
+    for (int64_t first = begin + static_cast<int64_t>(blockIdx.x) * some; first < end; first += static_cast<int64_t>(gridDim.x) * some)
     {
-        const int64_t n = a.offsets == nullptr ? row / a.tokens : 0, t = a.offsets == nullptr ? row - n * a.tokens : row;
-        const T *from = static_cast<const T *>(r.data) + n * r.sequence + t * r.token;
-        uint32_t *to = reinterpret_cast<uint32_t *>(a.to[array]) + row * heads * half;
-        for (int i = threadIdx.x; i < heads * half; i += 256)
+        const int count = static_cast<int>(min(static_cast<int64_t>(some), end - first)) * each;
+        uint2 *to = reinterpret_cast<uint2 *>(a.to[array]) + first * each;
+#pragma unroll 2
+        for (int i = threadIdx.x; i < count; i += 256)
         {
-            const int h = i / half, c = (i - h * half) * 2;
-            const T *x = from + h * r.head + c;
-            float y[2];
-            uint32_t part[IN];
+            const int own = i / each, rest = i - own * each, h = rest / quads, c = (rest - h * quads) * 4;
+            const int64_t row = first + own, n = a.offsets == nullptr ? row / a.tokens : 0, t = row - n * a.tokens;
+            const T *x = static_cast<const T *>(r.data) + n * r.sequence + t * r.token + h * r.head + c;
+            Two y[2];
+            if (packs && c < columns)
+            {
+                const Pack<T, 4> p = load_pack<T, 4>(x);
+                y[0] = two(widen(p.x[0]), widen(p.x[1]));
+                y[1] = two(widen(p.x[2]), widen(p.x[3]));
+            }
+            else
+            {
+                float z[4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) y[e] = c + e < columns ? static_cast<float>(widen(x[e])) : 0.0f;
+                for (int e = 0; e < 4; ++e) z[e] = c + e < columns ? static_cast<float>(widen(x[e])) : 0.0f;
+                y[0] = two(z[0], z[1]);
+                y[1] = two(z[2], z[3]);
+            }
 #pragma unroll
             for (int k = 0; k < IN; ++k)
             {
-                part[k] = pack_bf16(two(y[0], y[1]));
-                const float first = __uint_as_float(part[k] << 16), second = __uint_as_float(part[k] & 0xffff0000u);
-                // infinities and NaN are the first part's alone
-                y[0] = isfinite(first) ? y[0] - first : 0.0f;
-                y[1] = isfinite(second) ? y[1] - second : 0.0f;
-                to[k * plane + i] = part[k];
+                uint2 part;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                {
+                    const uint32_t w = pack_bf16(y[e]);
+                    const Two left = sub2(y[e], unpack_bf16(w));
+                    // infinities and NaN are the first part's alone
+                    y[e] = two(odd_half(w) ? 0.0f : first_of(left), odd_half(w >> 16) ? 0.0f : second_of(left));
+                    (e ? part.y : part.x) = w;
+                }
+                to[k * plane + i] = part;
             }
         }
     }
@@ -155,11 +174,14 @@ int attention_split(AttentionArgs &a, int type, const TokenRows *arrays, const i
         s.from[i] = arrays[i];
         s.to[i] = reinterpret_cast<__nv_bfloat16 *>(at);
         s.columns[i] = columns[i];
+        const int64_t pack = 4 * (type == ACRO_B200_F32 ? 4 : 2);
+        s.packs[i] = columns[i] % 4 == 0 && reinterpret_cast<uintptr_t>(arrays[i].data) % pack == 0 && arrays[i].sequence % 4 == 0 && arrays[i].token % 4 == 0 &&
+                     arrays[i].head % 4 == 0;
         s.heads[i] = heads;
         plane[i] = {at, static_cast<int64_t>(heads) * filled * a.tokens, static_cast<int64_t>(heads) * filled, filled, arrays[i].group};
         at += attention_planes_bytes(type, rows, heads, columns[i]);
     }
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, 148 * 32)), count);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, 148 * 8)), count);
     if (type == ACRO_B200_F32) attention_split_kernel<float, 3><<<grid, 256, 0, stream>>>(s);
     else if (type == ACRO_B200_F16) attention_split_kernel<__half, 2><<<grid, 256, 0, stream>>>(s);
     else attention_split_kernel<__nv_bfloat16, 1><<<grid, 256, 0, stream>>>(s);

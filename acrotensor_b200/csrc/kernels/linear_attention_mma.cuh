@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <cuda.h>
+#include <type_traits>
 
 using namespace acro_b200_detail;
 
@@ -806,7 +807,7 @@ int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStrea
     for (int first = 0; first < a.passes && status == ACRO_B200_OK; first += part.passes)
     {
         part.passes = 0;
-        while (first + part.passes < a.passes && a.pass[first + part.passes].sums == a.pass[first].sums)
+        while (first + part.passes < a.passes && (std::is_same<T, float>::value || a.pass[first + part.passes].sums == a.pass[first].sums))
         {
             part.pass[part.passes] = a.pass[first + part.passes];
             of.q[part.passes] = maps.q[first + part.passes];
