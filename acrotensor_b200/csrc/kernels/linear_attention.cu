@@ -383,35 +383,53 @@ struct ShareArgs
     const void *sums[2];
     TokenRows out[2];
     int32_t columns[2];
+    int32_t heads, group;
+    const int64_t *offsets;
+    int64_t sequences, tokens;
 };
 
-// out[row, h, c] = sum over the query heads of head h, in ascending order: the gradients of shared keys and values.
+// out[row, h, c] = sum over the query heads of head h, in ascending order: the gradients of shared keys (blockIdx.y = 0) and values.
 template <class T>
-__global__ void __launch_bounds__(kThreads) attention_share_kernel(const __grid_constant__ AttentionArgs a, ShareArgs both, int heads, int group)
+__global__ void __launch_bounds__(kThreads) attention_share_kernel(const __grid_constant__ ShareArgs a)
 {
     using A = typename Element<T>::Acc;
-    const A *sums = static_cast<const A *>(both.sums[blockIdx.y]);
-    const TokenRows out = both.out[blockIdx.y];
-    const int columns = both.columns[blockIdx.y];
+    constexpr int AT_ONCE = 4;
+    const A *sums = static_cast<const A *>(blockIdx.y ? a.sums[1] : a.sums[0]);
+    const TokenRows &out = blockIdx.y ? a.out[1] : a.out[0];
+    const int columns = blockIdx.y ? a.columns[1] : a.columns[0], group = a.group;
     int64_t begin = 0, end = a.sequences * a.tokens;
     if (a.offsets != nullptr)
     {
         begin = min(max(a.offsets[0], int64_t(0)), a.tokens);
         end = min(max(a.offsets[a.sequences], int64_t(0)), a.tokens);
     }
-    const int each = heads * columns, some = max(1, 1024 / each);       // rows at once
+    const int each = a.heads * columns, some = max(1, 1024 / each);     // rows at once
     for (int64_t first = begin + static_cast<int64_t>(blockIdx.x) * some; first < end; first += static_cast<int64_t>(gridDim.x) * some)
     {
         const int count = static_cast<int>(min(static_cast<int64_t>(some), end - first)) * each;
-#pragma unroll 2
-        for (int i = threadIdx.x; i < count; i += kThreads)
+        for (int i0 = threadIdx.x; i0 < count; i0 += AT_ONCE * kThreads)
         {
-            const int own = i / each, rest = i - own * each, h = rest / columns, c = rest - h * columns;
-            const int64_t row = first + own, n = a.offsets == nullptr ? row / a.tokens : 0, t = row - n * a.tokens;
-            const A *x = sums + (row * heads + h) * group * columns + c;
-            A s = x[0];
-            for (int k = 1; k < group; ++k) s += x[k * columns];
-            static_cast<T *>(out.data)[n * out.sequence + t * out.token + h * out.head + c] = narrow<T>(s);
+            A s[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) s[u] = 0;
+            for (int k = 0; k < group; ++k)
+            {
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u)
+                {
+                    const int i = i0 + u * kThreads, h = i / columns;       // over the heads of all these rows
+                    if (i < count) s[u] += sums[((first * a.heads + h) * group + k) * columns + (i - h * columns)];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+            {
+                const int i = i0 + u * kThreads;
+                if (i >= count) break;
+                const int own = i / each, rest = i - own * each, h = rest / columns, c = rest - h * columns;
+                const int64_t row = first + own, n = a.offsets == nullptr ? row / a.tokens : 0, t = row - n * a.tokens;
+                static_cast<T *>(out.data)[n * out.sequence + t * out.token + h * out.head + c] = narrow<T>(s[u]);
+            }
         }
     }
 }
@@ -949,7 +967,8 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
         return run_all(d, a, arrays, columns, 4, at, as_stream(stream));
     }
     // a row of sums per query head, added up afterwards
-    ShareArgs both = {{nullptr, nullptr}, {rows_from(rows ? *dk : none, 1), rows_from(rows ? *dv : none, 1)}, {d.dk, d.dv}};
+    ShareArgs both = {{nullptr, nullptr}, {rows_from(rows ? *dk : none, 1), rows_from(rows ? *dv : none, 1)}, {d.dk, d.dv}, d.kv_heads, group, offsets, d.sequences,
+                      d.tokens};
     for (int i = 0; i < 2; ++i)
     {
         both.sums[i] = at;
@@ -964,10 +983,10 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((packed ? 1 : d.sequences) * d.tokens, 148 * 8)), 2);
     switch (d.type)
     {
-    case ACRO_B200_F64: attention_share_kernel<double><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group); break;
-    case ACRO_B200_F32: attention_share_kernel<float><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group); break;
-    case ACRO_B200_BF16: attention_share_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group); break;
-    default: attention_share_kernel<__half><<<grid, kThreads, 0, st>>>(a, both, d.kv_heads, group);
+    case ACRO_B200_F64: attention_share_kernel<double><<<grid, kThreads, 0, st>>>(both); break;
+    case ACRO_B200_F32: attention_share_kernel<float><<<grid, kThreads, 0, st>>>(both); break;
+    case ACRO_B200_BF16: attention_share_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(both); break;
+    default: attention_share_kernel<__half><<<grid, kThreads, 0, st>>>(both);
     }
     return launch_status("acro_b200_linear_attention_backward");
 }
