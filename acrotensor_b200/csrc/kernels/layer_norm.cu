@@ -18,6 +18,7 @@
 #include "element.cuh"
 
 #include <algorithm>
+#include <initializer_list>
 
 using namespace acro_b200_detail;
 
@@ -498,6 +499,14 @@ bool packs_fit(int type, int64_t width, std::initializer_list<const void *> poin
     return true;
 }
 
+// Pointers that kernels will read or write, null ones aside.
+bool all_on_device(std::initializer_list<const void *> pointers)
+{
+    for (const void *p : pointers)
+        if (p != nullptr && !on_current_device(p)) return false;
+    return true;
+}
+
 const char *shape_fault(int type, int64_t rows, int64_t width)
 {
     if (!known_type(type)) return "unknown element type";
@@ -519,7 +528,7 @@ int acro_b200_layer_norm(int type, const void *x, int64_t x_stride, const void *
     if (x == nullptr || y == nullptr) return fail_invalid("acro_b200_layer_norm: null pointer");
     if (x_stride < width || y_stride < width) return fail_invalid("acro_b200_layer_norm: rows overlap (a row stride is smaller than the width)");
     if (x == y && x_stride != y_stride) return fail_invalid("acro_b200_layer_norm: in place, but with different row strides");
-    if (!on_current_device(x) || !on_current_device(y)) return fail_invalid("acro_b200_layer_norm: a pointer is not memory of the current device");
+    if (!all_on_device({x, weight, bias, y, mean, rstd})) return fail_invalid("acro_b200_layer_norm: a pointer is not memory of the current device");
     NormArgs a = {x, weight, bias, nullptr, y, mean, rstd, nullptr, rows, width, x_stride, y_stride, 0, eps, 0};
     const Shape s = norm_shape(type, rows, width, packs_fit(type, width, {x, weight, bias, y}, {x_stride, y_stride}), false);
     a.group = s.group;
@@ -559,7 +568,7 @@ int acro_b200_layer_norm_backward(int type, const void *dy, int64_t dy_stride, c
         return fail_invalid(std::string(name) + "rows overlap (a row stride is smaller than the width)");
     if ((dx == x && dx_stride != x_stride) || (dx == dy && dx_stride != dy_stride))
         return fail_invalid(std::string(name) + "in place, but with different row strides");
-    if (!on_current_device(dy) || !on_current_device(x) || !on_current_device(dx))
+    if (!all_on_device({dy, x, weight, mean, rstd, dx, dweight, dbias}))
         return fail_invalid(std::string(name) + "a pointer is not memory of the current device");
     const Shape s = norm_shape(type, rows, width, packs_fit(type, width, {x, weight, dy, dx}, {x_stride, dy_stride, dx_stride}), true);
     const bool sums = dweight != nullptr || dbias != nullptr;

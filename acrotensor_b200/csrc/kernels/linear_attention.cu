@@ -3,6 +3,7 @@
 #include "linear_attention.cuh"
 
 #include <algorithm>
+#include <initializer_list>
 
 using namespace acro_b200_detail;
 
@@ -615,6 +616,14 @@ size_t shared_bytes(const acro_b200_linear_attention_desc &d, bool packed, int c
 
 TokenRows rows_from(const acro_b200_token_array &x, int group) { return {x.data, x.sequence_stride, x.token_stride, x.head_stride, group}; }
 
+// Pointers that kernels will read or write, null ones aside.
+bool all_on_device(std::initializer_list<const void *> pointers)
+{
+    for (const void *p : pointers)
+        if (p != nullptr && !on_current_device(p)) return false;
+    return true;
+}
+
 std::string array_fault(const acro_b200_token_array *x, int64_t columns, int heads, int64_t tokens, int64_t sequences, bool packed, const char *name)
 {
     const std::string n(name);
@@ -778,9 +787,8 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
     const size_t states = states_bytes(d, packed, 1), need = states + planes_bytes(d, packed, false);
     if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
         fault = "scratch is smaller than acro_b200_linear_attention_scratch_bytes or not 16-byte aligned";
-    if (fault.empty() && need > 0 && !on_current_device(scratch)) fault = "scratch is not memory of the current device";
-    if (fault.empty() && ((initial_state != nullptr && !on_current_device(initial_state)) || (final_state != nullptr && !on_current_device(final_state))))
-        fault = "a state is not memory of the current device";
+    if (fault.empty() && !all_on_device({log_decay, offsets, slots, initial_state, final_state, need > 0 ? scratch : nullptr}))
+        fault = "log_decay, offsets, slots, a state or scratch is not memory of the current device";
     if (fault.empty() && rows && (out->data == q->data || out->data == k->data || out->data == v->data))
         fault = "out takes the place of an operand that is still read";
     if (!fault.empty()) return fail_invalid(name + fault);
@@ -828,7 +836,7 @@ int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc,
     if (fault.empty()) fault = array_fault(v, d.dv, d.kv_heads, 1, d.sequences, false, "v");
     if (fault.empty()) fault = array_fault(out, d.dv, d.q_heads, 1, d.sequences, false, "out");
     if (fault.empty() && (log_decay == nullptr || state_in == nullptr || state_out == nullptr)) fault = "null pointer";
-    if (fault.empty() && (!on_current_device(state_in) || !on_current_device(state_out))) fault = "a state is not memory of the current device";
+    if (fault.empty() && !all_on_device({log_decay, state_in, state_out, slots})) fault = "log_decay, slots or a state is not memory of the current device";
     if (fault.empty() && (state_count < 0 || (slots == nullptr && state_count != d.sequences))) fault = "without slots there is one state per sequence";
     if (!fault.empty()) return fail_invalid(name + fault);
     StepArgs a = {};
@@ -914,15 +922,15 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     const size_t need = acro_b200_linear_attention_backward_scratch_bytes(desc, packed);
     if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
         fault = "scratch is smaller than acro_b200_linear_attention_backward_scratch_bytes or not 16-byte aligned";
-    if (fault.empty() && need > 0 && !on_current_device(scratch)) fault = "scratch is not memory of the current device";
-    for (const void *s : {initial_state, d_final_state, static_cast<const void *>(d_initial_state)})
-        if (fault.empty() && s != nullptr && !on_current_device(s)) fault = "a state is not memory of the current device";
+    if (fault.empty() && !all_on_device({log_decay, offsets, initial_state, d_final_state, d_initial_state, need > 0 ? scratch : nullptr}))
+        fault = "log_decay, offsets, a state or scratch is not memory of the current device";
     if (fault.empty() && d_initial_state != nullptr && (d_initial_state == d_final_state || d_initial_state == initial_state))
         fault = "d_initial_state takes the place of a state that is still read";
     if (fault.empty() && rows)
         for (const acro_b200_token_array *to : {dq, dk, dv})
             for (const acro_b200_token_array *from : {q, k, v, dout})
                 if (to->data == from->data) fault = "a gradient takes the place of an operand that is still read";
+    if (fault.empty() && rows && (dq->data == dk->data || dq->data == dv->data || dk->data == dv->data)) fault = "two gradients take the same place";
     if (!fault.empty()) return fail_invalid(name + fault);
     AttentionArgs a = {};
     int status = common_args(d, log_decay, offsets, &a);

@@ -449,6 +449,122 @@ def test_operands_that_would_be_overwritten_are_refused():
         ab.linear_attention(long.blank(1, 64), long.q, long.k, long.v, long.g, scratch=torch.empty(64, device="cuda"), stream=stream())
     with pytest.raises(ab.AcroError):       # host memory
         ab.linear_attention(torch.empty(1, 70, 1, 64, dtype=torch.bfloat16), p.q, p.k, p.v, p.g, stream=stream())
+    with pytest.raises(ab.AcroError):
+        ab.linear_attention_backward(outs[0], outs[0], outs[1], p.dout, p.q, p.k, p.v, p.g, stream=stream())
+
+
+def test_host_memory_is_refused_wherever_it_stands():
+    """Every pointer that a kernel would follow: an error, not a launch."""
+    p = Problem("f32", [40, 30], True, 2, 2, 16, 16)
+    out, host = p.blank(2, 16), lambda x: x.cpu()
+    slots = torch.zeros(2, dtype=torch.int32, device="cuda")
+    good = dict(log_decay=p.g, offsets=p.offsets, initial_state=p.initial, final_state=p.initial.clone(), slots=slots)
+    for name in good:
+        with pytest.raises(ab.AcroError):
+            ab.linear_attention(out, p.q, p.k, p.v, **{**good, name: host(good[name])}, stream=stream())
+    q, k, v, o = p.q[:2], p.k[:2], p.v[:2], out[:2]
+    good = dict(state_out=p.initial.clone(), q=q, k=k, v=v, log_decay=p.g, state_in=p.initial, slots=slots)
+    for name in good:
+        with pytest.raises(ab.AcroError):
+            ab.linear_attention_step(o, **{**good, name: host(good[name])}, stream=stream())
+    good = dict(log_decay=p.g, offsets=p.offsets, initial_state=p.initial, d_final_state=p.dfinal, d_initial_state=torch.empty_like(p.dfinal))
+    outs = [p.blank(2, 16) for _ in range(3)]
+    for name in good:
+        with pytest.raises(ab.AcroError):
+            ab.linear_attention_backward(*outs, p.dout, p.q, p.k, p.v, **{**good, name: host(good[name])}, stream=stream())
+    x, w, r = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda"), torch.ones(4, device="cuda")
+    good = dict(out=torch.empty_like(x), x=x, weight=w, bias=w, mean=r, rstd=r)
+    for name in good:
+        with pytest.raises(ab.AcroError):
+            ab.layer_norm(**{**good, name: host(good[name])}, stream=stream())
+    good = dict(dx=torch.empty_like(x), dweight=w, dbias=w.clone(), dout=x, x=x, mean=r, rstd=r, weight=w,
+                scratch=scratch_for(ab.layer_norm_backward_scratch_bytes(x)))
+    for name in good:
+        with pytest.raises(ab.AcroError):
+            ab.layer_norm_backward(**{**good, name: host(good[name])}, stream=stream())
+    status_ok()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32", "f64"])
+def test_nothing_at_all(kind):
+    """No sequences, no rows, no tokens: states pass through, gradients of states too."""
+    p = Problem(kind, [0, 0, 0], True, 2, 1, 16, 8, spare=0)
+    assert p.q.numel() == 0
+    out, end = p.forward()
+    assert torch.equal(end, p.initial)
+    assert torch.equal(p.backward()[3], p.dfinal)
+    e = torch.empty(2, 0, 2, 16, dtype=DTYPES[kind], device="cuda")
+    final = torch.empty_like(p.initial[:2])
+    ab.linear_attention(e[..., :8], e, e[:, :, :1], e[:, :, :1, :8], p.g, initial_state=p.initial[:2], final_state=final, stream=stream())
+    assert torch.equal(final, p.initial[:2])
+    n = torch.empty(0, 5, 2, 16, dtype=DTYPES[kind], device="cuda")
+    ab.linear_attention(n, n, n, n, p.g, stream=stream())
+    status_ok()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32", "f16"])
+def test_arrays_off_their_boundaries(kind):
+    """Rows that start off the 16-byte boundaries which copies like best, head strides longer than the head, tokens behind heads."""
+    dt = DTYPES[kind]
+    for d, pad, offset in ((64, 1, 0), (64, 0, 3), (40, 3, 1), (128, 8, 8)):
+        p = Problem(kind, [150, 140], True, 2, 2, d, d, seed=pad + offset)
+        for name in ("q", "k", "v", "dout"):
+            x = getattr(p, name)
+            rows, h = x.shape[0], x.shape[1]
+            buf = torch.full((h, rows * (d + pad) + offset + 8), float("nan"), dtype=dt, device="cuda")
+            view = buf[:, offset:offset + rows * (d + pad)].unflatten(1, (rows, d + pad))[..., :d].transpose(0, 1)
+            view.copy_(x)
+            setattr(p, name, view)
+        p.check_forward(*p.forward())
+        p.check_backward(*p.backward())
+    status_ok()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32", "f64"])
+def test_more_sequences_than_threads(kind):
+    """Thousands of sequences, most of them a few tokens or none, long ones among them."""
+    lengths = [i % 4 for i in range(1500)] + [700] + [i % 3 for i in range(900)] + [1300, 1]
+    p = Problem(kind, lengths, True, 1, 1, 16, 16, decay=[-1 / 50])
+    out, end = p.forward()
+    grads = p.backward()
+    keep = [0, 1, 2, 3, 799, 801, 1499, 1500, 1501, 2398, 2399, 2400, 2401]
+    for i in keep:
+        one = Problem(kind, [lengths[i]], True, 1, 1, 16, 16, decay=[-1 / 50])
+        for name in ("q", "k", "v", "dout"):
+            x = p.of(getattr(p, name), i)
+            setattr(one, name, torch.cat([x, torch.full((3,) + tuple(x.shape[1:]), float("nan"), dtype=x.dtype, device="cuda")]))
+        one.initial, one.dfinal = p.initial[i:i + 1], p.dfinal[i:i + 1]
+        pad = lambda x: torch.cat([p.of(x, i), torch.full((3,) + tuple(x.shape[1:]), -7.0, dtype=x.dtype, device="cuda")])
+        one.check_forward(pad(out), end[i:i + 1])
+        one.check_backward(*[pad(x) for x in grads[:3]], grads[3][i:i + 1])
+    p.untouched(out, *grads[:3])
+    status_ok()
+
+
+def test_offsets_beyond_31_bits():
+    """A cache of more than 2^31 entries, and arrays of more than 2^31 elements of which one sequence at the end is used."""
+    count, d = 140000, 128
+    cache = torch.empty(count, 1, d, d, device="cuda")
+    p = Problem("bf16", [1, 1], False, 1, 1, d, d)
+    slots = [count - 1, 131072]
+    cache[slots] = p.initial
+    out = torch.zeros(2, 1, d, dtype=torch.bfloat16, device="cuda")
+    ab.linear_attention_step(out, cache, p.q[:, 0], p.k[:, 0], p.v[:, 0], p.g, cache, scale=p.scale,
+                             slots=torch.tensor(slots, dtype=torch.int32, device="cuda"), stream=stream())
+    p.check_forward(out[:, None], cache[slots])
+    del cache
+    rows, heads, tokens = 70000, 256, 130
+    big = Problem("bf16", [tokens], True, heads, heads, d, d, states=False, spare=0)
+    wide_rows = {n: torch.empty(rows, heads, d, dtype=torch.bfloat16, device="cuda") for n in ("q", "k", "v", "out")}
+    for n in ("q", "k", "v"):
+        wide_rows[n][-tokens:] = getattr(big, n)
+    offsets = torch.tensor([rows - tokens, rows], device="cuda")
+    q, k, v, out = (wide_rows[n] for n in ("q", "k", "v", "out"))
+    ab.linear_attention(out, q, k, v, big.g, scale=big.scale, offsets=offsets, scratch=scratch_for(ab.linear_attention_scratch_bytes(q, k, v, offsets)),
+                        stream=stream())
+    expect, _ = big.forward()
+    assert torch.equal(out[-tokens:], expect)
+    status_ok()
 
 
 # ---------------------------------------------------------------- layer norm
