@@ -5,6 +5,7 @@
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <initializer_list>
 
 #include "common.cuh"
 
@@ -232,6 +233,22 @@ inline bool on_current_device(const void *p)
     }
     if (a.type == cudaMemoryTypeDevice) return a.device == dev;
     return a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeHost && a.devicePointer != nullptr);
+}
+
+// The same for several pointers, null ones aside.
+inline bool all_on_device(std::initializer_list<const void *> pointers)
+{
+    for (const void *p : pointers)
+        if (p != nullptr && !on_current_device(p)) return false;
+    return true;
+}
+
+// Do these arrays start on a boundary of their elements?
+inline bool aligned_to(std::initializer_list<const void *> pointers, size_t bytes)
+{
+    for (const void *p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return false;
+    return true;
 }
 
 }

@@ -18,7 +18,6 @@
 #include "element.cuh"
 
 #include <algorithm>
-#include <initializer_list>
 
 using namespace acro_b200_detail;
 
@@ -499,14 +498,6 @@ bool packs_fit(int type, int64_t width, std::initializer_list<const void *> poin
     return true;
 }
 
-// Pointers that kernels will read or write, null ones aside.
-bool all_on_device(std::initializer_list<const void *> pointers)
-{
-    for (const void *p : pointers)
-        if (p != nullptr && !on_current_device(p)) return false;
-    return true;
-}
-
 const char *shape_fault(int type, int64_t rows, int64_t width)
 {
     if (!known_type(type)) return "unknown element type";
@@ -528,6 +519,8 @@ int acro_b200_layer_norm(int type, const void *x, int64_t x_stride, const void *
     if (x == nullptr || y == nullptr) return fail_invalid("acro_b200_layer_norm: null pointer");
     if (x_stride < width || y_stride < width) return fail_invalid("acro_b200_layer_norm: rows overlap (a row stride is smaller than the width)");
     if (x == y && x_stride != y_stride) return fail_invalid("acro_b200_layer_norm: in place, but with different row strides");
+    if (!aligned_to({x, weight, bias, y}, element_bytes(type)) || !aligned_to({mean, rstd}, statistic_bytes(type)))
+        return fail_invalid("acro_b200_layer_norm: a pointer is not aligned to its elements");
     if (!all_on_device({x, weight, bias, y, mean, rstd})) return fail_invalid("acro_b200_layer_norm: a pointer is not memory of the current device");
     NormArgs a = {x, weight, bias, nullptr, y, mean, rstd, nullptr, rows, width, x_stride, y_stride, 0, eps, 0};
     const Shape s = norm_shape(type, rows, width, packs_fit(type, width, {x, weight, bias, y}, {x_stride, y_stride}), false);
@@ -553,10 +546,13 @@ int acro_b200_layer_norm_backward(int type, const void *dy, int64_t dy_stride, c
     const char *name = "acro_b200_layer_norm_backward: ";
     if (const char *fault = shape_fault(type, rows, width)) return fail_invalid(std::string(name) + fault);
     cudaStream_t st = as_stream(stream);
+    if (!aligned_to({dy, x, weight, dx}, element_bytes(type)) || !aligned_to({mean, rstd, dweight, dbias}, statistic_bytes(type)))
+        return fail_invalid(std::string(name) + "a pointer is not aligned to its elements");
+    if (dweight != nullptr && dweight == dbias) return fail_invalid(std::string(name) + "dweight and dbias take the same place");
     if (rows == 0)
     {
         // sums over no rows
-        if ((dweight != nullptr && !on_current_device(dweight)) || (dbias != nullptr && !on_current_device(dbias)))
+        if (!all_on_device({dweight, dbias}))
             return fail_invalid(std::string(name) + "a pointer is not memory of the current device");
         const size_t bytes = static_cast<size_t>(width) * statistic_bytes(type);
         if (dweight != nullptr && cudaMemsetAsync(dweight, 0, bytes, st) != cudaSuccess) return fail_cuda(cudaGetLastError(), name);

@@ -3,7 +3,6 @@
 #include "linear_attention.cuh"
 
 #include <algorithm>
-#include <initializer_list>
 
 using namespace acro_b200_detail;
 
@@ -134,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
     int turned = 0;
     if (!states_only)
     {
-        if (cut) from = static_cast<const A *>(p.segment_states) + (item.item * a.heads + head) * size;
+        if (cut) from = static_cast<const A *>(p.segment_states) + (item.segment_state * a.heads + head) * size;
         else if (p.initial != nullptr)
         {
             from = static_cast<const A *>(p.initial) + (item.state * a.heads + head) * size;
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
     __syncthreads();
     A *to = nullptr;
     turned = 0;
-    if (states_only) to = static_cast<A *>(p.segment_states) + (item.item * a.heads + head) * size;
+    if (states_only) to = static_cast<A *>(p.segment_states) + (item.segment_state * a.heads + head) * size;
     else if (item.last && p.final != nullptr)
     {
         to = static_cast<A *>(p.final) + (item.state * a.heads + head) * size;
@@ -298,7 +297,6 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
 template <class A>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionArgs a)
 {
-    __shared__ unsigned long long total;
     __shared__ double left[2];
     const AttentionPass &p = a.pass[blockIdx.z];
     const int head = blockIdx.x % a.heads;
@@ -310,23 +308,7 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
     if (count <= 1) return;
     // only the sequence's last segment is shorter; what it leaves matters backward in time alone
     if (threadIdx.x < 2) left[threadIdx.x] = exp(decay_log<A>(a.log_decay, head) * static_cast<double>(threadIdx.x == 0 ? a.segment : end - begin - (count - 1) * a.segment));
-    if (threadIdx.x == 2) total = 0;
     __syncthreads();
-    int64_t first = n * count;
-    if (a.offsets != nullptr)
-    {
-        unsigned long long before = 0;
-        for (int64_t i = threadIdx.x; i < n; i += kThreads)
-        {
-            int64_t b, e;
-            packed_range(a, i, &b, &e);
-            before += segments_of(e - b, a.segment);
-        }
-        if (before > 0) atomicAdd(&total, before);
-        __syncthreads();
-        first = static_cast<int64_t>(total);
-    }
-    if (first + count > a.items) return;        // more segments than rows allow: only with offsets that decrease
     const int64_t state = state_of(a.slots, n, a.state_count, a.bad_index);
     if (state < 0) return;
     const double whole = left[0], tail = left[1];
@@ -348,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
                 const A *from = static_cast<const A *>(p.initial) + (state * a.heads + head) * size;
                 run[e] = p.turned ? from[i % p.dv * p.dq + i / p.dv] : from[i];
             }
-            states[e] = static_cast<A *>(p.segment_states) + (first * a.heads + head) * size + i;
+            states[e] = static_cast<A *>(p.segment_states) + static_cast<int64_t>(head) * size + i;
         }
         for (int64_t k0 = 0; k0 < count; k0 += kJoin)
         {
@@ -357,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
             for (int k = 0; k < kJoin; ++k)
                 if (k0 + k + 1 < count)
                 {
-                    const int64_t at = (reverse ? count - 1 - k0 - k : k0 + k) * step;
+                    const int64_t at = segment_state(a, n, begin, reverse ? count - 1 - k0 - k : k0 + k) * step;
                     own[0][k] = states[0][at];
                     own[1][k] = states[1][at];
                 }
@@ -366,8 +348,9 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
             {
                 if (k0 + k >= count) break;
                 const int64_t at = reverse ? count - 1 - k0 - k : k0 + k;
-                states[0][at * step] = static_cast<A>(run[0]);
-                if (both) states[1][at * step] = static_cast<A>(run[1]);
+                const int64_t place = segment_state(a, n, begin, at) * step;
+                states[0][place] = static_cast<A>(run[0]);
+                if (both) states[1][place] = static_cast<A>(run[1]);
                 if (k0 + k + 1 < count)
                 {
                     const double left_over = at == count - 1 ? tail : whole;
@@ -544,8 +527,9 @@ __global__ void __launch_bounds__(kThreads) attention_step_kernel(StepArgs a)
 
 constexpr int kSegmentQuantum = 128;    // every kernel's chunk divides it
 constexpr int kPlaneTokens = 128;       // fewer tokens stay on the ordinary cores
+constexpr int64_t kMaxRows = int64_t(1) << 40;      // of all heads, more than any memory holds: sizes of scratch stay within 64 bits
 
-std::string head_fault(const acro_b200_linear_attention_desc *d)
+std::string head_fault(const acro_b200_linear_attention_desc *d, bool packed)
 {
     if (d == nullptr) return "null descriptor";
     if (!known_type(d->type)) return "unknown element type";
@@ -553,6 +537,8 @@ std::string head_fault(const acro_b200_linear_attention_desc *d)
     if (d->q_heads > 65535) return "more than 65535 heads";
     if (d->dk < 1 || d->dk > kMaxHead || d->dv < 1 || d->dv > kMaxHead) return "head sizes are not in 1 .. 256";
     if (d->sequences < 0 || d->tokens < 0) return "negative number of sequences or tokens";
+    const int64_t most = kMaxRows / d->q_heads;
+    if (d->tokens > most || d->sequences > most || (!packed && d->sequences > 0 && d->tokens > most / d->sequences)) return "more than 2^40 rows of all heads";
     if (!(d->scale - d->scale == 0)) return "the scale is not finite";
     return "";
 }
@@ -602,7 +588,7 @@ size_t states_bytes(const acro_b200_linear_attention_desc &d, bool packed, int p
     {
         const int64_t segment = segment_tokens(d, packed, tensor_cores != 0, passes);
         if (may_cut(d, segment) && (tensor_cores == 0 || d.type != ACRO_B200_F64))
-            most = std::max(most, round256(static_cast<size_t>(item_bound(d, packed, segment)) * d.q_heads * d.dk * d.dv * statistic_bytes(d.type)));
+            most = std::max(most, round256(static_cast<size_t>(states_of_segments(d.sequences, d.tokens, segment, packed)) * d.q_heads * d.dk * d.dv * statistic_bytes(d.type)));
     }
     return most;
 }
@@ -616,21 +602,14 @@ size_t shared_bytes(const acro_b200_linear_attention_desc &d, bool packed, int c
 
 TokenRows rows_from(const acro_b200_token_array &x, int group) { return {x.data, x.sequence_stride, x.token_stride, x.head_stride, group}; }
 
-// Pointers that kernels will read or write, null ones aside.
-bool all_on_device(std::initializer_list<const void *> pointers)
-{
-    for (const void *p : pointers)
-        if (p != nullptr && !on_current_device(p)) return false;
-    return true;
-}
-
-std::string array_fault(const acro_b200_token_array *x, int64_t columns, int heads, int64_t tokens, int64_t sequences, bool packed, const char *name)
+std::string array_fault(const acro_b200_linear_attention_desc &d, const acro_b200_token_array *x, int64_t columns, int heads, int64_t tokens, int64_t sequences,
+                        bool packed, const char *name)
 {
     const std::string n(name);
     if (x == nullptr || x->data == nullptr) return n + " is a null pointer";
     if ((heads > 1 && x->head_stride < columns) || (tokens > 1 && x->token_stride < columns) || (!packed && sequences > 1 && x->sequence_stride < columns))
         return n + " has rows that overlap";
-    if (!on_current_device(x->data)) return n + " is not memory of the current device";
+    if (!aligned_to({x->data}, element_bytes(d.type))) return n + " is not aligned to its elements";
     return "";
 }
 
@@ -758,7 +737,7 @@ extern "C" {
 
 size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
 {
-    if (!head_fault(desc).empty()) return 0;
+    if (!head_fault(desc, packed != 0).empty()) return 0;
     return states_bytes(*desc, packed != 0, 1) + planes_bytes(*desc, packed != 0, false);
 }
 
@@ -768,17 +747,17 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
                                void *stream)
 {
     const std::string name = "acro_b200_linear_attention: ";
-    std::string fault = head_fault(desc);
+    std::string fault = head_fault(desc, offsets != nullptr);
     if (!fault.empty()) return fail_invalid(name + fault);
     const acro_b200_linear_attention_desc &d = *desc;
     if (d.sequences == 0) return ACRO_B200_OK;
     const bool packed = offsets != nullptr, rows = d.tokens > 0;
     if (rows)
     {
-        if (fault.empty()) fault = array_fault(q, d.dk, d.q_heads, d.tokens, d.sequences, packed, "q");
-        if (fault.empty()) fault = array_fault(k, d.dk, d.kv_heads, d.tokens, d.sequences, packed, "k");
-        if (fault.empty()) fault = array_fault(v, d.dv, d.kv_heads, d.tokens, d.sequences, packed, "v");
-        if (fault.empty()) fault = array_fault(out, d.dv, d.q_heads, d.tokens, d.sequences, packed, "out");
+        if (fault.empty()) fault = array_fault(d, q, d.dk, d.q_heads, d.tokens, d.sequences, packed, "q");
+        if (fault.empty()) fault = array_fault(d, k, d.dk, d.kv_heads, d.tokens, d.sequences, packed, "k");
+        if (fault.empty()) fault = array_fault(d, v, d.dv, d.kv_heads, d.tokens, d.sequences, packed, "v");
+        if (fault.empty()) fault = array_fault(d, out, d.dv, d.q_heads, d.tokens, d.sequences, packed, "out");
     }
     if (fault.empty() && log_decay == nullptr) fault = "log_decay is a null pointer";
     if (fault.empty() && slots != nullptr && state_count < 0) fault = "negative state_count";
@@ -787,10 +766,13 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
     const size_t states = states_bytes(d, packed, 1), need = states + planes_bytes(d, packed, false);
     if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
         fault = "scratch is smaller than acro_b200_linear_attention_scratch_bytes or not 16-byte aligned";
-    if (fault.empty() && !all_on_device({log_decay, offsets, slots, initial_state, final_state, need > 0 ? scratch : nullptr}))
-        fault = "log_decay, offsets, slots, a state or scratch is not memory of the current device";
+    if (fault.empty() && (!aligned_to({log_decay, initial_state, final_state}, statistic_bytes(d.type)) || !aligned_to({offsets}, 8) || !aligned_to({slots}, 4)))
+        fault = "log_decay, offsets, slots or a state is not aligned to its elements";
     if (fault.empty() && rows && (out->data == q->data || out->data == k->data || out->data == v->data))
         fault = "out takes the place of an operand that is still read";
+    if (fault.empty() && ((rows && !all_on_device({q->data, k->data, v->data, out->data})) ||
+                          !all_on_device({log_decay, offsets, slots, initial_state, final_state, need > 0 ? scratch : nullptr})))
+        fault = "an array, log_decay, offsets, slots, a state or scratch is not memory of the current device";
     if (!fault.empty()) return fail_invalid(name + fault);
     AttentionArgs a = {};
     int status = common_args(d, log_decay, offsets, &a);
@@ -825,19 +807,24 @@ int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc,
                                     void *state_out, const int32_t *slots, int64_t state_count, void *stream)
 {
     const std::string name = "acro_b200_linear_attention_step: ";
-    std::string fault = head_fault(desc);
+    std::string fault = head_fault(desc, false);
     if (!fault.empty()) return fail_invalid(name + fault);
     const acro_b200_linear_attention_desc &d = *desc;
     if (d.tokens != 1) return fail_invalid(name + "a step takes one token of each sequence");
     if (d.sequences == 0) return ACRO_B200_OK;
     // the distance of two requests is that of two sequences
-    fault = array_fault(q, d.dk, d.q_heads, 1, d.sequences, false, "q");
-    if (fault.empty()) fault = array_fault(k, d.dk, d.kv_heads, 1, d.sequences, false, "k");
-    if (fault.empty()) fault = array_fault(v, d.dv, d.kv_heads, 1, d.sequences, false, "v");
-    if (fault.empty()) fault = array_fault(out, d.dv, d.q_heads, 1, d.sequences, false, "out");
+    fault = array_fault(d, q, d.dk, d.q_heads, 1, d.sequences, false, "q");
+    if (fault.empty()) fault = array_fault(d, k, d.dk, d.kv_heads, 1, d.sequences, false, "k");
+    if (fault.empty()) fault = array_fault(d, v, d.dv, d.kv_heads, 1, d.sequences, false, "v");
+    if (fault.empty()) fault = array_fault(d, out, d.dv, d.q_heads, 1, d.sequences, false, "out");
     if (fault.empty() && (log_decay == nullptr || state_in == nullptr || state_out == nullptr)) fault = "null pointer";
-    if (fault.empty() && !all_on_device({log_decay, state_in, state_out, slots})) fault = "log_decay, slots or a state is not memory of the current device";
+    if (fault.empty() && (!aligned_to({log_decay, state_in, state_out}, statistic_bytes(d.type)) || !aligned_to({slots}, 4)))
+        fault = "log_decay, slots or a state is not aligned to its elements";
+    if (fault.empty() && (out->data == q->data || out->data == k->data || out->data == v->data))
+        fault = "out takes the place of an operand that is still read";
     if (fault.empty() && (state_count < 0 || (slots == nullptr && state_count != d.sequences))) fault = "without slots there is one state per sequence";
+    if (fault.empty() && !all_on_device({q->data, k->data, v->data, out->data, log_decay, state_in, state_out, slots}))
+        fault = "an array, log_decay, slots or a state is not memory of the current device";
     if (!fault.empty()) return fail_invalid(name + fault);
     StepArgs a = {};
     const int group = d.q_heads / d.kv_heads;
@@ -895,7 +882,7 @@ int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc,
 
 size_t acro_b200_linear_attention_backward_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed)
 {
-    if (!head_fault(desc).empty()) return 0;
+    if (!head_fault(desc, packed != 0).empty()) return 0;
     return 3 * states_bytes(*desc, packed != 0, 3) + shared_bytes(*desc, packed != 0, desc->dk) + shared_bytes(*desc, packed != 0, desc->dv) +
            planes_bytes(*desc, packed != 0, true);
 }
@@ -907,7 +894,7 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
                                         size_t scratch_bytes, void *stream)
 {
     const std::string name = "acro_b200_linear_attention_backward: ";
-    std::string fault = head_fault(desc);
+    std::string fault = head_fault(desc, offsets != nullptr);
     if (!fault.empty()) return fail_invalid(name + fault);
     const acro_b200_linear_attention_desc &d = *desc;
     if (d.sequences == 0) return ACRO_B200_OK;
@@ -917,13 +904,13 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
         {dq, d.dk, d.q_heads, "dq"}, {dk, d.dk, d.kv_heads, "dk"}, {dv, d.dv, d.kv_heads, "dv"}};
     if (rows)
         for (const auto &x : given)
-            if (fault.empty()) fault = array_fault(x.x, x.columns, x.heads, d.tokens, d.sequences, packed, x.name);
+            if (fault.empty()) fault = array_fault(d, x.x, x.columns, x.heads, d.tokens, d.sequences, packed, x.name);
     if (fault.empty() && log_decay == nullptr) fault = "log_decay is a null pointer";
     const size_t need = acro_b200_linear_attention_backward_scratch_bytes(desc, packed);
     if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))
         fault = "scratch is smaller than acro_b200_linear_attention_backward_scratch_bytes or not 16-byte aligned";
-    if (fault.empty() && !all_on_device({log_decay, offsets, initial_state, d_final_state, d_initial_state, need > 0 ? scratch : nullptr}))
-        fault = "log_decay, offsets, a state or scratch is not memory of the current device";
+    if (fault.empty() && (!aligned_to({log_decay, initial_state, d_final_state, d_initial_state}, statistic_bytes(d.type)) || !aligned_to({offsets}, 8)))
+        fault = "log_decay, offsets or a state is not aligned to its elements";
     if (fault.empty() && d_initial_state != nullptr && (d_initial_state == d_final_state || d_initial_state == initial_state))
         fault = "d_initial_state takes the place of a state that is still read";
     if (fault.empty() && rows)
@@ -931,6 +918,11 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
             for (const acro_b200_token_array *from : {q, k, v, dout})
                 if (to->data == from->data) fault = "a gradient takes the place of an operand that is still read";
     if (fault.empty() && rows && (dq->data == dk->data || dq->data == dv->data || dk->data == dv->data)) fault = "two gradients take the same place";
+    if (fault.empty() && rows)
+        for (const auto &x : given)
+            if (!all_on_device({x.x->data})) fault = std::string(x.name) + " is not memory of the current device";
+    if (fault.empty() && !all_on_device({log_decay, offsets, initial_state, d_final_state, d_initial_state, need > 0 ? scratch : nullptr}))
+        fault = "log_decay, offsets, a state or scratch is not memory of the current device";
     if (!fault.empty()) return fail_invalid(name + fault);
     AttentionArgs a = {};
     int status = common_args(d, log_decay, offsets, &a);

@@ -42,7 +42,7 @@ struct AttentionPass
     double state_scale, out_scale;      // on k v^T as it enters the state, on q^T S; their product on (q.k) v
     const void *initial;                // state a sequence starts from, or null: zero
     void *final;                        // state it ends with, or null
-    void *segment_states;               // [items][heads][dq][dv], or null when no sequence is cut
+    void *segment_states;               // [states_of_segments][heads][dq][dv], or null when no sequence is cut
 };
 
 struct AttentionArgs
@@ -65,14 +65,28 @@ struct SegmentItem
 {
     int64_t begin, end;                 // tokens of the sequence (of all rows when packed)
     int64_t sequence;                   // -1: no such item, or a sequence that is not there
-    int64_t item;                       // its number in the natural order
+    int64_t segment_state;              // where the states of a cut sequence's segment are kept
     int64_t sequence_begin, sequence_end;
     int64_t state;                      // which of the user's states
     int32_t last;                       // is this the sequence's last item in the order of time?
     int32_t first;
 };
 
-__device__ __forceinline__ int64_t segments_of(int64_t length, int64_t segment) { return length <= segment ? 1 : (length + segment - 1) / segment; }
+__host__ __device__ __forceinline__ int64_t segments_of(int64_t length, int64_t segment) { return length <= segment ? 1 : (length + segment - 1) / segment; }
+
+// Where the state of segment `index` of a cut sequence is kept.  Packed: two places for every `segment` rows, the second for a
+// sequence's first segment.  Two segments that start within the same `segment` rows are the last one of a sequence and the first one
+// of the next that is cut, so that is enough, and the memory does not grow with the number of sequences.
+__host__ __device__ __forceinline__ int64_t states_of_segments(int64_t sequences, int64_t tokens, int64_t segment, bool packed)
+{
+    return packed ? 2 * (tokens / segment + 1) : sequences * segments_of(tokens, segment);
+}
+
+__device__ __forceinline__ int64_t segment_state(const AttentionArgs &a, int64_t sequence, int64_t sequence_begin, int64_t index)
+{
+    if (a.offsets != nullptr) return 2 * (sequence_begin / a.segment + index) + (index == 0);
+    return sequence * segments_of(a.tokens, a.segment) + index;
+}
 
 // Rows [*begin, *end) of a packed sequence.  Offsets that decrease or leave the arrays are cut back (and reported): no access
 // ever leaves the rows.
@@ -145,8 +159,8 @@ __device__ __forceinline__ void scan_two(int64_t &x, int64_t &y, int64_t &total_
 }
 
 // Item `launched` of the list of all sequences' segments.  Packed sequences put their whole segments in front and their (shorter) last
-// ones behind, so that the long work starts first; states are kept under the natural number, s.item.  Every thread of the CTA (at most
-// 1024, whole warps) calls it and gets the same answer; holds CTA barriers.
+// ones behind, so that the long work starts first.  Every thread of the CTA (at most 1024, whole warps) calls it and gets the same
+// answer; holds CTA barriers.
 __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t launched, bool reverse)
 {
     SegmentItem s;
@@ -156,13 +170,12 @@ __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t
         const int64_t each = segments_of(a.tokens, a.segment);
         s.sequence = launched / each;
         index = launched - s.sequence * each;
-        s.item = launched;
         s.sequence_begin = 0;
         s.sequence_end = a.tokens;
     }
     else
     {
-        __shared__ int64_t found[5], sums[32][2];
+        __shared__ int64_t found[4], sums[32][2];
         if (threadIdx.x == 0) found[0] = -1;
         // the number of whole segments of all sequences
         int64_t all = 0;
@@ -174,44 +187,39 @@ __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t
         }
         int64_t none = 0, whole, nothing;
         scan_two(all, none, whole, nothing, sums);
-        int64_t before = 0, before_whole = 0;
+        int64_t before_last = 0, before_whole = 0;
         for (int64_t base = 0; base < a.sequences; base += blockDim.x)
         {
             const int64_t n = base + threadIdx.x;
-            int64_t b = 0, e = 0, start = 0, start_whole = 0;
+            int64_t b = 0, e = 0, mine_last = 0, mine_whole = 0;
             if (n < a.sequences)
             {
                 packed_range(a, n, &b, &e);
-                start = segments_of(e - b, a.segment);
-                start_whole = (e - b) / a.segment;
+                mine_whole = (e - b) / a.segment;
+                mine_last = segments_of(e - b, a.segment) - mine_whole;
             }
-            const int64_t mine = start, mine_whole = start_whole;
-            int64_t total, total_whole;
-            scan_two(start, start_whole, total, total_whole, sums);
-            start += before;
+            int64_t start_last = mine_last, start_whole = mine_whole, total_last, total_whole;
+            scan_two(start_last, start_whole, total_last, total_whole, sums);
+            start_last += before_last;
             start_whole += before_whole;
-            const int64_t start_last = start - start_whole;      // last segments in front of this sequence's: whole ones do not count
             int64_t which = -1;
             if (launched < whole && launched >= start_whole && launched < start_whole + mine_whole) which = launched - start_whole;
-            if (launched >= whole && mine > mine_whole && launched - whole == start_last) which = mine_whole;
+            if (launched >= whole && mine_last > 0 && launched - whole == start_last) which = mine_whole;
             if (which >= 0)
             {
                 found[0] = n;
-                found[1] = start + which;
-                found[2] = b;
-                found[3] = e;
-                found[4] = which;
+                found[1] = b;
+                found[2] = e;
+                found[3] = which;
             }
-            before += total;
+            before_last += total_last;
             before_whole += total_whole;
         }
         __syncthreads();
         s.sequence = found[0];
-        s.item = found[1];
-        if (s.sequence >= 0 && s.item >= a.items) s.sequence = -1;       // only with offsets that decrease: more segments than rows allow
-        s.sequence_begin = found[2];
-        s.sequence_end = found[3];
-        index = found[4];
+        s.sequence_begin = found[1];
+        s.sequence_end = found[2];
+        index = found[3];
     }
     if (s.sequence < 0) return s;
     s.state = state_of(a.slots, s.sequence, a.state_count, a.bad_index);
@@ -221,6 +229,7 @@ __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t
         return s;
     }
     const int64_t count = segments_of(s.sequence_end - s.sequence_begin, a.segment);
+    s.segment_state = segment_state(a, s.sequence, s.sequence_begin, index);
     s.begin = s.sequence_begin + index * a.segment;
     s.end = s.begin + a.segment < s.sequence_end ? s.begin + a.segment : s.sequence_end;
     s.first = reverse ? index == count - 1 : index == 0;

@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         {
             const float *from = nullptr;
             int turned = 0;
-            if (cut) from = static_cast<const float *>(p.segment_states) + (item.item * a.heads + head) * size;
+            if (cut) from = static_cast<const float *>(p.segment_states) + (item.segment_state * a.heads + head) * size;
             else if (p.initial != nullptr)
             {
                 from = static_cast<const float *>(p.initial) + (item.state * a.heads + head) * size;
@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(StateLayout<NQ, NV, IN>::kBlock, 1) attention_
         if (!ok && lane == 0) *a.wait_flag = 1;
         tmem_fence_after_sync();
         add(chunks - 1);
-        float *to = static_cast<float *>(p.segment_states) + (item.item * a.heads + head) * (static_cast<int64_t>(p.dq) * p.dv);
+        float *to = static_cast<float *>(p.segment_states) + (item.segment_state * a.heads + head) * (static_cast<int64_t>(p.dq) * p.dv);
 #pragma unroll
         for (int j = 0; j < NQ * 16; ++j)
             if (b < p.dv && d0 + j < p.dq) to[(d0 + j) * p.dv + b] = j % 2 ? second_of(sum[j / 2]) : first_of(sum[j / 2]);

@@ -173,6 +173,7 @@ def linear_attention(out, q, k, v, log_decay, scale=1.0, offsets=None, initial_s
     sequence n in the rows offsets[n] .. offsets[n+1]-1.  k and v may have fewer heads (a divisor of q's).  States are
     [sequences, heads, dk, dv]; with ``slots`` (int32 per sequence, negative: not there) [any number, heads, dk, dv].  ``final_state`` may be
     ``initial_state``.  ``scratch``: any contiguous array of :func:`linear_attention_scratch_bytes` bytes."""
+    scale = float(scale)
     key = (0, scale, _form(q), _form(k), _form(v), _form(out), _form(log_decay), _form(offsets), _form(initial_state), _form(final_state), _form(slots))
     plan = _known(key)
     if plan is None:
@@ -194,6 +195,7 @@ def linear_attention_step(out, state_out, q, k, v, log_decay, state_in, scale=1.
 
     q, k [requests, heads, dk], v, out [requests, heads, dv]; states [requests, heads, dk, dv], or with ``slots`` (int32 per request,
     negative: not there) [any number, heads, dk, dv].  ``state_out`` may be ``state_in``."""
+    scale = float(scale)
     key = (1, scale, _form(q), _form(k), _form(v), _form(out), _form(log_decay), _form(state_in), _form(state_out), _form(slots))
     plan = _known(key)
     if plan is None:
@@ -224,6 +226,7 @@ def linear_attention_backward(dq, dk, dv, dout, q, k, v, log_decay, scale=1.0, o
                               d_initial_state=None, scratch=None, stream=None):
     """Gradients of :func:`linear_attention` for ``dout`` (and ``d_final_state``) with respect to q, k, v (and the initial state).  The
     decays are constants of the layer and get none.  Shapes as there; states [sequences, heads, dk, dv]."""
+    scale = float(scale)
     key = (2, scale, _form(q), _form(k), _form(v), _form(dout), _form(dq), _form(dk), _form(dv), _form(log_decay), _form(offsets), _form(initial_state),
            _form(d_final_state), _form(d_initial_state))
     plan = _known(key)

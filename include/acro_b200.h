@@ -394,7 +394,8 @@ int acro_b200_halo_destroy(acro_b200_halo *halo);
  * Element types: 64, 32 and 16 bits.  Sums, states, decays and row statistics are in 32 bits (64 for ACRO_B200_F64): the
  * "type of sums" below.  All pointers are device memory of the current device; memory of another device is refused.
  * Entries of index arrays are read on the device only: one that is out of range or repeated is skipped, nothing outside the
- * arrays is touched, and acro_b200_device_status() reports ACRO_B200_EINVAL.
+ * arrays is touched, and acro_b200_device_status() reports ACRO_B200_EINVAL.  Calls may be captured into a CUDA graph; the first one on
+ * each device belongs before the first capture.  Arrays start on a boundary of their elements.
  */
 #define ACRO_B200_F64 0
 #define ACRO_B200_F32 1
@@ -425,15 +426,17 @@ typedef struct acro_b200_linear_attention_desc
  *     S_t = lam S_(t-1) + k_t v_t^T,     out_t = scale q_t^T S_t,
  * a Gram form that forgets, chained with a product.  Computed in chunks of tokens (the tokens of a chunk against one another,
  * the earlier ones through the state), long sequences cut into segments when there are few heads.
- *   log_decay      q_heads values of the type of sums; 0 never forgets, -infinity keeps the token itself only
+ *   log_decay      q_heads values of the type of sums; 0 never forgets, -infinity keeps the token itself only; above 0 a state grows
+ *                  with its length and may overflow
  *   offsets        NULL, or sequences + 1 ascending row numbers: sequence n has the rows offsets[n] .. offsets[n+1]-1.  Rows that belong
- *                  to no sequence are neither read nor written.  A sequence may be empty: its final state is its initial state.
+ *                  to no sequence have no effect and are not written.  A sequence may be empty: its final state is its initial state.
  *   initial_state  NULL (zero), or states [state_count][q_heads][dk][dv], contiguous; final_state NULL or the same, and may be the same memory
  *   slots          NULL (state n belongs to sequence n, state_count = sequences), or the state of each sequence.  A negative slot marks
  *                  a sequence that is not there: its rows and states are left as they were.
  *   scratch        acro_b200_linear_attention_scratch_bytes(desc, packed) bytes (0 is possible), 16-byte aligned; calls that share
  *                  it must not overlap on the device.
- * out must not be q, k or v.  No host synchronisation; may be captured.
+ * out must not be q, k or v.  No host synchronisation.  An infinity or NaN of a token reaches only the rows that see it by the
+ * formula; an infinity of v may become a NaN there, in its column.  Same bits on every run on one device.
  */
 size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed);
 int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -441,7 +444,7 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
                                const void *initial_state, void *final_state, const int32_t *slots, int64_t state_count, void *scratch, size_t scratch_bytes,
                                void *stream);
 /* One token of each of desc->sequences requests (desc->tokens = 1): state_out[slot] = lam state_in[slot] + k v^T,
- * out = scale q^T state_out[slot].  state_out may be state_in.  Request n is sequence n of the arrays. */
+ * out = scale q^T state_out[slot].  state_out may be state_in; out must not be q, k or v.  Request n is sequence n of the arrays. */
 int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
                                     const acro_b200_token_array *v, const acro_b200_token_array *out, const void *log_decay, const void *state_in,
                                     void *state_out, const int32_t *slots, int64_t state_count, void *stream);

@@ -99,6 +99,52 @@ def test_scratch_grows_with_segments_and_shared_heads():
         ab.linear_attention(b["out"], b["q"], b["k"], b["v"], b["g"])                        # no scratch given
 
 
+def test_scratch_does_not_grow_with_the_number_of_packed_sequences():
+    few, many = torch.zeros(3, dtype=torch.int64), torch.zeros(5001, dtype=torch.int64)
+    for dtype in (torch.bfloat16, torch.float32, torch.float64):
+        a = arrays(lead=(65536,), heads=2, kv=2, dtype=dtype)
+        for bytes_of in (ab.linear_attention_scratch_bytes, ab.linear_attention_backward_scratch_bytes):
+            assert 0 < bytes_of(a["q"], a["k"], a["v"], many) == bytes_of(a["q"], a["k"], a["v"], few)
+
+
+def test_sizes_that_no_memory_holds_are_refused():
+    """Sizes whose scratch would pass 64 bits: an error, not a small scratch."""
+    for sequences, tokens, packed in ((1, 2 ** 62, 0), (2 ** 62, 1, 1), (2 ** 40, 2 ** 40, 0), (3, 2 ** 39, 1)):
+        desc = LinearAttentionDesc(type=1, q_heads=4, kv_heads=2, dk=8, dv=16, sequences=sequences, tokens=tokens, scale=1.0)
+        assert lib().acro_b200_linear_attention_scratch_bytes(desc, packed) == 0
+        assert lib().acro_b200_linear_attention(desc, *[None] * 4, None, None, None, None, None, sequences, None, 0, None) == _lib.EINVAL
+        assert b"2^40 rows" in lib().acro_b200_last_error()
+
+
+def between_elements(call, count):
+    """Addresses (never followed: this memory is no device's) of which one at a time is off its elements by a byte."""
+    for bad in range(count):
+        at = [4096 * (i + 1) + (i == bad) for i in range(count)]
+        assert call(at) == _lib.EINVAL and b"aligned to its elements" in lib().acro_b200_last_error(), bad
+
+
+def test_pointers_between_elements_are_refused():
+    """They would fault on the device."""
+    desc = LinearAttentionDesc(type=2, q_heads=1, kv_heads=1, dk=16, dv=16, sequences=1, tokens=1, scale=1.0)
+    rows = lambda at: [_lib.TokenArray(a, 16, 16, 16) for a in at]
+    between_elements(lambda at: lib().acro_b200_linear_attention(desc, *rows(at[:4]), *at[4:9], 1, None, 0, None), 9)
+    between_elements(lambda at: lib().acro_b200_linear_attention_step(desc, *rows(at[:4]), *at[4:8], 1, None), 8)
+    between_elements(lambda at: lib().acro_b200_linear_attention_backward(desc, *rows(at[:4]), *at[4:8], *rows(at[8:11]), at[11], None, 0, None), 12)
+    between_elements(lambda at: lib().acro_b200_layer_norm(2, at[0], 8, at[1], at[2], at[3], 8, at[4], at[5], 3, 8, 1e-5, None), 6)
+    between_elements(lambda at: lib().acro_b200_layer_norm_backward(2, at[0], 8, at[1], 8, *at[2:6], 8, at[6], at[7], 3, 8, None, 0, None), 8)
+
+
+def test_two_results_in_one_place_are_refused():
+    """And a step's result in the place of an operand that other heads still read.  (Addresses that are never followed.)"""
+    desc = LinearAttentionDesc(type=2, q_heads=1, kv_heads=1, dk=16, dv=16, sequences=1, tokens=1, scale=1.0)
+    rows = [_lib.TokenArray(4096 * (i + 1), 16, 16, 16) for i in range(4)]
+    for operand in rows[:3]:
+        assert lib().acro_b200_linear_attention_step(desc, *rows[:3], operand, *[1 << 20] * 3, None, 1, None) == _lib.EINVAL
+    at = [4096 * (i + 1) for i in range(6)]
+    assert lib().acro_b200_layer_norm_backward(2, at[0], 8, at[1], 8, *at[2:6], 8, 1 << 20, 1 << 20, 3, 8, None, 0, None) == _lib.EINVAL
+    assert b"same place" in lib().acro_b200_last_error()
+
+
 @pytest.mark.parametrize("kw", [
     {"weight": torch.zeros(7)}, {"weight": torch.zeros(8, dtype=torch.float64)}, {"bias": torch.zeros(16)[::2]}, {"mean": torch.zeros(2)},
     {"mean": torch.zeros(3, dtype=torch.float64)}, {"out": torch.zeros(3, 7)}, {"out": torch.zeros(3, 8, dtype=torch.float16)}, {"eps": -1.0},

@@ -541,6 +541,27 @@ def test_more_sequences_than_threads(kind):
     status_ok()
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32", "f64"])
+def test_many_sequences_are_cut(kind):
+    """Packed sequences that are all longer than a segment, or end anywhere inside one, with short ones between them."""
+    lengths = [513, 1, 1025, 0, 700, 512, 1537, 3, 1024, 640, 0, 129, 2049, 511, 515, 520, 1400, 64, 999, 1281]
+    p = Problem(kind, lengths, True, 1, 1, 16, 16, decay=[-1 / 300])
+    p.check_forward(*p.forward())
+    p.check_backward(*p.backward())
+    status_ok()
+
+
+def test_a_scale_that_changes_in_place():
+    """A scale given as an array is taken at its value of each call."""
+    p = Problem("f32", [9], False, 1, 1, 16, 16)
+    scale, outs = torch.tensor(1.0), []
+    for value in (1.0, 2.0):
+        scale.fill_(value)
+        outs.append(p.blank(1, 16))
+        ab.linear_attention(outs[-1], p.q, p.k, p.v, p.g, scale=scale, initial_state=p.initial, stream=stream())
+    assert torch.equal(outs[1], 2 * outs[0])
+
+
 def test_offsets_beyond_31_bits():
     """A cache of more than 2^31 entries, and arrays of more than 2^31 elements of which one sequence at the end is used."""
     count, d = 140000, 128
