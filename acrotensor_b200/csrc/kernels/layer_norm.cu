@@ -5,11 +5,15 @@
 //
 // Both are bound by HBM: 2 and 3 elements moved per entry against about ten operations.  So a row is read once, stays in
 // registers between its moments and its result, and leaves once.  A row belongs to a group of G threads (a power of two up to a warp,
-// or whole warps); a CTA holds several groups when rows are short.  Groups walk over rows and load the next row's
-// bytes before they work on one.  Elements are worked on in pairs, with weight and bias in registers, and a group has a barrier of its
-// own: a row per CTA of 512 threads, element by element, stood at 34 % of the copy rate in bf16 (24 instructions an element).  A ring
-// of rows in shared memory (asynchronous copies, 2 to 4 rows ahead) was slower in every shape but one.  The variance is the mean square of the centred entries (a second walk over the registers), not a
-// difference of moments, which cancels for rows far from zero.
+// or whole warps); a CTA holds several groups when rows are short.  Groups walk over rows and load the next row's bytes before
+// they work on one.  Elements are worked on in pairs, with weight and bias in registers, and a group has a barrier of its own.
+// The variance is the mean square of the centred entries (a second walk over the registers), not a difference of moments, which
+// cancels for rows far from zero.
+//
+// 16384 x 4096 in fp32: 91 us, gradient 151 us (90 and 81 % of the measured copy rate).  In bf16 52 and 93 us (79 and 66 %; a copy of these
+// arrays takes 44 us, a sum of two of them 60): half the bytes for the same instructions, so that issue (55 to 60 % of its slots) and
+// the barriers' latency count, with 16 warps an SM for want of registers.  More rows on their way did not help: two or three rows
+// ahead in registers 67 and 83 us, a ring of four in shared memory (bulk copies) 68 and 95 us.
 //
 // The gradient's column sums run over all rows: a thread owns the same columns of every row that its group takes, so the sums over
 // those rows stay in its registers (in shared memory beyond 16 columns a thread); the groups of a CTA are added in ascending order, a CTA
@@ -51,25 +55,39 @@ __device__ __forceinline__ void group_sum(A (&v)[N], A *slot, int group)
     }
     const int warps = group / 32;
     if (warps <= 1) return;
-    const int warp = (threadIdx.x % group) / 32;
+    struct alignas(N * sizeof(A)) All { A v[N]; };
+    All *all = reinterpret_cast<All *>(slot);
     if (threadIdx.x % 32 == 0)
     {
+        All &mine = all[threadIdx.x % group / 32];
 #pragma unroll
-        for (int i = 0; i < N; ++i) slot[warp * N + i] = v[i];
+        for (int i = 0; i < N; ++i) mine.v[i] = v[i];
     }
+    // the group's own barrier
     asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / group), "r"(group) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0;
+#pragma unroll 4
     for (int k = 0; k < warps; ++k)
     {
+        const All other = all[k];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += slot[k * N + i];
+        for (int i = 0; i < N; ++i) v[i] += other.v[i];
     }
 }
 
-// THREADS: the largest CTA (256 when rows are short enough: twice the registers a thread).
+// 1 / sqrt(v).  In 32 bits the function's two steps of error less a Newton step: a third of the instructions of a root and a quotient.
+__device__ __forceinline__ double inverse_root(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ float inverse_root(float v)
+{
+    const float r = rsqrtf(v), left = fmaf(-v * r, r, 1.0f);
+    return left == left ? fmaf(0.5f * r, left, r) : r;       // zero and infinity have no step
+}
+
+// THREADS: the largest CTA (256 when rows are short enough: twice the registers a thread, and two CTAs an SM.  Left to itself the compiler took
+// 152 registers in bf16 and one CTA: 66 us instead of 52 for 16384 x 4096; fp64 needs them).
 template <class T, int VEC, int COLS, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_kernel(NormArgs a)
+__global__ void __launch_bounds__(THREADS, sizeof(T) < 8 ? 512 / THREADS : 1) norm_kernel(NormArgs a)
 {
     using A = typename Element<T>::Acc;
     using P = typename PairOf<A>::type;
@@ -82,8 +100,13 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(NormArgs a)
     int64_t base = static_cast<int64_t>(blockIdx.x) * groups;
     // the thread's columns of weight and bias stay in registers (one and zero where there are none)
     Row next, weight, bias;
+    const A eps = static_cast<A>(a.eps);
+    const T *from = static_cast<const T *>(a.x) + (base + mine) * a.x_stride;
+    T *to = static_cast<T *>(a.y) + (base + mine) * a.y_stride;
+    const int64_t from_step = step * a.x_stride, to_step = step * a.y_stride;
     const auto fetch = [&](int64_t row) {
-        if (row < a.rows) next.load(static_cast<const T *>(a.x) + row * a.x_stride, lane, a.group, width);
+        if (row < a.rows) next.load(from, lane, a.group, width);
+        from += from_step;
     };
     fetch(base + mine);
     if (a.w != nullptr) weight.load(static_cast<const T *>(a.w), lane, a.group, width);
@@ -110,15 +133,17 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(NormArgs a)
 #pragma unroll
         for (int k = 0; k < COLS / 2; ++k)
         {
-            const bool one = Row::column(k, 0, lane, a.group) < width, other = Row::column(k, 1, lane, a.group) < width;
+            // columns behind the width weigh nothing; a pack lies before the width or behind it
+            if (Row::column(k, 0, lane, a.group) >= width) continue;
             x[k] = sub2(x[k], means);
-            if (VEC == 1 && !other) x[k] = two(first_of(x[k]), A(0));
-            if (!one) x[k] = two(A(0), A(0));
+            if (VEC == 1 && Row::column(k, 1, lane, a.group) >= width) x[k] = two(first_of(x[k]), A(0));
             sum = fma2(x[k], x[k], sum);
         }
         s[0] = first_of(sum) + second_of(sum);
         group_sum(s, slots[1] + slot, a.group);
-        const A rstd = A(1) / sqrt(s[0] * inv + static_cast<A>(a.eps));
+        const A rstd = inverse_root(s[0] * inv + eps);
+        T *out_row = to;
+        to += to_step;
         if (!there) continue;
         if (lane == 0)
         {
@@ -129,7 +154,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(NormArgs a)
         Row out;
 #pragma unroll
         for (int k = 0; k < COLS / 2; ++k) out.pair[k] = narrow2<T>(fma2(mul2(x[k], scale), widen2<T>(weight.pair[k]), widen2<T>(bias.pair[k])));
-        out.store(static_cast<T *>(a.y) + row * a.y_stride, lane, a.group, width);
+        out.store(out_row, lane, a.group, width);
     }
 }
 
@@ -153,7 +178,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_kernel(NormArgs a)
         s[0] += d * d;
     }
     group_sum(s, slots[1], kWideThreads);
-    const A rstd = A(1) / sqrt(s[0] * inv + static_cast<A>(a.eps));
+    const A rstd = inverse_root(s[0] * inv + static_cast<A>(a.eps));
     if (threadIdx.x == 0)
     {
         if (a.mean != nullptr) static_cast<A *>(a.mean)[row] = mean;
@@ -172,16 +197,16 @@ __global__ void __launch_bounds__(kWideThreads) norm_wide_kernel(NormArgs a)
 // Up to 16 columns a thread the column sums are registers; beyond that each thread keeps its own in shared memory (sums[2][width],
 // touched by their owner alone until the end).
 template <class T, int VEC, int COLS, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_gradient_kernel(NormArgs a)
+__global__ void __launch_bounds__(THREADS, sizeof(T) < 8 ? 512 / THREADS : 1) norm_gradient_kernel(NormArgs a)
 {
     using A = typename Element<T>::Acc;
     using P = typename PairOf<A>::type;
     using Row = RowPart<T, VEC, COLS>;
     constexpr bool kRegisters = COLS <= 16;
     constexpr int kSums = kRegisters ? COLS / 2 : 1;
-    __shared__ A slots[2][2 * THREADS / 32];
+    __shared__ __align__(16) A slots[2][2 * THREADS / 32];
     extern __shared__ __align__(16) unsigned char dynamic[];
-    // pair k of thread t at entry k * threads + t (dw, then db), or [2][width] when groups are added up
+    // pair k of thread t at entry k * threads + t (dw, then db), or [groups][2][width] when groups are added up
     P *own = reinterpret_cast<P *>(dynamic);
     A *sums = reinterpret_cast<A *>(own);
     const int groups = blockDim.x / a.group, mine = threadIdx.x / a.group, lane = threadIdx.x % a.group, width = static_cast<int>(a.width);
@@ -200,10 +225,16 @@ __global__ void __launch_bounds__(THREADS) norm_gradient_kernel(NormArgs a)
     int64_t base = static_cast<int64_t>(blockIdx.x) * groups;
     Row next_x, next_g, weight;
     A next_mean = 0, next_rstd = 0;
+    // pointers that walk along, where registers are left for them (4999 x 1001 in fp32: 19 us, 23 with products; 4096 x 16384 in bf16: 159 and 147)
+    const T *x_from = static_cast<const T *>(a.x) + (base + mine) * a.x_stride, *g_from = static_cast<const T *>(a.dy) + (base + mine) * a.dy_stride;
+    T *to = static_cast<T *>(a.y) + (base + mine) * a.y_stride;
+    const int64_t x_step = step * a.x_stride, g_step = step * a.dy_stride, to_step = step * a.y_stride;
     const auto fetch = [&](int64_t row) {
         if (row >= a.rows) return;
-        next_x.load(static_cast<const T *>(a.x) + row * a.x_stride, lane, a.group, width);
-        next_g.load(static_cast<const T *>(a.dy) + row * a.dy_stride, lane, a.group, width);
+        next_x.load(kRegisters ? x_from : static_cast<const T *>(a.x) + row * a.x_stride, lane, a.group, width);
+        next_g.load(kRegisters ? g_from : static_cast<const T *>(a.dy) + row * a.dy_stride, lane, a.group, width);
+        x_from += x_step;
+        g_from += g_step;
         next_mean = static_cast<const A *>(a.mean)[row];
         next_rstd = static_cast<const A *>(a.rstd)[row];
     };
@@ -251,7 +282,8 @@ __global__ void __launch_bounds__(THREADS) norm_gradient_kernel(NormArgs a)
             Row out;
 #pragma unroll
             for (int k = 0; k < COLS / 2; ++k) out.pair[k] = narrow2<T>(mul2(scale, fma2(x[k], mean_gx, sub2(g[k], mean_g))));
-            out.store(static_cast<T *>(a.y) + row * a.y_stride, lane, a.group, width);
+            out.store(kRegisters ? to : static_cast<T *>(a.y) + row * a.y_stride, lane, a.group, width);
+            to += to_step;
         }
     }
     if (a.partial == nullptr) return;
@@ -274,28 +306,27 @@ __global__ void __launch_bounds__(THREADS) norm_gradient_kernel(NormArgs a)
     }
     else
     {
-        // the groups' sums, one group after the other
-        for (int one = 0; one < groups; ++one)
-        {
-            if (mine == one)
+        // the groups' sums in ascending order
+        A *to = groups == 1 ? out : sums + static_cast<size_t>(mine) * 2 * width;
+#pragma unroll
+        for (int k = 0; k < kSums; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
             {
-                A *to = groups == 1 ? out : sums;
-#pragma unroll
-                for (int k = 0; k < kSums; ++k)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                    {
-                        const int c = Row::column(k, e, lane, a.group);
-                        if (c >= width) continue;
-                        const A w = e ? second_of(dw[k]) : first_of(dw[k]), b = e ? second_of(db[k]) : first_of(db[k]);
-                        to[c] = one == 0 ? w : to[c] + w;
-                        to[width + c] = one == 0 ? b : to[width + c] + b;
-                    }
+                const int c = Row::column(k, e, lane, a.group);
+                if (c >= width) continue;
+                to[c] = e ? second_of(dw[k]) : first_of(dw[k]);
+                to[width + c] = e ? second_of(db[k]) : first_of(db[k]);
             }
-            __syncthreads();
+        if (groups == 1) return;
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * width; c += blockDim.x)
+        {
+            A s = sums[c];
+#pragma unroll 4
+            for (int one = 1; one < groups; ++one) s += sums[one * 2 * width + c];
+            out[c] = s;
         }
-        if (groups > 1)
-            for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) out[c] = sums[c];
     }
 }
 
@@ -303,7 +334,7 @@ template <class T>
 __global__ void __launch_bounds__(kWideThreads) norm_gradient_wide_kernel(NormArgs a)
 {
     using A = typename Element<T>::Acc;
-    __shared__ A slot[2 * kWideThreads / 32];
+    __shared__ __align__(16) A slot[2 * kWideThreads / 32];
     const int64_t row = blockIdx.x;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride, *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
     const A inv = A(1) / static_cast<A>(a.width), mean = static_cast<const A *>(a.mean)[row], rstd = static_cast<const A *>(a.rstd)[row];
@@ -376,7 +407,7 @@ int sms() { return sm_count() > 0 ? sm_count() : 148; }
 
 // Columns a thread: as many as give it 64 bytes of a row (the gradient, which reads two rows: 32), at least 8, as long as the threads
 // then still fill the GPU; fewer for few rows, down to 8; more when 512 threads would not cover the row.  (16384 x 4096 in bf16, 8 / 16 / 32
-// columns: forward 99 / 68 / 58 us, gradient 126 / 93 us; in fp32 the gradient takes 157 / 168 us with 8 / 16.)
+// columns: forward 119 / 64 / 52 us, gradient 117 / 93 us with 8 / 16; forward in fp32 130 / 91 us with 8 / 16.)
 Shape norm_shape(int type, int64_t rows, int64_t width, bool vectors, bool gradient)
 {
     Shape s;
@@ -430,7 +461,7 @@ int launch(const Shape &s, const NormArgs &a, bool gradient, cudaStream_t stream
     if constexpr (COLS <= 16 || THREADS > 256)
     {
         const int smem = COLS > 16 ? COLS * s.threads * 2 * static_cast<int>(sizeof(typename Element<T>::Acc))
-                                   : s.groups() > 1 ? 2 * static_cast<int>(a.width * sizeof(typename Element<T>::Acc)) : 0;
+                                   : s.groups() > 1 ? s.groups() * 2 * static_cast<int>(a.width * sizeof(typename Element<T>::Acc)) : 0;
         cudaError_t status = cudaFuncSetAttribute(norm_gradient_kernel<T, VEC, COLS, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (status != cudaSuccess) return fail_cuda(status, name);
         norm_gradient_kernel<T, VEC, COLS, THREADS><<<gradient_parts(a.rows, s), s.threads, smem, stream>>>(a);
