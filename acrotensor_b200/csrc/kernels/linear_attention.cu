@@ -292,8 +292,9 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
 }
 
 // Turns the segments' own states into the states that they start from: one thread per entry of a state, walking a sequence's
-// segments in the order of time, 16 loads ahead (with the decay's power taken in every step and one load at a time 144 segments of
-// 128 x 128 took 89 us).
+// segments in the order of time, 16 loads ahead.  Bound by the latency of offsets, powers and loads: 19 us with cold caches for 12 segments
+// of 16 heads of 128 x 128 (25 MB).  Taking the powers behind the first loads did not shorten it; with the power taken in every step and
+// one load at a time 144 segments took 89 us.
 template <class A>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttentionArgs a)
 {
@@ -544,22 +545,24 @@ std::string head_fault(const acro_b200_linear_attention_desc *d, bool packed)
 }
 
 // Tokens of a segment.  A cut of the sequences into `wanted` segments each makes the GPU's waves of CTAs shorter, and costs a second
-// walk over k and v (about 0.6 of the main pass on either path) and the join (as long as 6 chunks of 64 tokens): the cheapest number
-// is taken.  `resident`: CTAs an SM holds (tensor-core pass: 1; the other: 2 at least).  Packed sequences are treated as one axis of all
-// their rows, since their lengths are not known here.
+// walk over k and v (0.4 of the main pass on the tensor cores, 0.6 on the other path) and the join (as long as 6 chunks of 64 tokens): the cheapest number
+// is taken, for the CTAs that an SM holds (tensor-core pass: 1; the other: 2 at least).  Packed sequences are treated as one axis of all
+// their rows, since their lengths are not known here; segments of three quarters of that length cost the same over 15 packed shapes, half
+// the length 14 % more.  On the tensor cores a segment has 256 tokens at least: 13 shapes took 101 us on average with 512, 87 with 256 (4 x 1024
+// tokens of 12 heads in fp32 96 and 81 us), 86 with 128 but one of them 14 % more than before.
 int64_t segment_tokens(const acro_b200_linear_attention_desc &d, bool packed, bool tensor_cores, int passes)
 {
     const int64_t slots = (sm_count() > 0 ? sm_count() : 148) * (tensor_cores ? 1 : 2);
     const int64_t whole = std::max<int64_t>(1, (d.tokens + kSegmentQuantum - 1) / kSegmentQuantum) * kSegmentQuantum;
     const int64_t pairs = (packed ? 1 : std::max<int64_t>(1, d.sequences)) * d.q_heads * passes;
-    const int64_t shortest = kSegmentQuantum * (tensor_cores ? 4 : 1);
+    const int64_t shortest = kSegmentQuantum * (tensor_cores ? 2 : 1);
     int64_t best = whole;
     double cost = static_cast<double>((pairs + slots - 1) / slots) * whole;
     for (int64_t wanted = 2; wanted <= slots / pairs + 1 && whole / wanted >= shortest; ++wanted)
     {
         const int64_t segment = ((d.tokens + wanted - 1) / wanted + kSegmentQuantum - 1) / kSegmentQuantum * kSegmentQuantum;
         const int64_t each = (d.tokens + segment - 1) / segment;
-        const double c = 1.6 * static_cast<double>((pairs * each + slots - 1) / slots) * segment + 6 * 64;
+        const double c = (tensor_cores ? 1.4 : 1.6) * static_cast<double>((pairs * each + slots - 1) / slots) * segment + 6 * 64;
         if (c < cost)
         {
             cost = c;
