@@ -10,15 +10,16 @@
 // columns, and becomes an A operand by a store into tensor memory, without a way through shared memory.
 //
 // Precision: accumulators and the state are fp32; every operand is a sum of bf16 parts (8 bits each).  Inputs: IN parts, 1 for bf16, 2 for
-// fp16 (exact) and 3 for fp32 (2^-26).  P~ and S: 2 parts (an error of 2^-18 of an entry, 2^-9 of what the rounding of a bf16 result
-// loses), 3 for fp32.  K~: 3 parts, because the final state is an fp32 result and collects every chunk's change.  Of the products of
-// parts those that the next smaller part of either operand would outweigh are left out.  The small ones are multiplied first: the tensor
-// cores' additions lose up to a step of the sum so far, so fewer of them happen at its full size; and no sum of theirs spans more
+// fp16 (exact) and 3 for fp32 (2^-26).  P~, S and K~: 3 parts whatever the inputs, so that scores and states have on their way into a product
+// the bits that they have in fp32 (with two parts of P~ and S, 2^-18, a few bf16 results in ten thousand were rounded the other way; a chunk of
+// 128 columns took 2.75 us where it takes 3.08 with three, of 64 columns 1.71 and 2.09).  Of the products of parts those are left out that lie
+// below 2^-24 of the whole.  The small ones are multiplied first: the tensor cores' additions lose up to a step of the sum so far, so fewer
+// of them happen at its full size; and no sum of theirs spans more
 // than a chunk (spanning a segment of 58 cost the final state a digit).
 //
-// Bound, for bf16 and 128 columns: by HBM 128 KB a chunk, about 2850 cycles of an SM at its share of 6.5 TB/s.  Shared memory comes first:
-// the products' operands take 2050 cycles of it (48 cycles for 64 columns with both operands there, measured alone), copies, K~, P~ and
-// stores 2100, of the 4750 cycles (2.64 us) that a chunk takes with all SMs at work.  64 columns: 1.76 us a chunk.  The roles overlap: one
+// Bound, for bf16 and 128 columns: by HBM 64 KB a chunk, about 2850 cycles of an SM at its share of 6.5 TB/s.  Shared memory comes first:
+// the products' operands take about 2370 cycles of it (48 cycles for 64 columns with both operands there, measured alone), copies, K~, P~ and
+// stores 2170, of the 5500 cycles (3.08 us) that a chunk takes with all SMs at work.  64 columns: 2.09 us a chunk.  The roles overlap: one
 // warp issues copies and products, eight convert operands, sixteen keep the state and write; waiting warps sleep on barriers, one arrival
 // a warp; loops are short (the instruction cache held the first versions back).
 #ifndef ACRO_B200_KERNELS_LINEAR_ATTENTION_MMA_CUH
@@ -57,7 +58,7 @@ struct Maps
 template <int NQ, int NV, int IN>
 struct Layout
 {
-    static constexpr int kParts = IN == 3 ? 3 : 2;              // of P~ and S
+    static constexpr int kParts = 3;                            // of P~ and S
     static constexpr int kQ = 0, kK = IN * NQ * kBox, kV = 2 * IN * NQ * kBox, kStage = IN * (2 * NQ + NV) * kBox;
     static constexpr int kFits = (kSmem - (3 * NQ + kParts) * kBox - 4096) / kStage;
     static constexpr int kStages = kFits < (NQ == 2 ? 3 : 4) ? kFits : NQ == 2 ? 3 : 4;
@@ -104,15 +105,20 @@ __device__ __forceinline__ void warp_arrive(uint64_t *bar)
 
 __device__ __forceinline__ bool all_wait(uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_asleep(bar, parity)); }
 
-// What a part of a product starts from: the pairs (part i of A, part j of B) with i + j < N, the small ones first.
-template <int PA, int PB, int N, class F>
+// The products of parts of A and B: the pairs (part i of A, part j of B) with i + j < 3, the small ones first.  `later`: not the first pair.
+template <int PA, int PB, class F>
 __device__ __forceinline__ void for_pairs(F &&issue)
 {
+    bool later = false;
 #pragma unroll
-    for (int sum = N - 1; sum >= 0; --sum)
+    for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
         for (int i = 0; i <= sum; ++i)
-            if (i < PA && sum - i < PB) issue(i, sum - i);
+            if (i < PA && sum - i < PB)
+            {
+                issue(i, sum - i, later);
+                later = true;
+            }
 }
 
 // Two results to rows `to` and `after` of the output's type.
@@ -231,11 +237,11 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
         const auto issue_scores = [&](int c) {
             const uint32_t stage = base + c % L::kStages * L::kStage;
             const uint64_t q = umma_operand(stage + L::kQ, 16, 1024), k = umma_operand(stage + L::kK, 16, 1024);
-            for_pairs<IN, IN, IN>([&](int x, int y) {
+            for_pairs<IN, IN>([&](int x, int y, bool later) {
 #pragma unroll
                 for (int i = 0; i < NQ * 4; ++i)
                     umma(leader, kScores, q + (x * NQ * kBox + i / 4 * kBox + i % 4 * 32) / 16, k + (y * NQ * kBox + i / 4 * kBox + i % 4 * 32) / 16, by_columns,
-                         x > 0 || y < IN - 1 || i > 0);
+                         later || i > 0);
             });
             umma_commit(leader, &sh.scores);
         };
@@ -254,31 +260,31 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
             ok = (c == 0 || all_wait(&sh.change_free, parity ^ 1)) && all_wait(&sh.ready[c % L::kStages], c / L::kStages & 1);
             if (!ok) break;
             tmem_fence_after_sync();
-            for_pairs<IN, 3, 3>([&](int x, int y) {
+            for_pairs<IN, 3>([&](int x, int y, bool later) {
 #pragma unroll
                 for (int k = 0; k < kChunk / 16; ++k)
-                    umma(leader, kDelta, v + (x * NV * kBox + k * 2048) / 16, scaled + (y * NQ * kBox + k * 2048) / 16, change_shape, x > 0 || y < 2 || k > 0);
+                    umma(leader, kDelta, v + (x * NV * kBox + k * 2048) / 16, scaled + (y * NQ * kBox + k * 2048) / 16, change_shape, later || k > 0);
             });
             umma_commit(leader, &sh.change);
             // the previous chunk's results have been read, and before that its end state was published
             ok = c == 0 ? all_wait(&sh.state, 0) : all_wait(&sh.out_free, parity ^ 1);
             if (!ok) break;
             tmem_fence_after_sync();
-            for_pairs<SP, IN, SP>([&](int x, int y) {
+            for_pairs<SP, IN>([&](int x, int y, bool later) {
 #pragma unroll
                 for (int i = 0; i < NQ * 4; ++i)
                     umma_tmem(leader, kFar, L::kState + x * NQ * 32 + i * 8, q + (y * NQ * kBox + i / 4 * kBox + i % 4 * 32) / 16, by_columns,
-                              (IN == 1 ? x < SP - 1 : x > 0 || y < SP - 1) || i > 0);
+                              later || i > 0);
             });
             // all of the previous chunk's products were waited for by the readers of their results: its stage is free
             if (L::kStages > 1 && loaded < chunks) load(loaded++);
             ok = all_wait(&sh.weights, parity);
             if (!ok) break;
             tmem_fence_after_sync();
-            for_pairs<IN, SP, SP>([&](int x, int y) {
+            for_pairs<IN, SP>([&](int x, int y, bool later) {
 #pragma unroll
                 for (int k = 0; k < kChunk / 16; ++k)
-                    umma(leader, kNear, v + (x * NV * kBox + k * 2048) / 16, weights + (y * kBox + k * 32) / 16, near_shape, x > 0 || y < SP - 1 || k > 0);
+                    umma(leader, kNear, v + (x * NV * kBox + k * 2048) / 16, weights + (y * kBox + k * 32) / 16, near_shape, later || k > 0);
             });
             umma_commit(leader, &sh.out);
             if (L::kStages == 1 && loaded < chunks)
@@ -664,10 +670,10 @@ __global__ void __launch_bounds__(StateLayout<NQ, NV, IN>::kBlock, 1) attention_
             tmem_fence_after_sync();
             const uint64_t v = umma_operand(base + c % L::kStages * L::kStage + L::kV, NV == 2 ? kBox : 0, 1024),
                            k = umma_operand(base + L::kScaled + (c & 1) * L::kParts, kBox, 1024);
-            for_pairs<IN, 3, 3>([&](int x, int y) {
+            for_pairs<IN, 3>([&](int x, int y, bool later) {
 #pragma unroll
                 for (int i = 0; i < kChunk / 16; ++i)
-                    umma(leader, tmem + (c & 1) * NQ * 64, v + (x * NV * kBox + i * 2048) / 16, k + (y * NQ * kBox + i * 2048) / 16, shape, x > 0 || y < 2 || i > 0);
+                    umma(leader, tmem + (c & 1) * NQ * 64, v + (x * NV * kBox + i * 2048) / 16, k + (y * NQ * kBox + i * 2048) / 16, shape, later || i > 0);
             });
             umma_commit(leader, &sh.done[c & 1]);
             if (loaded < chunks)
