@@ -100,6 +100,13 @@ __device__ __forceinline__ uint32_t pack_bf16(Two x)
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(second_of(x)), "f"(first_of(x)));
     return r;
 }
+// The same, but finite values above the largest bf16 (and infinities) become that one: what is left of a finite value is finite.
+__device__ __forceinline__ uint32_t pack_bf16_finite(Two x)
+{
+    uint32_t r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(second_of(x)), "f"(first_of(x)));
+    return r;
+}
 __device__ __forceinline__ Two unpack_bf16(uint32_t x) { return two(x << 16, x & 0xffff0000u); }
 
 // Two neighbouring elements as they lie in memory.

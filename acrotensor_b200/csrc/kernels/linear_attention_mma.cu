@@ -106,7 +106,13 @@ __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_const
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                 {
-                    const uint32_t w = pack_bf16(y[e]);
+                    uint32_t w = pack_bf16(y[e]);
+                    if (__builtin_expect(odd_pair(w), 0))
+                    {
+                        // finite values above the largest bf16 are parts, too
+                        const uint32_t most = pack_bf16_finite(y[e]);
+                        w = (isfinite(first_of(y[e])) ? most & 0xffffu : w & 0xffffu) | (isfinite(second_of(y[e])) ? most & 0xffff0000u : w & 0xffff0000u);
+                    }
                     const Two left = sub2(y[e], unpack_bf16(w));
                     // infinities and NaN are the first part's alone
                     y[e] = two(odd_half(w) ? 0.0f : first_of(left), odd_half(w >> 16) ? 0.0f : second_of(left));

@@ -83,10 +83,11 @@ struct Shared
     uint64_t full[4], ready[4], scores, weights, state, out, out_free, change, change_free, drained;
 };
 
-// The next bf16 part of x: returns it and leaves the remainder.  (Of an infinity the remainder is NaN: sums that meet one are not finite.)
+// The next bf16 part of x: returns it and leaves the remainder.  Parts of fp32 values above the largest bf16 are finite; an infinity stands
+// in the last part (pack_bf16), a NaN in all.
 __device__ __forceinline__ uint32_t take_part(Two &x)
 {
-    const uint32_t part = pack_bf16(x);
+    const uint32_t part = pack_bf16_finite(x);
     x = sub2(x, unpack_bf16(part));
     return part;
 }

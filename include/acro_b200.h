@@ -436,7 +436,8 @@ typedef struct acro_b200_linear_attention_desc
  *   scratch        acro_b200_linear_attention_scratch_bytes(desc, packed) bytes (0 is possible), 16-byte aligned; calls that share
  *                  it must not overlap on the device.
  * out must not be q, k or v.  No host synchronisation.  An infinity or NaN of a token reaches only the rows that see it by the
- * formula; an infinity of v may become a NaN there, in its column.  Same bits on every run on one device.
+ * formula; an infinity of v may become a NaN there, in its column, and one of q or k in 32 and 16 bits a NaN in the rows and the state
+ * that it meets.  Same bits on every run on one device.
  */
 size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed);
 int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,

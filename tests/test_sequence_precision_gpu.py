@@ -103,3 +103,39 @@ def test_single_precision_keeps_its_last_bits(of, d):
     if of == "v":
         v[0, 0], v[0, 1] = x[:, None], -y[:, None]
     near("f32", forward("f32", q, k, v)[1:], (x.double() - y.double())[:, None])
+
+
+@pytest.mark.parametrize("kind,of", [("f32", "q"), ("f32", "k"), ("f32", "v"), ("f32", "state"), ("bf16", "state"), ("f32", "score"), ("bf16", "score")])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_above_the_largest_bf16_stay_finite(kind, of, d):
+    """3.4e38 is an fp32 value beyond the numbers of bf16: as an operand, as a state and as a score.  One term an entry: 16 roundings at most."""
+    most, little = 3.4e38, 2.0 ** -20
+    q, k, v, state = zeros(kind, 1, d), zeros(kind, 1, d), zeros(kind, 1, d), torch.zeros(1, 1, d, d, device="cuda")
+    q[..., 0], k[0, 5, 0, 0], v[0, 5] = 1, 1, 1
+    if of == "q":
+        q[..., 0], v[0, 5] = most, little
+    if of == "k":
+        k[0, 5, 0, 0], v[0, 5] = most, little
+    if of == "v":
+        v[0, 5], k[0, 5, 0, 0] = most, little
+    if of == "state":
+        state[..., 1, :], q[..., 1] = most, little
+    if of == "score":       # (2 - 2^-8) 2^127
+        q[..., 0], q[..., 1] = 1.9921875 * 2.0 ** 64, 2.0 ** 60
+        k[0, 5, 0, 0], k[0, 5, 0, 1], v[0, 5] = 2.0 ** 63, 2.0 ** 59, little
+    exact, _ = ref.attention(*[x[0].double().cpu().numpy() for x in (q, k, v)], torch.zeros(1).numpy(), 1.0, state[0].double().cpu().numpy())
+    exact = torch.as_tensor(exact, device="cuda")
+    got = forward(kind, q, k, v, state)
+    assert bool(((got - exact).abs() <= (ref.HALF_STEP[kind] + 16 * 2.0 ** -24) * exact.abs()).all())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_gradients_of_values_above_the_largest_bf16_stay_finite(d):
+    q, k, v, do = (zeros("f32", 1, d) for _ in range(4))
+    q[0, 7, 0, 0], k[..., 0], do[0, 7] = 1, 2.0 ** -20, 3.4e38
+    dq, dk, dv = (torch.full_like(x, -7.0) for x in (q, k, v))
+    ab.linear_attention_backward(dq, dk, dv, do, q, k, v, torch.zeros(1, device="cuda"), stream=stream(),
+                                 scratch=scratch_for(ab.linear_attention_backward_scratch_bytes(q, k, v)))
+    want = 2.0 ** -20 * float(torch.tensor(3.4e38))
+    assert bool(((dv[0, :8].double() - want).abs() <= 16 * 2.0 ** -24 * want).all()) and bool((dv[0, 8:] == 0).all())
+    assert bool((dq == 0).all()) and bool((dk == 0).all())
