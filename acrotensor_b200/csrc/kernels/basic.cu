@@ -4,6 +4,7 @@
 
 #include <atomic>
 #include <dlfcn.h>
+#include <map>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -68,6 +69,28 @@ std::atomic<unsigned long long> g_context_epoch{0};
 namespace acro_b200_detail
 {
 unsigned long long context_epoch() { return g_context_epoch.load(); }
+
+cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes)
+{
+    // the largest limit set so far, of each kernel on each device; a limit belongs to a CUDA context
+    static std::mutex lock;
+    static std::map<std::pair<const void *, int>, size_t> allowed;
+    static unsigned long long epoch = 0;
+    int dev = -1;
+    cudaError_t status = cudaGetDevice(&dev);
+    if (status != cudaSuccess) return status;
+    std::lock_guard<std::mutex> guard(lock);
+    if (epoch != context_epoch())
+    {
+        allowed.clear();
+        epoch = context_epoch();
+    }
+    size_t &most = allowed[{kernel, dev}];
+    if (bytes <= most) return cudaSuccess;
+    status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (status == cudaSuccess) most = bytes;
+    return status;
+}
 
 int *wait_flag_device_ptr()
 {

@@ -32,6 +32,15 @@ int *bad_index_flag_device_ptr();
 // again when the value has moved on.
 unsigned long long context_epoch();
 
+// Lets `kernel` be launched on the current device with at least `bytes` of dynamic shared memory.  The limit belongs to the kernel, not to
+// a launch, so it is only ever raised: a limit set to one call's own size would be lowered by the call of another host thread between
+// this call's setting and its launch.
+cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes);
+template <class... ARGS> cudaError_t allow_dynamic_smem(void (*kernel)(ARGS...), size_t bytes)
+{
+    return allow_dynamic_smem(reinterpret_cast<const void *>(kernel), bytes);
+}
+
 inline cudaStream_t as_stream(void *s) { return static_cast<cudaStream_t>(s); }
 
 // To be called right after a kernel launch.

@@ -462,7 +462,7 @@ int launch(const Shape &s, const NormArgs &a, bool gradient, cudaStream_t stream
     {
         const int smem = COLS > 16 ? COLS * s.threads * 2 * static_cast<int>(sizeof(typename Element<T>::Acc))
                                    : s.groups() > 1 ? s.groups() * 2 * static_cast<int>(a.width * sizeof(typename Element<T>::Acc)) : 0;
-        cudaError_t status = cudaFuncSetAttribute(norm_gradient_kernel<T, VEC, COLS, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t status = allow_dynamic_smem(norm_gradient_kernel<T, VEC, COLS, THREADS>, smem);
         if (status != cudaSuccess) return fail_cuda(status, name);
         norm_gradient_kernel<T, VEC, COLS, THREADS><<<gradient_parts(a.rows, s), s.threads, smem, stream>>>(a);
     }

@@ -639,7 +639,7 @@ int run_pass_tiled(const AttentionArgs &all, bool states_only, cudaStream_t stre
         slices = std::max(slices, (a.pass[i].dv + SV - 1) / SV);
         smem = std::max(smem, pass_smem_bytes<typename Element<T>::Acc, C, SV>(a.pass[i].dq));
     }
-    cudaError_t status = cudaFuncSetAttribute(attention_pass_kernel<T, C, SV>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(attention_pass_kernel<T, C, SV>, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_linear_attention");
     const int64_t grid = a.items * a.heads * slices;
     if (grid > INT32_MAX) return fail_unsupported("acro_b200_linear_attention: more than 2^31 segments x heads");

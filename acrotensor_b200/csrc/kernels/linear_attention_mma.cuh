@@ -786,7 +786,7 @@ int launch_as(const AttentionArgs &a, const Maps &maps, cudaStream_t stream)
 {
     using L = Layout<NQ, NV, IN>;
     const char *name = "acro_b200_linear_attention";
-    cudaError_t status = cudaFuncSetAttribute(attention_mma_kernel<NQ, NV, IN, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic);
+    cudaError_t status = allow_dynamic_smem(attention_mma_kernel<NQ, NV, IN, OUT>, L::kDynamic);
     if (status != cudaSuccess) return fail_cuda(status, name);
     const dim3 grid(static_cast<unsigned>(a.items * a.heads), a.passes);
     attention_mma_kernel<NQ, NV, IN, OUT><<<grid, kBlock, L::kDynamic, stream>>>(a, maps);
@@ -801,7 +801,7 @@ int launch(const AttentionArgs &a, const Maps &maps, bool states_only, cudaStrea
     {
         using L = StateLayout<NQ, NV, IN>;
         const char *name = "acro_b200_linear_attention";
-        cudaError_t status = cudaFuncSetAttribute(attention_states_kernel<NQ, NV, IN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic);
+        cudaError_t status = allow_dynamic_smem(attention_states_kernel<NQ, NV, IN>, L::kDynamic);
         if (status != cudaSuccess) return fail_cuda(status, name);
         const dim3 grid(static_cast<unsigned>(a.items * a.heads), a.passes);
         attention_states_kernel<NQ, NV, IN><<<grid, L::kBlock, L::kDynamic, stream>>>(a, maps);
