@@ -182,7 +182,7 @@ int launch_inv_det(const InvDetArgs &args, cudaStream_t s)
     {
         const size_t smem = static_cast<size_t>(STAGES) * kTile * BLK * sizeof(double);
         auto kernel = inv_det_pipe_kernel<DIM, STAGES>;
-        cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        cudaError_t status = allow_dynamic_smem(kernel, smem);
         if (status != cudaSuccess) return fail_cuda(status, "acro_b200_batch_inv_det (shared memory opt-in)");
         const int64_t n_full = args.count / kTile;
         int64_t grid = static_cast<int64_t>(sm_count()) * 3;

@@ -444,7 +444,7 @@ int launch_padded(const PaddedArgs &args, int trans_a, int trans_b, int sms, cud
     const size_t smem = sizeof(Smem<N>);
     auto kernel = trans_a ? (trans_b ? batched_gemm_padded_kernel<N, true, true> : batched_gemm_padded_kernel<N, true, false>)
                           : (trans_b ? batched_gemm_padded_kernel<N, false, true> : batched_gemm_padded_kernel<N, false, false>);
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_batched_gemm (shared memory opt-in)");
     int64_t grid = static_cast<int64_t>(sms) * (N == 64 ? 1 : 4);
     if (grid > args.batch) grid = args.batch;
@@ -458,7 +458,7 @@ int launch_ring(const GemmArgs &args, int trans_a, int trans_b, int sms, cudaStr
     const size_t smem = sizeof(Smem<N>);
     auto kernel = trans_a ? (trans_b ? batched_gemm_kernel<N, true, true> : batched_gemm_kernel<N, true, false>)
                           : (trans_b ? batched_gemm_kernel<N, false, true> : batched_gemm_kernel<N, false, false>);
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_batched_gemm (shared memory opt-in)");
     int64_t grid = static_cast<int64_t>(sms) * (N == 64 ? 1 : 4);
     if (grid > args.batch) grid = args.batch;
@@ -616,7 +616,7 @@ int launch_groups64(const GemmArgs &args, int trans_a, int trans_b, int sms, cud
     const size_t smem = sizeof(Smem<64>);
     auto kernel = trans_a ? (trans_b ? batched_gemm64_groups_kernel<true, true> : batched_gemm64_groups_kernel<true, false>)
                           : (trans_b ? batched_gemm64_groups_kernel<false, true> : batched_gemm64_groups_kernel<false, false>);
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_batched_gemm (shared memory opt-in)");
     int64_t grid = sms;
     if (grid > args.batch) grid = args.batch;
@@ -782,7 +782,7 @@ int acro_b200_gram(const double *X, const double *Y, double *S, int64_t rows, in
     const int tail = static_cast<int>(rows - slabs * slab);
     auto kernel = big ? batched_gemm_padded_kernel<64, true, false, true> : batched_gemm_padded_kernel<32, true, false, true>;
     const size_t smem = big ? sizeof(Smem<64>) : sizeof(Smem<32>);
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_gram (shared memory opt-in)");
 
     PaddedArgs pa;
@@ -797,7 +797,7 @@ int acro_b200_gram(const double *X, const double *Y, double *S, int64_t rows, in
         // full 64 x 64 slabs fill the ring's slots exactly: the two-group kernel of the batched 64^3 product, accumulating
         // (X_slab stored k x m: first operand transposed); one tile of partial sums per group
         auto gk = batched_gemm64_groups_kernel<true, false, true>;
-        status = cudaFuncSetAttribute(gk, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Smem<64>)));
+        status = allow_dynamic_smem(gk, sizeof(Smem<64>));
         if (status != cudaSuccess) return fail_cuda(status, "acro_b200_gram (shared memory opt-in)");
         int64_t grid = sms;
         if (grid > slabs) grid = slabs;

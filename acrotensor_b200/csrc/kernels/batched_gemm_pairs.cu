@@ -234,7 +234,7 @@ int launch_pairs(const PairArgs &args, int trans_a, int trans_b, int grid, cudaS
         if (!ACC && !trans_a && !trans_b && args.k == 27) kernel = batched_gemm_pairs_kernel<false, false, ACC, 27, 27, 27>;
     }
     const PairLayout L = pair_layout(args, ACC);
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L.total);
+    cudaError_t status = allow_dynamic_smem(kernel, L.total);
     if (status != cudaSuccess) return fail_cuda(status, where);
     kernel<<<grid, kThreads, L.total, stream>>>(args);
     return launch_status(where);

@@ -248,7 +248,7 @@ int batched_gemm_small_launch(const double *A, const double *B, double *C, int64
     const size_t smem = static_cast<size_t>(args.group) * (kStages * (m * k + k * n) + m * n) * 8 + kStages * sizeof(uint64_t);
     auto kernel = trans_a ? (trans_b ? batched_gemm_small_kernel<true, true> : batched_gemm_small_kernel<true, false>)
                           : (trans_b ? batched_gemm_small_kernel<false, true> : batched_gemm_small_kernel<false, false>);
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_batched_gemm (shared memory opt-in)");
     int per_sm = static_cast<int>((200 * 1024) / (smem + 1024));
     if (per_sm > 6) per_sm = 6;

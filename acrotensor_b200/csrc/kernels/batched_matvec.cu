@@ -185,7 +185,7 @@ int batched_matvec_launch(const double *M, const double *X, double *Y, int64_t b
     args.wait_flag = wait_flag_device_ptr();
     if (args.wait_flag == nullptr) return fail_cuda(cudaErrorUnknown, "acro_b200_batched_gemm (status flag)");
     const size_t smem = static_cast<size_t>(2) * group * (rows * cols + xin) * 8 + 8 + 2 * sizeof(uint64_t);
-    cudaError_t status = cudaFuncSetAttribute(batched_matvec_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(batched_matvec_kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_batched_gemm (shared memory opt-in)");
     int per_sm = static_cast<int>((200 * 1024) / (smem + 1024));
     if (per_sm > 8) per_sm = 8;

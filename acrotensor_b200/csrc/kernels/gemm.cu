@@ -347,7 +347,7 @@ extern "C" int acro_b200_gemm_batched(const double *A, const double *P, double *
     const int64_t tiles = batch * ((M + T - 1) / T) * ((N + T - 1) / T);
     if (tiles > (int64_t(1) << 30) || K > (int64_t(1) << 30)) return fail_unsupported("acro_b200_gemm: more than 2^30 tiles of C or K above 2^30");
     auto launch = [&](auto kernel, size_t smem, int per_sm) {
-        cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        cudaError_t status = allow_dynamic_smem(kernel, smem);
         if (status != cudaSuccess) return fail_cuda(status, "acro_b200_gemm (shared memory opt-in)");
         int64_t grid = static_cast<int64_t>(sms) * per_sm;
         if (grid > tiles) grid = tiles;

@@ -181,7 +181,7 @@ int gram_stream_launch(const double *X, const double *Y, double *partials, int64
     args.wait_flag = wait_flag_device_ptr();
     if (args.wait_flag == nullptr) return fail_cuda(cudaErrorUnknown, "acro_b200_gram (status flag)");
     const size_t smem = static_cast<size_t>(2) * group * (a + b) * 8 + static_cast<size_t>(kThreads) * kBlock * kBlock * 8 + 2 * sizeof(uint64_t);
-    cudaError_t status = cudaFuncSetAttribute(gram_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(gram_stream_kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_gram (shared memory opt-in)");
     int per_sm = static_cast<int>((200 * 1024) / (smem + 1024));
     if (per_sm > 4) per_sm = 4;

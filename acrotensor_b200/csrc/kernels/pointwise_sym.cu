@@ -272,7 +272,7 @@ int launch_pipe(const PointwiseArgs &args, cudaStream_t s, int ctas_per_sm)
     constexpr int BLK = DIM * DIM;
     const size_t smem = static_cast<size_t>(STAGES) * kTile * BLK * sizeof(double) * (SAME_XY ? 1 : 2);
     auto kernel = pointwise_sym_pipe_kernel<DIM, SAME_XY, STAGES>;
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_pointwise_sym (shared memory opt-in)");
     const int64_t n_full = args.points / kTile;
     int64_t grid = static_cast<int64_t>(sm_count()) * ctas_per_sm;
@@ -460,21 +460,21 @@ int launch_cell(const PointwiseArgs &args_in, cudaStream_t s)
         if (same_xy)
         {
             auto kernel = pointwise_cell_pipe_kernel<DIM, true, 4>;
-            status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            status = allow_dynamic_smem(kernel, smem);
             if (status != cudaSuccess) return fail_cuda(status, "acro_b200_pointwise_sym (shared memory opt-in)");
             kernel<<<static_cast<int>(grid), kTile, smem, s>>>(args, tile_pts);
         }
         else if (DIM == 3)
         {
             auto kernel = pointwise_cell_pipe_kernel<DIM, false, 3>;
-            status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            status = allow_dynamic_smem(kernel, smem);
             if (status != cudaSuccess) return fail_cuda(status, "acro_b200_pointwise_sym (shared memory opt-in)");
             kernel<<<static_cast<int>(grid), kTile, smem, s>>>(args, tile_pts);
         }
         else
         {
             auto kernel = pointwise_cell_pipe_kernel<DIM, false, 4>;
-            status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            status = allow_dynamic_smem(kernel, smem);
             if (status != cudaSuccess) return fail_cuda(status, "acro_b200_pointwise_sym (shared memory opt-in)");
             kernel<<<static_cast<int>(grid), kTile, smem, s>>>(args, tile_pts);
         }

@@ -728,7 +728,7 @@ int acro_b200_rank1_gemm(const double *W, const double *B1, const double *B2, do
     {
         const TmemSymLayout L = tmem_sym_layout(ni);
         auto tm_kernel = q == QN ? rank1_gemm_sym_tmem_kernel<QN> : rank1_gemm_sym_tmem_kernel<0>;
-        cudaError_t st = cudaFuncSetAttribute(tm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L.total);
+        cudaError_t st = allow_dynamic_smem(tm_kernel, L.total);
         if (st != cudaSuccess) return fail_cuda(st, "acro_b200_rank1_gemm (shared memory opt-in)");
         const int64_t sym_tiles = (elements + TM_TE - 1) / TM_TE;
         int64_t g1 = sms;
@@ -740,7 +740,7 @@ int acro_b200_rank1_gemm(const double *W, const double *B1, const double *B2, do
     {
         const SymLayout L = sym_layout(ni, SymSmall::TILE_E, SymSmall::IMAGES);
         auto sym_kernel = q == QN ? rank1_gemm_sym_kernel<SymSmall, QN> : rank1_gemm_sym_kernel<SymSmall, 0>;
-        cudaError_t st = cudaFuncSetAttribute(sym_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L.total);
+        cudaError_t st = allow_dynamic_smem(sym_kernel, L.total);
         if (st != cudaSuccess) return fail_cuda(st, "acro_b200_rank1_gemm (shared memory opt-in)");
         const int64_t sym_tiles = (elements + SymSmall::TILE_E - 1) / SymSmall::TILE_E;
         int64_t g1 = static_cast<int64_t>(sms) * SymSmall::CTAS;
@@ -749,7 +749,7 @@ int acro_b200_rank1_gemm(const double *W, const double *B1, const double *B2, do
         return launch_status("acro_b200_rank1_gemm (symmetric)");
     }
     auto kernel = rank1_gemm_kernel<4>;
-    cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(kernel, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_rank1_gemm (shared memory opt-in)");
     int64_t grid = static_cast<int64_t>(sms) * 2;
     if (grid > n_tiles) grid = n_tiles;

@@ -270,7 +270,7 @@ int launch_mass(const MassArgs &args, int sms, cudaStream_t stream)
 {
     const size_t smem = sizeof(Smem<G>);
     // The opt-in is a per-device function attribute; setting it again is a cheap host call.
-    cudaError_t status = cudaFuncSetAttribute(sumfact_mass_kernel<G>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaError_t status = allow_dynamic_smem(sumfact_mass_kernel<G>, smem);
     if (status != cudaSuccess) return fail_cuda(status, "acro_b200_sumfact_mass (shared memory opt-in)");
     const int64_t n_tiles = (args.elements + ET - 1) / ET;
     int64_t grid = static_cast<int64_t>(sms) * G::CTAS;

@@ -76,3 +76,17 @@ def test_heads_of_different_sizes():
 def test_rows_of_different_widths():
     """Groups of threads that are added up in shared memory beside rows of one group, which take none."""
     at_once(lambda: norm_gradient(100), lambda: norm_gradient(2000))
+
+
+def matvec(n):
+    torch.manual_seed(n)
+    a, x, y = (torch.randn(64, *s, dtype=torch.float64, device="cuda") for s in ((n, n), (n,), (n,)))
+
+    def call(stream):
+        _lib.check(lib().acro_b200_batched_gemm(a.data_ptr(), x.data_ptr(), y.data_ptr(), 64, n, 1, n, _lib.OP_ASSIGN, stream))
+        return (y,)
+    return call
+
+
+def test_contractions_of_different_sizes():
+    at_once(lambda: matvec(64), lambda: matvec(8))
