@@ -72,23 +72,15 @@ unsigned long long context_epoch() { return g_context_epoch.load(); }
 
 cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes)
 {
-    // the largest limit set so far, of each kernel on each device; a limit belongs to a CUDA context
+    // The largest limit that each kernel was given so far.  It is set in every call all the same, because it belongs to a device and a
+    // CUDA context, of which this thread may have others than the last caller.
     static std::mutex lock;
-    static std::map<std::pair<const void *, int>, size_t> allowed;
-    static unsigned long long epoch = 0;
-    int dev = -1;
-    cudaError_t status = cudaGetDevice(&dev);
-    if (status != cudaSuccess) return status;
+    static std::map<const void *, size_t> largest;
     std::lock_guard<std::mutex> guard(lock);
-    if (epoch != context_epoch())
-    {
-        allowed.clear();
-        epoch = context_epoch();
-    }
-    size_t &most = allowed[{kernel, dev}];
-    if (bytes <= most) return cudaSuccess;
-    status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    if (status == cudaSuccess) most = bytes;
+    size_t &most = largest[kernel];
+    const size_t limit = bytes > most ? bytes : most;
+    const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(limit));
+    if (status == cudaSuccess) most = limit;
     return status;
 }
 
