@@ -783,7 +783,8 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
     if (slots != nullptr)
     {
         a.slots = slots;
-        a.state_count = state_count;
+        // without states the slots only say which sequences are there
+        a.state_count = initial_state != nullptr || final_state != nullptr ? state_count : int64_t(INT32_MAX) + 1;
     }
     const acro_b200_token_array none = {};
     const int group = d.q_heads / d.kv_heads;

@@ -171,8 +171,8 @@ def linear_attention(out, q, k, v, log_decay, scale=1.0, offsets=None, initial_s
 
     q, k [sequences, tokens, heads, dk], v, out [..., dv]; or, with ``offsets`` (int64, sequences + 1 row numbers), [rows, heads, columns] with
     sequence n in the rows offsets[n] .. offsets[n+1]-1.  k and v may have fewer heads (a divisor of q's).  States are
-    [sequences, heads, dk, dv]; with ``slots`` (int32 per sequence, negative: not there) [any number, heads, dk, dv].  ``final_state`` may be
-    ``initial_state``.  ``scratch``: any contiguous array of :func:`linear_attention_scratch_bytes` bytes."""
+    [sequences, heads, dk, dv]; with ``slots`` (int32 per sequence, negative: not there) [any number, heads, dk, dv].  Slots without states
+    only say which sequences are there.  ``final_state`` may be ``initial_state``.  ``scratch``: any contiguous array of :func:`linear_attention_scratch_bytes` bytes."""
     scale = float(scale)
     key = (0, scale, _form(q), _form(k), _form(v), _form(out), _form(log_decay), _form(offsets), _form(initial_state), _form(final_state), _form(slots))
     plan = _known(key)

@@ -432,7 +432,8 @@ typedef struct acro_b200_linear_attention_desc
  *                  to no sequence have no effect and are not written.  A sequence may be empty: its final state is its initial state.
  *   initial_state  NULL (zero), or states [state_count][q_heads][dk][dv], contiguous; final_state NULL or the same, and may be the same memory
  *   slots          NULL (state n belongs to sequence n, state_count = sequences), or the state of each sequence.  A negative slot marks
- *                  a sequence that is not there: its rows and states are left as they were.
+ *                  a sequence that is not there: its rows and states are left as they were.  Without states that is all the slots say,
+ *                  and state_count is not looked at.
  *   scratch        acro_b200_linear_attention_scratch_bytes(desc, packed) bytes (0 is possible), 16-byte aligned; calls that share
  *                  it must not overlap on the device.
  * out must not be q, k or v.  No host synchronisation.  An infinity or NaN of a token reaches only the rows that see it by the
