@@ -58,6 +58,18 @@ struct SplitArgs
     int64_t sequences, tokens;
 };
 
+// Rows that a CTA of the split kernel takes at once, `each` quads of columns a row.
+__host__ __device__ __forceinline__ int split_at_once(int each) { return each >= 1024 ? 1 : 1024 / each; }
+
+// Infinities and NaN among two values as bf16, with zeros in their place.
+__device__ __forceinline__ uint32_t take_odd(Two &x)
+{
+    const bool first = !isfinite(first_of(x)), second = !isfinite(second_of(x));
+    const uint32_t all = pack_bf16(x);
+    x = two(first ? 0.0f : first_of(x), second ? 0.0f : second_of(x));
+    return (first ? all & 0xffffu : 0u) | (second ? all & 0xffff0000u : 0u);
+}
+
 template <class T, int IN>
 __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_constant__ SplitArgs a)
 {
@@ -72,7 +84,7 @@ __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_const
         begin = min(max(a.offsets[0], int64_t(0)), rows);
         end = min(max(a.offsets[a.sequences], int64_t(0)), rows);
     }
-    const int some = max(1, 1024 / each);       // rows at once
+    const int some = split_at_once(each);
     const int64_t plane = rows * each;
     for (int64_t first = begin + static_cast<int64_t>(blockIdx.x) * some; first < end; first += static_cast<int64_t>(gridDim.x) * some)
     {
@@ -99,25 +111,15 @@ __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_const
                 y[0] = two(z[0], z[1]);
                 y[1] = two(z[2], z[3]);
             }
+            // infinities and NaN are the first part's alone; finite values have finite parts, above the largest bf16 too
+            uint2 odd = make_uint2(0, 0);
+            if (__builtin_expect(!(isfinite(first_of(y[0])) && isfinite(second_of(y[0])) && isfinite(first_of(y[1])) && isfinite(second_of(y[1]))), 0))
+                odd = make_uint2(take_odd(y[0]), take_odd(y[1]));
 #pragma unroll
             for (int k = 0; k < IN; ++k)
             {
-                uint2 part;
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                {
-                    uint32_t w = pack_bf16(y[e]);
-                    if (__builtin_expect(odd_pair(w), 0))
-                    {
-                        // finite values above the largest bf16 are parts, too
-                        const uint32_t most = pack_bf16_finite(y[e]);
-                        w = (isfinite(first_of(y[e])) ? most & 0xffffu : w & 0xffffu) | (isfinite(second_of(y[e])) ? most & 0xffff0000u : w & 0xffff0000u);
-                    }
-                    const Two left = sub2(y[e], unpack_bf16(w));
-                    // infinities and NaN are the first part's alone
-                    y[e] = two(odd_half(w) ? 0.0f : first_of(left), odd_half(w >> 16) ? 0.0f : second_of(left));
-                    (e ? part.y : part.x) = w;
-                }
+                uint2 part = make_uint2(take_part(y[0]), take_part(y[1]));
+                if (k == 0) part = make_uint2(part.x | odd.x, part.y | odd.y);
                 to[k * plane + i] = part;
             }
         }
@@ -173,6 +175,7 @@ int attention_split(AttentionArgs &a, int type, const TokenRows *arrays, const i
     s.sequences = a.sequences;
     s.tokens = a.tokens;
     TokenRows plane[4];
+    int some = 1024;
     unsigned char *at = static_cast<unsigned char *>(planes);
     for (int i = 0; i < count; ++i)
     {
@@ -184,10 +187,11 @@ int attention_split(AttentionArgs &a, int type, const TokenRows *arrays, const i
         s.packs[i] = columns[i] % 4 == 0 && reinterpret_cast<uintptr_t>(arrays[i].data) % pack == 0 && arrays[i].sequence % 4 == 0 && arrays[i].token % 4 == 0 &&
                      arrays[i].head % 4 == 0;
         s.heads[i] = heads;
+        some = std::min(some, split_at_once(heads * filled / 4));
         plane[i] = {at, static_cast<int64_t>(heads) * filled * a.tokens, static_cast<int64_t>(heads) * filled, filled, arrays[i].group};
         at += attention_planes_bytes(type, rows, heads, columns[i]);
     }
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, 148 * 8)), count);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((rows + some - 1) / some, 148 * 8)), count);
     if (type == ACRO_B200_F32) attention_split_kernel<float, 3><<<grid, 256, 0, stream>>>(s);
     else if (type == ACRO_B200_F16) attention_split_kernel<__half, 2><<<grid, 256, 0, stream>>>(s);
     else attention_split_kernel<__nv_bfloat16, 1><<<grid, 256, 0, stream>>>(s);
