@@ -304,9 +304,15 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
     const int64_t n = blockIdx.x / a.heads;
     const bool reverse = p.reverse != 0;
     int64_t begin = 0, end = a.tokens;
-    if (a.offsets != nullptr) packed_range(a, n, &begin, &end);
+    if (a.offsets != nullptr && !rows_of_sequence(a.offsets, n, a.tokens, INT64_MIN, begin, end)) return;
     const int64_t count = segments_of(end - begin, a.segment);
     if (count <= 1) return;
+    if (a.offsets != nullptr)
+    {
+        bool lower = false;
+        for (int64_t i = threadIdx.x; i < n; i += kThreads) lower |= a.offsets[i] > begin;
+        if (__syncthreads_or(lower) != 0) return;
+    }
     // only the sequence's last segment is shorter; what it leaves matters backward in time alone
     if (threadIdx.x < 2) left[threadIdx.x] = exp(decay_log<A>(a.log_decay, head) * static_cast<double>(threadIdx.x == 0 ? a.segment : end - begin - (count - 1) * a.segment));
     __syncthreads();
@@ -373,7 +379,11 @@ struct ShareArgs
     int64_t sequences, tokens;
 };
 
-// out[row, h, c] = sum over the query heads of head h, in ascending order: the gradients of shared keys (blockIdx.y = 0) and values.
+// Rows that a CTA of the share kernel takes at once.
+__host__ __device__ __forceinline__ int share_at_once(int heads, int columns) { return heads * columns >= 1024 ? 1 : 1024 / (heads * columns); }
+
+// out[row, h, c] = sum over the query heads of head h, in ascending order: the gradients of shared keys (blockIdx.y = 0) and values, for the
+// rows that sequences own.
 template <class T>
 __global__ void __launch_bounds__(kThreads) attention_share_kernel(const __grid_constant__ ShareArgs a)
 {
@@ -382,38 +392,51 @@ __global__ void __launch_bounds__(kThreads) attention_share_kernel(const __grid_
     const A *sums = static_cast<const A *>(blockIdx.y ? a.sums[1] : a.sums[0]);
     const TokenRows &out = blockIdx.y ? a.out[1] : a.out[0];
     const int columns = blockIdx.y ? a.columns[1] : a.columns[0], group = a.group;
-    int64_t begin = 0, end = a.sequences * a.tokens;
+    const int each = a.heads * columns, some = share_at_once(a.heads, columns);
+    int64_t begin = 0, end = a.sequences * a.tokens, ranges = 1, highest = INT64_MIN;
+    bool whole = true;
     if (a.offsets != nullptr)
     {
-        begin = min(max(a.offsets[0], int64_t(0)), a.tokens);
-        end = min(max(a.offsets[a.sequences], int64_t(0)), a.tokens);
+        // one range from the first sequence to the last, unless some are skipped
+        begin = a.offsets[0];
+        end = a.offsets[a.sequences];
+        whole = offsets_ascend(a.offsets, a.sequences, a.tokens);
+        if (!whole) ranges = a.sequences;
     }
-    const int each = a.heads * columns, some = max(1, 1024 / each);     // rows at once
-    for (int64_t first = begin + static_cast<int64_t>(blockIdx.x) * some; first < end; first += static_cast<int64_t>(gridDim.x) * some)
+    for (int64_t range = 0; range < ranges; ++range)
     {
-        const int count = static_cast<int>(min(static_cast<int64_t>(some), end - first)) * each;
-        for (int i0 = threadIdx.x; i0 < count; i0 += AT_ONCE * kThreads)
+        if (!whole)
         {
-            A s[AT_ONCE];
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) s[u] = 0;
-            for (int k = 0; k < group; ++k)
+            const bool there = rows_of_sequence(a.offsets, range, a.tokens, highest, begin, end);
+            highest = max(highest, begin);
+            if (!there) continue;
+        }
+        for (int64_t first = begin + static_cast<int64_t>(blockIdx.x) * some; first < end; first += static_cast<int64_t>(gridDim.x) * some)
+        {
+            const int count = static_cast<int>(min(static_cast<int64_t>(some), end - first)) * each;
+            for (int i0 = threadIdx.x; i0 < count; i0 += AT_ONCE * kThreads)
             {
+                A s[AT_ONCE];
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) s[u] = 0;
+                for (int k = 0; k < group; ++k)
+                {
+#pragma unroll
+                    for (int u = 0; u < AT_ONCE; ++u)
+                    {
+                        const int i = i0 + u * kThreads, h = i / columns;       // over the heads of all these rows
+                        if (i < count) s[u] += sums[((first * a.heads + h) * group + k) * columns + (i - h * columns)];
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < AT_ONCE; ++u)
                 {
-                    const int i = i0 + u * kThreads, h = i / columns;       // over the heads of all these rows
-                    if (i < count) s[u] += sums[((first * a.heads + h) * group + k) * columns + (i - h * columns)];
+                    const int i = i0 + u * kThreads;
+                    if (i >= count) break;
+                    const int own = i / each, rest = i - own * each, h = rest / columns, c = rest - h * columns;
+                    const int64_t row = first + own, n = a.offsets == nullptr ? row / a.tokens : 0, t = row - n * a.tokens;
+                    static_cast<T *>(out.data)[n * out.sequence + t * out.token + h * out.head + c] = narrow<T>(s[u]);
                 }
-            }
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u)
-            {
-                const int i = i0 + u * kThreads;
-                if (i >= count) break;
-                const int own = i / each, rest = i - own * each, h = rest / columns, c = rest - h * columns;
-                const int64_t row = first + own, n = a.offsets == nullptr ? row / a.tokens : 0, t = row - n * a.tokens;
-                static_cast<T *>(out.data)[n * out.sequence + t * out.token + h * out.head + c] = narrow<T>(s[u]);
             }
         }
     }
@@ -984,7 +1007,8 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     cudaStream_t st = as_stream(stream);
     status = run_all(d, a, arrays, columns, 4, at, st);
     if (status != ACRO_B200_OK || !rows) return status;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((packed ? 1 : d.sequences) * d.tokens, 148 * 8)), 2);
+    const int some = std::min(share_at_once(d.kv_heads, d.dk), share_at_once(d.kv_heads, d.dv));
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(((packed ? 1 : d.sequences) * d.tokens + some - 1) / some, 148 * 8)), 2);
     switch (d.type)
     {
     case ACRO_B200_F64: attention_share_kernel<double><<<grid, kThreads, 0, st>>>(both); break;

@@ -88,16 +88,23 @@ __device__ __forceinline__ int64_t segment_state(const AttentionArgs &a, int64_t
     return sequence * segments_of(a.tokens, a.segment) + index;
 }
 
-// Rows [*begin, *end) of a packed sequence.  Offsets that decrease or leave the arrays are cut back (and reported): no access
-// ever leaves the rows.
-__device__ __forceinline__ void packed_range(const AttentionArgs &a, int64_t n, int64_t *begin, int64_t *end)
+// An entry of `offsets` is bad when it is not in 0 .. rows or lower than one in front of it.  A sequence that starts or ends at a bad
+// entry is skipped (and reported), so that the others have rows, and places for segments' states, of their own.
+
+// Are all entries good?  Every thread of the CTA calls it; holds a CTA barrier.
+__device__ __forceinline__ bool offsets_ascend(const int64_t *offsets, int64_t sequences, int64_t rows)
 {
-    const int64_t b = a.offsets[n], e = a.offsets[n + 1];
-    int64_t lo = b < 0 ? 0 : b > a.tokens ? a.tokens : b;
-    int64_t hi = e < lo ? lo : e > a.tokens ? a.tokens : e;
-    if (lo != b || hi != e) atomicOr(a.bad_index, 1);
-    *begin = lo;
-    *end = hi;
+    bool bad = false;
+    for (int64_t n = threadIdx.x; n < sequences; n += blockDim.x) bad |= offsets[n] < 0 || offsets[n + 1] < offsets[n] || offsets[n + 1] > rows;
+    return __syncthreads_or(bad) == 0;
+}
+
+// Rows begin .. end-1 of sequence n, or false for one that is skipped.  `highest`: the highest entry in front of n.
+__device__ __forceinline__ bool rows_of_sequence(const int64_t *offsets, int64_t n, int64_t rows, int64_t highest, int64_t &begin, int64_t &end)
+{
+    begin = offsets[n];
+    end = offsets[n + 1];
+    return begin >= 0 && begin >= highest && end >= begin && end <= rows;
 }
 
 // Which state belongs to entry n of `slots`: -1 when the entry is negative (a request that is not there), out of range or the
@@ -158,6 +165,41 @@ __device__ __forceinline__ void scan_two(int64_t &x, int64_t &y, int64_t &total_
     y += ahead_y - own_y;
 }
 
+// The highest of `highest` and the `mine` of the threads in front of this one; `highest` becomes that of all threads.  Every thread calls
+// it; holds CTA barriers.
+__device__ __forceinline__ int64_t highest_ahead(int64_t mine, int64_t &highest, int64_t (*sums)[2])
+{
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const int64_t up = __shfl_up_sync(0xffffffffu, mine, o);
+        if (lane >= o && up > mine) mine = up;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp][0] = mine;
+    __syncthreads();
+    int64_t ahead = __shfl_up_sync(0xffffffffu, mine, 1);
+    if (lane == 0 || ahead < highest) ahead = highest;
+    for (int w = 0; w < warps; ++w)
+    {
+        if (w < warp && sums[w][0] > ahead) ahead = sums[w][0];
+        if (sums[w][0] > highest) highest = sums[w][0];
+    }
+    return ahead;
+}
+
+// Rows of sequence base + threadIdx.x, or false.  `ascend`: all entries are good.  `highest`: the highest entry in front of base,
+// then that in front of base + blockDim.x.  Every thread calls it; holds CTA barriers unless `ascend`.
+__device__ __forceinline__ bool next_rows(const AttentionArgs &a, int64_t base, bool ascend, int64_t &highest, int64_t &begin, int64_t &end, int64_t (*sums)[2])
+{
+    const int64_t n = base + threadIdx.x;
+    const bool there = n < a.sequences;
+    int64_t ahead = 0;
+    if (!ascend) ahead = highest_ahead(there ? a.offsets[n] : INT64_MIN, highest, sums);
+    return there && rows_of_sequence(a.offsets, n, a.tokens, ahead, begin, end);
+}
+
 // Item `launched` of the list of all sequences' segments.  Packed sequences put their whole segments in front and their (shorter) last
 // ones behind, so that the long work starts first.  Every thread of the CTA (at most 1024, whole warps) calls it and gets the same
 // answer; holds CTA barriers.
@@ -178,23 +220,30 @@ __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t
         __shared__ int64_t found[4], sums[32][2];
         if (threadIdx.x == 0) found[0] = -1;
         // the number of whole segments of all sequences
-        int64_t all = 0;
+        int64_t all = 0, b, e, highest = INT64_MIN;
+        bool bad = false;
         for (int64_t n = threadIdx.x; n < a.sequences; n += blockDim.x)
         {
-            int64_t b, e;
-            packed_range(a, n, &b, &e);
-            all += (e - b) / a.segment;
+            if (rows_of_sequence(a.offsets, n, a.tokens, 0, b, e)) all += (e - b) / a.segment;
+            else bad = true;
+        }
+        const bool ascend = __syncthreads_or(bad) == 0;
+        if (!ascend)
+        {
+            if (threadIdx.x == 0) atomicOr(a.bad_index, 1);
+            all = 0;
+            for (int64_t base = 0; base < a.sequences; base += blockDim.x)
+                if (next_rows(a, base, false, highest, b, e, sums)) all += (e - b) / a.segment;
         }
         int64_t none = 0, whole, nothing;
         scan_two(all, none, whole, nothing, sums);
         int64_t before_last = 0, before_whole = 0;
+        highest = INT64_MIN;
         for (int64_t base = 0; base < a.sequences; base += blockDim.x)
         {
-            const int64_t n = base + threadIdx.x;
-            int64_t b = 0, e = 0, mine_last = 0, mine_whole = 0;
-            if (n < a.sequences)
+            int64_t mine_last = 0, mine_whole = 0;
+            if (next_rows(a, base, ascend, highest, b, e, sums))
             {
-                packed_range(a, n, &b, &e);
                 mine_whole = (e - b) / a.segment;
                 mine_last = segments_of(e - b, a.segment) - mine_whole;
             }
@@ -207,7 +256,7 @@ __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t
             if (launched >= whole && mine_last > 0 && launched - whole == start_last) which = mine_whole;
             if (which >= 0)
             {
-                found[0] = n;
+                found[0] = base + threadIdx.x;
                 found[1] = b;
                 found[2] = e;
                 found[3] = which;

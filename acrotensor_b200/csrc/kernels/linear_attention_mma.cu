@@ -80,9 +80,13 @@ __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_const
     int64_t begin = 0, end = rows;
     if (a.offsets != nullptr)
     {
-        // rows that no sequence owns are not read
-        begin = min(max(a.offsets[0], int64_t(0)), rows);
-        end = min(max(a.offsets[a.sequences], int64_t(0)), rows);
+        // rows that no sequence owns are not read (where sequences are skipped, all rows are)
+        const int64_t from = a.offsets[0], to = a.offsets[a.sequences];
+        if (offsets_ascend(a.offsets, a.sequences, rows))
+        {
+            begin = from;
+            end = to;
+        }
     }
     const int some = split_at_once(each);
     const int64_t plane = rows * each;

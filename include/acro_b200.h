@@ -393,9 +393,10 @@ int acro_b200_halo_destroy(acro_b200_halo *halo);
  * Sequence operators: what a layer over token sequences needs beside its contractions.  No counterpart in the reference.
  * Element types: 64, 32 and 16 bits.  Sums, states, decays and row statistics are in 32 bits (64 for ACRO_B200_F64): the
  * "type of sums" below.  All pointers are device memory of the current device; memory of another device is refused.
- * Entries of index arrays are read on the device only: one that is out of range or repeated is skipped, nothing outside the
- * arrays is touched, and acro_b200_device_status() reports ACRO_B200_EINVAL.  Calls may be captured into a CUDA graph; the first one on
- * each device belongs before the first capture.  Arrays start on a boundary of their elements.
+ * Entries of index arrays are read on the device only: what belongs to one that is out of range, decreasing or repeated is skipped
+ * (its rows and states are left as they were), nothing outside the arrays is touched, and acro_b200_device_status() reports
+ * ACRO_B200_EINVAL.  Calls may be captured into a CUDA graph; the first one on each device belongs before the first capture.  Arrays
+ * start on a boundary of their elements.
  */
 #define ACRO_B200_F64 0
 #define ACRO_B200_F32 1
@@ -430,6 +431,7 @@ typedef struct acro_b200_linear_attention_desc
  *                  with its length and may overflow
  *   offsets        NULL, or sequences + 1 ascending row numbers: sequence n has the rows offsets[n] .. offsets[n+1]-1.  Rows that belong
  *                  to no sequence have no effect and are not written.  A sequence may be empty: its final state is its initial state.
+ *                  A sequence that starts or ends at a number below zero, behind the rows or lower than one in front of it is skipped.
  *   initial_state  NULL (zero), or states [state_count][q_heads][dk][dv], contiguous; final_state NULL or the same, and may be the same memory
  *   slots          NULL (state n belongs to sequence n, state_count = sequences), or the state of each sequence.  A negative slot marks
  *                  a sequence that is not there: its rows and states are left as they were.  Without states that is all the slots say,

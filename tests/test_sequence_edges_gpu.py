@@ -26,3 +26,47 @@ def test_slots_without_states_only_say_which_sequences_are_there(kind, lengths, 
         assert torch.equal(p.of(out, i), p.of(expect, i))
     assert bool((p.of(out, 1) == -7.0).all())
     p.untouched(out)
+
+
+def owned(offsets, rows):
+    """(sequence, begin, end) of the sequences that no bad entry starts or ends: below zero, behind the rows or lower than one in front."""
+    found, highest = [], -2 ** 63
+    for n, (b, e) in enumerate(zip(offsets, offsets[1:])):
+        if 0 <= b <= e <= rows and b >= highest:
+            found.append((n, b, e))
+        highest = max(highest, b)
+    return found
+
+
+OFFSETS = [(90, [0, 5000], 0), (90, [-5, 60], 0), (90, [60, 30], 0), (3000, [0, 5000], 0), (90, [0, 50, 20, 90], 1), (90, [-40, 30, 60, 90], 2), (90, [0, 30, 60, 5000], 2), (90, [2 ** 40, 30, -2 ** 60, 2 ** 62], 0),
+           (90, [0, 5000, 10, 5000], 0), (90, [5, 40, 40, 80, 70, 90], 3), (3000, [0, 1300, 900, 3000], 1), (3000, [0, 700, 2 ** 40, 2000, 3000], 1),
+           (3000, [100, 2900, 2900, 2950, -1, 3000], 3), (3000, list(range(1500)) + [0] + list(range(1501, 2001)) + [1700] + list(range(2002, 3001)), 2996)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32", "f64"])
+@pytest.mark.parametrize("rows,offsets,count", OFFSETS, ids=lambda x: str(x)[:30])
+def test_sequences_at_bad_offsets_are_left_alone(kind, rows, offsets, count):
+    """Their rows, their states and the rows between them; the others get what they get without them."""
+    n, d = len(offsets) - 1, 16
+    good = owned(offsets, rows)
+    assert len(good) == count
+    p = Problem(kind, [rows] + [0] * (n - 1), True, 2, 1, d, d, spare=0)
+    p.offsets = torch.tensor(offsets, device="cuda")
+    out, end = p.forward()
+    assert lib().acro_b200_device_status() == _lib.EINVAL
+    grads = p.backward()
+    assert lib().acro_b200_device_status() == _lib.EINVAL
+    left, gone = torch.ones(rows, dtype=torch.bool, device="cuda"), [i for i in range(n) if i not in {s for s, _, _ in good}]
+    for s, b, e in good:
+        left[b:e] = False
+    for x in (out,) + grads[:3]:
+        assert bool((x[left] == -7.0).all())
+    for x in (end, grads[3]):
+        assert bool((x[gone] == -7.0).all())
+    # one after the other, as many as there are different kinds of
+    for s, b, e in good[:3] + good[-3:] + [g for g in good if g[0] in (1498, 1501, 1502, 1999, 2000, 2002, 2003)]:
+        one = Problem(kind, [e - b], True, 2, 1, d, d, spare=0)
+        one.q, one.k, one.v, one.dout = (x[b:e] for x in (p.q, p.k, p.v, p.dout))
+        one.initial, one.dfinal = p.initial[s:s + 1], p.dfinal[s:s + 1]
+        one.check_forward(out[b:e], end[s:s + 1])
+        one.check_backward(*[x[b:e] for x in grads[:3]], grads[3][s:s + 1])
