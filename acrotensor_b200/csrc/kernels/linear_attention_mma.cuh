@@ -302,6 +302,8 @@ __global__ void __launch_bounds__(kBlock, 1) attention_mma_kernel(const __grid_c
                 issue_scores(c + 1);
             }
         }
+        // no product is in flight when this warp gives its tensor memory back
+        if (ok && chunks > 0) ok = all_wait(&sh.out, (chunks - 1) & 1);
         if (!ok)
         {
             if (lane == 0) *a.wait_flag = 1;
@@ -597,7 +599,7 @@ struct StateShared
 {
     float left[kChunk + 4];
     uint32_t tmem;
-    uint64_t full[4], ready[2], done[2];
+    uint64_t full[4], ready[2], done[2], drained;
 };
 
 template <int NQ, int NV, int IN>
@@ -626,6 +628,7 @@ __global__ void __launch_bounds__(StateLayout<NQ, NV, IN>::kBlock, 1) attention_
             mbar_init(&sh.ready[i], L::kMakers / 32);
             mbar_init(&sh.done[i], 1);
         }
+        mbar_init(&sh.drained, 1);
         fence_mbar_init();
     }
     if (warp == 16) tmem_alloc(&sh.tmem, L::kColumns);
@@ -686,10 +689,14 @@ __global__ void __launch_bounds__(StateLayout<NQ, NV, IN>::kBlock, 1) attention_
                 load(loaded++);
             }
         }
+        if (ok) ok = all_wait(&sh.done[(chunks - 1) & 1], (chunks - 1) / 2 & 1);
         if (!ok)
         {
             if (lane == 0) *a.wait_flag = 1;
+            // copies and products of this CTA that are still in flight
             for (int i = c; i < loaded; ++i) all_wait(&sh.full[i % L::kStages], i / L::kStages & 1);
+            umma_commit(leader, &sh.drained);
+            all_wait(&sh.drained, 0);
         }
     }
     else
@@ -768,13 +775,16 @@ __global__ void __launch_bounds__(StateLayout<NQ, NV, IN>::kBlock, 1) attention_
             add(c - 1);
         }
         if (ok) ok = all_wait(&sh.done[(chunks - 1) & 1], (chunks - 1) / 2 & 1);
-        if (!ok && lane == 0) *a.wait_flag = 1;
-        tmem_fence_after_sync();
-        add(chunks - 1);
-        float *to = static_cast<float *>(p.segment_states) + (item.segment_state * a.heads + head) * (static_cast<int64_t>(p.dq) * p.dv);
+        if (ok)
+        {
+            tmem_fence_after_sync();
+            add(chunks - 1);
+            float *to = static_cast<float *>(p.segment_states) + (item.segment_state * a.heads + head) * (static_cast<int64_t>(p.dq) * p.dv);
 #pragma unroll
-        for (int j = 0; j < NQ * 16; ++j)
-            if (b < p.dv && d0 + j < p.dq) to[(d0 + j) * p.dv + b] = j % 2 ? second_of(sum[j / 2]) : first_of(sum[j / 2]);
+            for (int j = 0; j < NQ * 16; ++j)
+                if (b < p.dv && d0 + j < p.dq) to[(d0 + j) * p.dv + b] = j % 2 ? second_of(sum[j / 2]) : first_of(sum[j / 2]);
+        }
+        else if (lane == 0) *a.wait_flag = 1;
     }
     tmem_fence_before_sync();
     __syncthreads();
