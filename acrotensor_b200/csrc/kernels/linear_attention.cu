@@ -628,12 +628,30 @@ size_t shared_bytes(const acro_b200_linear_attention_desc &d, bool packed, int c
 
 TokenRows rows_from(const acro_b200_token_array &x, int group) { return {x.data, x.sequence_stride, x.token_stride, x.head_stride, group}; }
 
+// Does no row of an array share an entry with another?  Of heads, tokens and sequences the one of a larger stride has to stride over all of
+// the smaller ones.
+bool rows_apart(const acro_b200_token_array &x, int64_t columns, int heads, int64_t tokens, int64_t sequences, bool packed)
+{
+    struct { int64_t stride, count; } dims[3] = {{x.head_stride, heads}, {x.token_stride, tokens}, {x.sequence_stride, packed ? 1 : sequences}};
+    std::sort(dims, dims + 3, [](const auto &a, const auto &b) { return a.stride < b.stride; });
+    __int128 extent = columns;
+    for (const auto &dim : dims)
+    {
+        if (dim.count <= 1) continue;
+        if (dim.stride < extent) return false;
+        extent += static_cast<__int128>(dim.stride) * (dim.count - 1);
+    }
+    return true;
+}
+
+// `written`: by different CTAs, so no two rows may share an entry; rows that are only read are as far apart as their columns in each dimension.
 std::string array_fault(const acro_b200_linear_attention_desc &d, const acro_b200_token_array *x, int64_t columns, int heads, int64_t tokens, int64_t sequences,
-                        bool packed, const char *name)
+                        bool packed, const char *name, bool written = false)
 {
     const std::string n(name);
     if (x == nullptr || x->data == nullptr) return n + " is a null pointer";
-    if ((heads > 1 && x->head_stride < columns) || (tokens > 1 && x->token_stride < columns) || (!packed && sequences > 1 && x->sequence_stride < columns))
+    if ((heads > 1 && x->head_stride < columns) || (tokens > 1 && x->token_stride < columns) || (!packed && sequences > 1 && x->sequence_stride < columns) ||
+        (written && !rows_apart(*x, columns, heads, tokens, sequences, packed)))
         return n + " has rows that overlap";
     if (!aligned_to({x->data}, element_bytes(d.type))) return n + " is not aligned to its elements";
     return "";
@@ -783,7 +801,7 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
         if (fault.empty()) fault = array_fault(d, q, d.dk, d.q_heads, d.tokens, d.sequences, packed, "q");
         if (fault.empty()) fault = array_fault(d, k, d.dk, d.kv_heads, d.tokens, d.sequences, packed, "k");
         if (fault.empty()) fault = array_fault(d, v, d.dv, d.kv_heads, d.tokens, d.sequences, packed, "v");
-        if (fault.empty()) fault = array_fault(d, out, d.dv, d.q_heads, d.tokens, d.sequences, packed, "out");
+        if (fault.empty()) fault = array_fault(d, out, d.dv, d.q_heads, d.tokens, d.sequences, packed, "out", true);
     }
     if (fault.empty() && log_decay == nullptr) fault = "log_decay is a null pointer";
     if (fault.empty() && slots != nullptr && state_count < 0) fault = "negative state_count";
@@ -843,7 +861,7 @@ int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc,
     fault = array_fault(d, q, d.dk, d.q_heads, 1, d.sequences, false, "q");
     if (fault.empty()) fault = array_fault(d, k, d.dk, d.kv_heads, 1, d.sequences, false, "k");
     if (fault.empty()) fault = array_fault(d, v, d.dv, d.kv_heads, 1, d.sequences, false, "v");
-    if (fault.empty()) fault = array_fault(d, out, d.dv, d.q_heads, 1, d.sequences, false, "out");
+    if (fault.empty()) fault = array_fault(d, out, d.dv, d.q_heads, 1, d.sequences, false, "out", true);
     if (fault.empty() && (log_decay == nullptr || state_in == nullptr || state_out == nullptr)) fault = "null pointer";
     if (fault.empty() && (!aligned_to({log_decay, state_in, state_out}, statistic_bytes(d.type)) || !aligned_to({slots}, 4)))
         fault = "log_decay, slots or a state is not aligned to its elements";
@@ -926,12 +944,12 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
     const acro_b200_linear_attention_desc &d = *desc;
     if (d.sequences == 0) return ACRO_B200_OK;
     const bool packed = offsets != nullptr, rows = d.tokens > 0;
-    const struct { const acro_b200_token_array *x; int columns, heads; const char *name; } given[] = {
-        {q, d.dk, d.q_heads, "q"}, {k, d.dk, d.kv_heads, "k"}, {v, d.dv, d.kv_heads, "v"}, {dout, d.dv, d.q_heads, "dout"},
-        {dq, d.dk, d.q_heads, "dq"}, {dk, d.dk, d.kv_heads, "dk"}, {dv, d.dv, d.kv_heads, "dv"}};
+    const struct { const acro_b200_token_array *x; int columns, heads; const char *name; bool written; } given[] = {
+        {q, d.dk, d.q_heads, "q", false}, {k, d.dk, d.kv_heads, "k", false}, {v, d.dv, d.kv_heads, "v", false}, {dout, d.dv, d.q_heads, "dout", false},
+        {dq, d.dk, d.q_heads, "dq", true}, {dk, d.dk, d.kv_heads, "dk", true}, {dv, d.dv, d.kv_heads, "dv", true}};
     if (rows)
         for (const auto &x : given)
-            if (fault.empty()) fault = array_fault(d, x.x, x.columns, x.heads, d.tokens, d.sequences, packed, x.name);
+            if (fault.empty()) fault = array_fault(d, x.x, x.columns, x.heads, d.tokens, d.sequences, packed, x.name, x.written);
     if (fault.empty() && log_decay == nullptr) fault = "log_decay is a null pointer";
     const size_t need = acro_b200_linear_attention_backward_scratch_bytes(desc, packed);
     if (fault.empty() && need > 0 && (scratch == nullptr || scratch_bytes < need || !aligned16(scratch)))

@@ -404,7 +404,8 @@ int acro_b200_halo_destroy(acro_b200_halo *halo);
 #define ACRO_B200_F16 3
 
 /* Rows of heads: element (sequence n, token t, head h, column c) is at data[n * sequence_stride + t * token_stride + h * head_stride + c]
- * (strides in elements; columns are contiguous, rows do not overlap).  With packed sequences (`offsets`) t counts over all rows. */
+ * (strides in elements; columns are contiguous; rows do not overlap: of heads, tokens and sequences the one of a larger stride strides
+ * over all of the smaller ones).  With packed sequences (`offsets`) t counts over all rows. */
 typedef struct acro_b200_token_array
 {
     void *data;
