@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 #include <initializer_list>
+#include <vector>
 
 namespace acro
 {
@@ -259,6 +260,26 @@ class StreamScratch
     size_t Bytes;
 };
 
+// Tensors that a call overwrites whole (null ones aside).  They stay on the side where they are until the call has been accepted, so that a refused
+// one leaves their values where the caller has them.
+class Results
+{
+    public:
+    Results(std::initializer_list<Tensor *> tensors) : Tensors(tensors)
+    {
+        for (Tensor *T : Tensors)
+            if (T != nullptr && !T->IsMappedToGPU()) T->MapToGPU();
+    }
+    void Written()
+    {
+        for (Tensor *T : Tensors)
+            if (T != nullptr) T->SwitchToGPU();
+    }
+
+    private:
+    std::vector<Tensor *> Tensors;
+};
+
 void require_shape(Tensor &T, std::initializer_list<int> dims, const char *what)
 {
     bool same = T.IsInitialized() && T.GetRank() == static_cast<int>(dims.size());
@@ -331,8 +352,7 @@ void TensorEngine::LinearAttention(Tensor &Out, Tensor &Q, Tensor &K, Tensor &V,
     RequireCuda("LinearAttention");
     for (Tensor *T : {&Q, &K, &V, &LogDecay, InitialState})
         if (T != nullptr) T->MoveToGPU();
-    Out.SwitchToGPU();
-    if (FinalState != nullptr && FinalState != InitialState) FinalState->SwitchToGPU();
+    Results results({&Out, FinalState});
     HeadDims o = q;
     o.columns = v.columns;
     const acro_b200_token_array rq = q.Rows(Q), rk = k.Rows(K), rv = v.Rows(V), ro = o.Rows(Out);
@@ -340,6 +360,7 @@ void TensorEngine::LinearAttention(Tensor &Out, Tensor &Q, Tensor &K, Tensor &V,
     check_abi(acro_b200_linear_attention(&d, &rq, &rk, &rv, &ro, LogDecay.GetDeviceData(), nullptr, device_data(InitialState), device_data(FinalState),
                                          nullptr, d.sequences, scratch.Get(), scratch.Size(), Stream()),
               "linear_attention");
+    results.Written();
 }
 
 void TensorEngine::LinearAttentionStep(Tensor &Out, Tensor &StateOut, Tensor &Q, Tensor &K, Tensor &V, Tensor &LogDecay, Tensor &StateIn, double scale)
@@ -355,8 +376,7 @@ void TensorEngine::LinearAttentionStep(Tensor &Out, Tensor &StateOut, Tensor &Q,
     require_shape(StateOut, {n, heads, dk, dv}, "StateOut");
     RequireCuda("LinearAttentionStep");
     for (Tensor *T : {&Q, &K, &V, &LogDecay, &StateIn}) T->MoveToGPU();
-    Out.SwitchToGPU();
-    if (&StateOut != &StateIn) StateOut.SwitchToGPU();
+    Results results({&Out, &StateOut});
     acro_b200_linear_attention_desc d = {};
     d.type = ACRO_B200_F64;
     d.q_heads = heads;
@@ -371,6 +391,7 @@ void TensorEngine::LinearAttentionStep(Tensor &Out, Tensor &StateOut, Tensor &Q,
     check_abi(acro_b200_linear_attention_step(&d, &rq, &rk, &rv, &ro, LogDecay.GetDeviceData(), StateIn.GetDeviceData(), StateOut.GetDeviceData(), nullptr,
                                               n, Stream()),
               "linear_attention_step");
+    results.Written();
 }
 
 void TensorEngine::LinearAttentionBackward(Tensor &dQ, Tensor &dK, Tensor &dV, Tensor &dOut, Tensor &Q, Tensor &K, Tensor &V, Tensor &LogDecay, double scale,
@@ -389,8 +410,7 @@ void TensorEngine::LinearAttentionBackward(Tensor &dQ, Tensor &dK, Tensor &dV, T
     RequireCuda("LinearAttentionBackward");
     for (Tensor *T : {&Q, &K, &V, &LogDecay, &dOut, InitialState, dFinalState})
         if (T != nullptr) T->MoveToGPU();
-    for (Tensor *T : {&dQ, &dK, &dV, dInitialState})
-        if (T != nullptr) T->SwitchToGPU();
+    Results results({&dQ, &dK, &dV, dInitialState});
     HeadDims o = q;
     o.columns = v.columns;
     const acro_b200_token_array rq = q.Rows(Q), rk = k.Rows(K), rv = v.Rows(V), ro = o.Rows(dOut), gq = q.Rows(dQ), gk = k.Rows(dK), gv = v.Rows(dV);
@@ -399,6 +419,7 @@ void TensorEngine::LinearAttentionBackward(Tensor &dQ, Tensor &dK, Tensor &dV, T
                                                   device_data(dFinalState), &gq, &gk, &gv, device_data(dInitialState), scratch.Get(), scratch.Size(),
                                                   Stream()),
               "linear_attention_backward");
+    results.Written();
 }
 
 void TensorEngine::LayerNorm(Tensor &Y, Tensor &X, Tensor *Weight, Tensor *Bias, double eps, Tensor *Mean, Tensor *Rstd)
@@ -414,11 +435,11 @@ void TensorEngine::LayerNorm(Tensor &Y, Tensor &X, Tensor *Weight, Tensor *Bias,
     RequireCuda("LayerNorm");
     for (Tensor *T : {&X, Weight, Bias})
         if (T != nullptr) T->MoveToGPU();
-    for (Tensor *T : {&Y, Mean, Rstd})
-        if (T != nullptr && T != &X) T->SwitchToGPU();
+    Results results({&Y, Mean, Rstd});
     check_abi(acro_b200_layer_norm(ACRO_B200_F64, X.GetDeviceData(), width, device_data(Weight), device_data(Bias), Y.GetDeviceData(), width, device_data(Mean),
                                    device_data(Rstd), rows, width, eps, Stream()),
               "layer_norm");
+    results.Written();
 }
 
 void TensorEngine::LayerNormBackward(Tensor &dX, Tensor *dWeight, Tensor *dBias, Tensor &dY, Tensor &X, Tensor &Mean, Tensor &Rstd, Tensor *Weight)
@@ -433,14 +454,14 @@ void TensorEngine::LayerNormBackward(Tensor &dX, Tensor *dWeight, Tensor *dBias,
     RequireCuda("LayerNormBackward");
     for (Tensor *T : {&dY, &X, &Mean, &Rstd, Weight})
         if (T != nullptr) T->MoveToGPU();
-    for (Tensor *T : {&dX, dWeight, dBias})
-        if (T != nullptr && T != &X && T != &dY) T->SwitchToGPU();
+    Results results({&dX, dWeight, dBias});
     const bool sums = dWeight != nullptr || dBias != nullptr;
     StreamScratch scratch(sums ? acro_b200_layer_norm_backward_scratch_bytes(ACRO_B200_F64, rows, width) : 0, Stream());
     check_abi(acro_b200_layer_norm_backward(ACRO_B200_F64, dY.GetDeviceData(), width, X.GetDeviceData(), width, device_data(Weight), Mean.GetDeviceData(),
                                             Rstd.GetDeviceData(), dX.GetDeviceData(), width, device_data(dWeight), device_data(dBias), rows, width,
                                             scratch.Get(), scratch.Size(), Stream()),
               "layer_norm_backward");
+    results.Written();
     if (ThePeerGroup == nullptr || !X.IsSharded()) return;
     for (Tensor *T : {dWeight, dBias})
         if (T != nullptr)

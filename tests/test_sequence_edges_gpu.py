@@ -70,3 +70,34 @@ def test_sequences_at_bad_offsets_are_left_alone(kind, rows, offsets, count):
         one.initial, one.dfinal = p.initial[s:s + 1], p.dfinal[s:s + 1]
         one.check_forward(out[b:e], end[s:s + 1])
         one.check_backward(*[x[b:e] for x in grads[:3]], grads[3][s:s + 1])
+
+
+def engine_calls(te, bad):
+    """(name, call of a result, the result's shape) of the engine's methods; with `bad` they are refused by the kernel layer: too many columns a
+    head, a negative eps, rows too wide to be overwritten."""
+    T, H, d = 5, 2, 257 if bad else 8
+    rng = np.random.default_rng(0)
+    t = lambda *s: ab.Tensor(s, hdata=rng.standard_normal(s))
+    yield "out", lambda r: te.LinearAttention(r, t(T, H, d), t(T, H, d), t(T, H, d), t(H), 1.0, None, None), (T, H, d)
+    yield "final", lambda r: te.LinearAttention(t(T, H, d), t(T, H, d), t(T, H, d), t(T, H, d), t(H), 1.0, None, r), (H, d, d)
+    yield "step", lambda r: te.LinearAttentionStep(r, t(T, H, d, d), t(T, H, d), t(T, H, d), t(T, H, d), t(H), t(T, H, d, d), 1.0), (T, H, d)
+    yield "dq", lambda r: te.LinearAttentionBackward(r, t(T, H, d), t(T, H, d), t(T, H, d), t(T, H, d), t(T, H, d), t(T, H, d), t(H), 1.0), (T, H, d)
+    if bad:
+        yield "norm", lambda r: te.LayerNorm(r, t(T, 9), eps=-1.0), (T, 9)
+        y = t(2, 9000)
+        yield "dweight", lambda r: te.LayerNormBackward(y, r, None, y, t(2, 9000), t(2), t(2)), (9000,)
+    else:
+        yield "norm", lambda r: te.LayerNorm(r, t(T, 9)), (T, 9)
+        yield "dweight", lambda r: te.LayerNormBackward(t(T, 9), r, None, t(T, 9), t(T, 9), t(T), t(T)), (9,)
+
+
+def test_engine_leaves_results_of_refused_calls_where_they_are():
+    te = ab.TensorEngine("Cuda")
+    for name, call, shape in engine_calls(te, True):
+        result = ab.Tensor(shape, hdata=np.full(shape, 5.0))
+        with pytest.raises(ab.AcroError):
+            call(result)
+        assert not result.IsOnGPU(), name
+        result.MoveFromGPU()
+        assert (result.numpy() == 5.0).all(), name
+    status_ok()
