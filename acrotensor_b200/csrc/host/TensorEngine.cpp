@@ -1,5 +1,6 @@
 // acro::TensorEngine: parse / bind / plan caches and single or recorded multi-kernel execution.
 #include "TensorEngine.hpp"
+#include "SliceTensor.hpp"
 #include "acro_b200.h"
 
 #include <cuda_runtime.h>
@@ -261,14 +262,18 @@ class StreamScratch
 };
 
 // Tensors that a call overwrites whole (null ones aside).  They stay on the side where they are until the call has been accepted, so that a refused
-// one leaves their values where the caller has them.
+// one leaves their values where the caller has them; a part of a larger tensor brings the rest of it along, which the call leaves as it is.
 class Results
 {
     public:
     Results(std::initializer_list<Tensor *> tensors) : Tensors(tensors)
     {
         for (Tensor *T : Tensors)
-            if (T != nullptr && !T->IsMappedToGPU()) T->MapToGPU();
+        {
+            if (T == nullptr || T->IsOnGPU()) continue;
+            if (dynamic_cast<SliceTensor *>(T) != nullptr) T->MoveToGPU();
+            else if (!T->IsMappedToGPU()) T->MapToGPU();
+        }
     }
     void Written()
     {

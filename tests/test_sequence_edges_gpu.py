@@ -101,3 +101,14 @@ def test_engine_leaves_results_of_refused_calls_where_they_are():
         result.MoveFromGPU()
         assert (result.numpy() == 5.0).all(), name
     status_ok()
+
+
+def test_engine_keeps_the_rest_of_a_tensor_whose_part_is_written():
+    te = ab.TensorEngine("Cuda")
+    for name, call, shape in engine_calls(te, False):
+        whole = ab.Tensor((3,) + shape, hdata=np.full((3,) + shape, 5.0))
+        call(ab.SliceTensor(whole, 1))
+        assert whole.IsOnGPU()
+        whole.MoveFromGPU()
+        assert (whole.numpy()[[0, 2]] == 5.0).all() and not (whole.numpy()[1] == 5.0).any(), name
+    status_ok()
