@@ -430,6 +430,7 @@ void TensorEngine::LinearAttentionBackward(Tensor &dQ, Tensor &dK, Tensor &dV, T
 void TensorEngine::LayerNorm(Tensor &Y, Tensor &X, Tensor *Weight, Tensor *Bias, double eps, Tensor *Mean, Tensor *Rstd)
 {
     ACROBATIC_ASSERT(X.IsInitialized() && X.GetRank() >= 1, "LayerNorm needs a tensor of at least one dim.");
+    ACROBATIC_ASSERT(X.GetRank() > 1 || !X.IsSharded(), "LayerNorm of a single row that is sharded over its entries.");
     const int width = X.GetDim(X.GetRank() - 1);
     const int64_t rows = X.GetSize64() / width;
     ACROBATIC_ASSERT(Y.IsInitialized() && Y.GetSize64() == X.GetSize64(), "Mismatched sizes of X and Y.");
@@ -450,6 +451,7 @@ void TensorEngine::LayerNorm(Tensor &Y, Tensor &X, Tensor *Weight, Tensor *Bias,
 void TensorEngine::LayerNormBackward(Tensor &dX, Tensor *dWeight, Tensor *dBias, Tensor &dY, Tensor &X, Tensor &Mean, Tensor &Rstd, Tensor *Weight)
 {
     ACROBATIC_ASSERT(X.IsInitialized() && X.GetRank() >= 1, "LayerNormBackward needs a tensor of at least one dim.");
+    ACROBATIC_ASSERT(X.GetRank() > 1 || !X.IsSharded(), "LayerNormBackward of a single row that is sharded over its entries.");
     const int width = X.GetDim(X.GetRank() - 1);
     const int64_t rows = X.GetSize64() / width;
     for (Tensor *T : {&dX, &dY}) ACROBATIC_ASSERT(T->IsInitialized() && T->GetSize64() == X.GetSize64(), "Mismatched sizes of X, dX and dY.");

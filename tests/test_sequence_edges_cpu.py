@@ -58,3 +58,13 @@ def test_overlap_of_packed_rows_and_of_a_step():
         arrays = [rows(i, (4 * D, 4 * D, D)) for i in range(3)] + [rows(3, strides)]
         assert lib().acro_b200_linear_attention_step(step, *arrays, 1 << 20, 1 << 21, 1 << 21, None, 3, None) == _lib.EINVAL
         assert word in lib().acro_b200_last_error()
+
+
+def test_engine_refuses_a_row_cut_over_the_ranks():
+    """A rank has a part of the row, and no mean or variance of it."""
+    te, stats = ab.TensorEngine("Cuda"), ab.Tensor(1)
+    x = ab.Tensor(8)
+    x.SetSharded(True)
+    for call in (lambda: te.LayerNorm(ab.Tensor(8), x), lambda: te.LayerNormBackward(ab.Tensor(8), None, None, ab.Tensor(8), x, stats, stats)):
+        with pytest.raises(ab.AcroError, match="sharded over its entries"):
+            call()
