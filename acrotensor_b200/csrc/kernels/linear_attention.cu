@@ -626,6 +626,15 @@ size_t shared_bytes(const acro_b200_linear_attention_desc &d, bool packed, int c
     return round256(static_cast<size_t>(rows) * d.q_heads * columns * statistic_bytes(d.type));
 }
 
+// Do two arrays of states share memory without being the same?  A sequence's state would be written while another one's is still read.
+bool states_cross(const acro_b200_linear_attention_desc &d, int64_t count, const void *x, const void *y)
+{
+    if (x == nullptr || y == nullptr || x == y) return false;
+    const __int128 bytes = static_cast<__int128>(count) * d.q_heads * d.dk * d.dv * static_cast<int64_t>(statistic_bytes(d.type));
+    const __int128 apart = static_cast<__int128>(reinterpret_cast<uintptr_t>(x)) - reinterpret_cast<uintptr_t>(y);
+    return apart < bytes && -apart < bytes;
+}
+
 TokenRows rows_from(const acro_b200_token_array &x, int group) { return {x.data, x.sequence_stride, x.token_stride, x.head_stride, group}; }
 
 // Does no row of an array share an entry with another?  Of heads, tokens and sequences the one of a larger stride has to stride over all of
@@ -814,6 +823,7 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
         fault = "log_decay, offsets, slots or a state is not aligned to its elements";
     if (fault.empty() && rows && (out->data == q->data || out->data == k->data || out->data == v->data))
         fault = "out takes the place of an operand that is still read";
+    if (fault.empty() && states_cross(d, state_count, initial_state, final_state)) fault = "final_state overlaps initial_state without being the same";
     if (fault.empty() && ((rows && !all_on_device({q->data, k->data, v->data, out->data})) ||
                           !all_on_device({log_decay, offsets, slots, initial_state, final_state, need > 0 ? scratch : nullptr})))
         fault = "an array, log_decay, offsets, slots, a state or scratch is not memory of the current device";
@@ -868,6 +878,7 @@ int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc,
     if (fault.empty() && (out->data == q->data || out->data == k->data || out->data == v->data))
         fault = "out takes the place of an operand that is still read";
     if (fault.empty() && (state_count < 0 || (slots == nullptr && state_count != d.sequences))) fault = "without slots there is one state per sequence";
+    if (fault.empty() && states_cross(d, state_count, state_in, state_out)) fault = "state_out overlaps state_in without being the same";
     if (fault.empty() && !all_on_device({q->data, k->data, v->data, out->data, log_decay, state_in, state_out, slots}))
         fault = "an array, log_decay, slots or a state is not memory of the current device";
     if (!fault.empty()) return fail_invalid(name + fault);
@@ -956,7 +967,9 @@ int acro_b200_linear_attention_backward(const acro_b200_linear_attention_desc *d
         fault = "scratch is smaller than acro_b200_linear_attention_backward_scratch_bytes or not 16-byte aligned";
     if (fault.empty() && (!aligned_to({log_decay, initial_state, d_final_state, d_initial_state}, statistic_bytes(d.type)) || !aligned_to({offsets}, 8)))
         fault = "log_decay, offsets or a state is not aligned to its elements";
-    if (fault.empty() && d_initial_state != nullptr && (d_initial_state == d_final_state || d_initial_state == initial_state))
+    if (fault.empty() && d_initial_state != nullptr &&
+        (d_initial_state == d_final_state || d_initial_state == initial_state || states_cross(d, d.sequences, d_initial_state, d_final_state) ||
+         states_cross(d, d.sequences, d_initial_state, initial_state)))
         fault = "d_initial_state takes the place of a state that is still read";
     if (fault.empty() && rows)
         for (const acro_b200_token_array *to : {dq, dk, dv})

@@ -434,6 +434,7 @@ typedef struct acro_b200_linear_attention_desc
  *                  to no sequence have no effect and are not written.  A sequence may be empty: its final state is its initial state.
  *                  A sequence that starts or ends at a number below zero, behind the rows or lower than one in front of it is skipped.
  *   initial_state  NULL (zero), or states [state_count][q_heads][dk][dv], contiguous; final_state NULL or the same, and may be the same memory
+ *                  (but not a part of it: such calls are refused)
  *   slots          NULL (state n belongs to sequence n, state_count = sequences), or the state of each sequence.  A negative slot marks
  *                  a sequence that is not there: its rows and states are left as they were.  Without states that is all the slots say,
  *                  and state_count is not looked at.
@@ -449,7 +450,7 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
                                const void *initial_state, void *final_state, const int32_t *slots, int64_t state_count, void *scratch, size_t scratch_bytes,
                                void *stream);
 /* One token of each of desc->sequences requests (desc->tokens = 1): state_out[slot] = lam state_in[slot] + k v^T,
- * out = scale q^T state_out[slot].  state_out may be state_in; out must not be q, k or v.  Request n is sequence n of the arrays. */
+ * out = scale q^T state_out[slot].  state_out may be state_in (but not overlap it otherwise); out must not be q, k or v.  Request n is sequence n of the arrays. */
 int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
                                     const acro_b200_token_array *v, const acro_b200_token_array *out, const void *log_decay, const void *state_in,
                                     void *state_out, const int32_t *slots, int64_t state_count, void *stream);

@@ -68,3 +68,24 @@ def test_engine_refuses_a_row_cut_over_the_ranks():
     for call in (lambda: te.LayerNorm(ab.Tensor(8), x), lambda: te.LayerNormBackward(ab.Tensor(8), None, None, ab.Tensor(8), x, stats, stats)):
         with pytest.raises(ab.AcroError, match="sharded over its entries"):
             call()
+
+
+STATE = 4 * D * D * 4       # bytes of one sequence's (request's) state
+
+
+@pytest.mark.parametrize("shift", [1, STATE // 4, 2 * STATE // 4 - 1])
+def test_states_that_overlap_without_being_the_same_are_refused(shift):
+    """Sequence 0 would write what sequence 1 starts from."""
+    plain = (12 * D, 4 * D, D)
+    at, log_decay = 1 << 30, 1 << 20
+    for other, word in ((at + 4 * shift, b"overlap"), (at - 4 * shift, b"overlap"), (at + 2 * STATE, b"not memory"), (at - 2 * STATE, b"not memory"),
+                        (at, b"not memory")):
+        assert lib().acro_b200_linear_attention(desc(), *[rows(i, plain) for i in range(4)], log_decay, None, at, other, None, 2, None, 0, None) == _lib.EINVAL
+        assert word in lib().acro_b200_last_error()
+        assert lib().acro_b200_linear_attention_step(desc(tokens=1), *[rows(i, plain) for i in range(4)], log_decay, at, other, None, 2, None) == _lib.EINVAL
+        assert word in lib().acro_b200_last_error()
+        for states in ((at, None, other), (None, at, other)):
+            initial, d_final, d_initial = states
+            assert lib().acro_b200_linear_attention_backward(desc(), *[rows(i, plain) for i in range(4)], log_decay, None, initial, d_final,
+                                                             *[rows(i, plain) for i in range(4, 7)], d_initial, None, 0, None) == _lib.EINVAL
+            assert (b"not memory" in lib().acro_b200_last_error()) == (abs(other - at) == 2 * STATE)
