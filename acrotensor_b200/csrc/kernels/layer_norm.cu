@@ -550,6 +550,7 @@ int acro_b200_layer_norm(int type, const void *x, int64_t x_stride, const void *
     if (x == nullptr || y == nullptr) return fail_invalid("acro_b200_layer_norm: null pointer");
     if (x_stride < width || y_stride < width) return fail_invalid("acro_b200_layer_norm: rows overlap (a row stride is smaller than the width)");
     if (x == y && x_stride != y_stride) return fail_invalid("acro_b200_layer_norm: in place, but with different row strides");
+    if (mean != nullptr && mean == rstd) return fail_invalid("acro_b200_layer_norm: mean and rstd take the same place");
     if (!aligned_to({x, weight, bias, y}, element_bytes(type)) || !aligned_to({mean, rstd}, statistic_bytes(type)))
         return fail_invalid("acro_b200_layer_norm: a pointer is not aligned to its elements");
     if (!all_on_device({x, weight, bias, y, mean, rstd})) return fail_invalid("acro_b200_layer_norm: a pointer is not memory of the current device");

@@ -89,3 +89,11 @@ def test_states_that_overlap_without_being_the_same_are_refused(shift):
             assert lib().acro_b200_linear_attention_backward(desc(), *[rows(i, plain) for i in range(4)], log_decay, None, initial, d_final,
                                                              *[rows(i, plain) for i in range(4, 7)], d_initial, None, 0, None) == _lib.EINVAL
             assert (b"not memory" in lib().acro_b200_last_error()) == (abs(other - at) == 2 * STATE)
+
+
+def test_statistics_in_one_place_are_refused():
+    at = [4096 * (i + 1) for i in range(5)]
+    call = lambda mean, rstd: lib().acro_b200_layer_norm(2, at[0], 8, at[1], at[2], at[3], 8, mean, rstd, 3, 8, 1e-5, None)
+    assert call(at[4], at[4]) == _lib.EINVAL and b"same place" in lib().acro_b200_last_error()
+    for mean, rstd in ((None, None), (at[4], None), (None, at[4]), (at[4], at[4] + 64)):
+        assert call(mean, rstd) == _lib.EINVAL and b"memory of the current device" in lib().acro_b200_last_error()
