@@ -70,8 +70,9 @@ __device__ __forceinline__ uint32_t take_odd(Two &x)
     return (first ? all & 0xffffu : 0u) | (second ? all & 0xffff0000u : 0u);
 }
 
+// Six CTAs an SM: with the 62 registers that fp32 takes otherwise, and four CTAs, 4 x 1024 rows of 12 heads of 64 took 27 us instead of 24.5.
 template <class T, int IN>
-__global__ void __launch_bounds__(256) attention_split_kernel(const __grid_constant__ SplitArgs a)
+__global__ void __launch_bounds__(256, 6) attention_split_kernel(const __grid_constant__ SplitArgs a)
 {
     const int array = blockIdx.y, columns = a.columns[array], heads = a.heads[array], quads = (columns + 7) / 8 * 2, each = heads * quads;
     const TokenRows &r = a.from[array];
@@ -116,9 +117,8 @@ __global__ void __launch_bounds__(256) attention_split_kernel(const __grid_const
                 y[1] = two(z[2], z[3]);
             }
             // infinities and NaN are the first part's alone; finite values have finite parts, above the largest bf16 too
-            uint2 odd = make_uint2(0, 0);
-            if (__builtin_expect(!(isfinite(first_of(y[0])) && isfinite(second_of(y[0])) && isfinite(first_of(y[1])) && isfinite(second_of(y[1]))), 0))
-                odd = make_uint2(take_odd(y[0]), take_odd(y[1]));
+            // (no branch: it would keep the next values' loads behind it)
+            const uint2 odd = make_uint2(take_odd(y[0]), take_odd(y[1]));
 #pragma unroll
             for (int k = 0; k < IN; ++k)
             {
