@@ -189,15 +189,62 @@ __device__ __forceinline__ int64_t highest_ahead(int64_t mine, int64_t &highest,
     return ahead;
 }
 
-// Rows of sequence base + threadIdx.x, or false.  `ascend`: all entries are good.  `highest`: the highest entry in front of base,
-// then that in front of base + blockDim.x.  Every thread calls it; holds CTA barriers unless `ascend`.
-__device__ __forceinline__ bool next_rows(const AttentionArgs &a, int64_t base, bool ascend, int64_t &highest, int64_t &begin, int64_t &end, int64_t (*sums)[2])
+// Rows of sequence base + threadIdx.x, or false.  `highest`: the highest entry in front of base, then that in front of base + blockDim.x.
+// Every thread calls it; holds CTA barriers.
+__device__ __forceinline__ bool next_rows(const AttentionArgs &a, int64_t base, int64_t &highest, int64_t &begin, int64_t &end, int64_t (*sums)[2])
 {
     const int64_t n = base + threadIdx.x;
     const bool there = n < a.sequences;
-    int64_t ahead = 0;
-    if (!ascend) ahead = highest_ahead(there ? a.offsets[n] : INT64_MIN, highest, sums);
+    const int64_t ahead = highest_ahead(there ? a.offsets[n] : INT64_MIN, highest, sums);
     return there && rows_of_sequence(a.offsets, n, a.tokens, ahead, begin, end);
+}
+
+// One block of sequences in the search for item `launched`: sets found (sequence, its rows, which of its segments) if it is among them.
+// `there`: thread's sequence n has the rows b .. e-1 (and is not skipped).  `before`: whole and last segments in front of the block, then
+// behind it; `whole`: whole segments of all sequences.  Every thread calls it; holds CTA barriers.
+__device__ __forceinline__ void find_in_block(const AttentionArgs &a, int64_t launched, int64_t n, bool there, int64_t b, int64_t e, int64_t whole,
+                                              int64_t &before_last, int64_t &before_whole, int64_t *found, int64_t (*sums)[2])
+{
+    int64_t mine_last = 0, mine_whole = 0;
+    if (there)
+    {
+        mine_whole = (e - b) / a.segment;
+        mine_last = segments_of(e - b, a.segment) - mine_whole;
+    }
+    int64_t start_last = mine_last, start_whole = mine_whole, total_last, total_whole;
+    scan_two(start_last, start_whole, total_last, total_whole, sums);
+    start_last += before_last;
+    start_whole += before_whole;
+    int64_t which = -1;
+    if (launched < whole && launched >= start_whole && launched < start_whole + mine_whole) which = launched - start_whole;
+    if (launched >= whole && mine_last > 0 && launched - whole == start_last) which = mine_whole;
+    if (which >= 0)
+    {
+        found[0] = n;
+        found[1] = b;
+        found[2] = e;
+        found[3] = which;
+    }
+    before_last += total_last;
+    before_whole += total_whole;
+}
+
+// The search among sequences of which some are skipped: their validity needs all entries in front of theirs.  A call of its own, so that the
+// kernels' first instructions stay few (inlined, it cost a cold launch 3 us).
+static __device__ __noinline__ void find_among_bad(const AttentionArgs &a, int64_t launched, int64_t *found, int64_t (*sums)[2])
+{
+    if (threadIdx.x == 0) atomicOr(a.bad_index, 1);
+    int64_t all = 0, none = 0, whole, nothing, b, e, highest = INT64_MIN;
+    for (int64_t base = 0; base < a.sequences; base += blockDim.x)
+        if (next_rows(a, base, highest, b, e, sums)) all += (e - b) / a.segment;
+    scan_two(all, none, whole, nothing, sums);
+    int64_t before_last = 0, before_whole = 0;
+    highest = INT64_MIN;
+    for (int64_t base = 0; base < a.sequences; base += blockDim.x)
+    {
+        const bool there = next_rows(a, base, highest, b, e, sums);
+        find_in_block(a, launched, base + threadIdx.x, there, b, e, whole, before_last, before_whole, found, sums);
+    }
 }
 
 // Item `launched` of the list of all sequences' segments.  Packed sequences put their whole segments in front and their (shorter) last
@@ -220,49 +267,30 @@ __device__ __forceinline__ SegmentItem find_item(const AttentionArgs &a, int64_t
         __shared__ int64_t found[4], sums[32][2];
         if (threadIdx.x == 0) found[0] = -1;
         // the number of whole segments of all sequences
-        int64_t all = 0, b, e, highest = INT64_MIN;
+        int64_t all = 0, b = 0, e = 0;
         bool bad = false;
         for (int64_t n = threadIdx.x; n < a.sequences; n += blockDim.x)
         {
             if (rows_of_sequence(a.offsets, n, a.tokens, 0, b, e)) all += (e - b) / a.segment;
             else bad = true;
         }
-        const bool ascend = __syncthreads_or(bad) == 0;
-        if (!ascend)
+        if (__syncthreads_or(bad) != 0) find_among_bad(a, launched, found, sums);
+        else
         {
-            if (threadIdx.x == 0) atomicOr(a.bad_index, 1);
-            all = 0;
+            int64_t none = 0, whole, nothing;
+            scan_two(all, none, whole, nothing, sums);
+            int64_t before_last = 0, before_whole = 0;
             for (int64_t base = 0; base < a.sequences; base += blockDim.x)
-                if (next_rows(a, base, false, highest, b, e, sums)) all += (e - b) / a.segment;
-        }
-        int64_t none = 0, whole, nothing;
-        scan_two(all, none, whole, nothing, sums);
-        int64_t before_last = 0, before_whole = 0;
-        highest = INT64_MIN;
-        for (int64_t base = 0; base < a.sequences; base += blockDim.x)
-        {
-            int64_t mine_last = 0, mine_whole = 0;
-            if (next_rows(a, base, ascend, highest, b, e, sums))
             {
-                mine_whole = (e - b) / a.segment;
-                mine_last = segments_of(e - b, a.segment) - mine_whole;
+                const int64_t n = base + threadIdx.x;
+                const bool there = n < a.sequences;
+                if (there)
+                {
+                    b = a.offsets[n];
+                    e = a.offsets[n + 1];
+                }
+                find_in_block(a, launched, n, there, b, e, whole, before_last, before_whole, found, sums);
             }
-            int64_t start_last = mine_last, start_whole = mine_whole, total_last, total_whole;
-            scan_two(start_last, start_whole, total_last, total_whole, sums);
-            start_last += before_last;
-            start_whole += before_whole;
-            int64_t which = -1;
-            if (launched < whole && launched >= start_whole && launched < start_whole + mine_whole) which = launched - start_whole;
-            if (launched >= whole && mine_last > 0 && launched - whole == start_last) which = mine_whole;
-            if (which >= 0)
-            {
-                found[0] = base + threadIdx.x;
-                found[1] = b;
-                found[2] = e;
-                found[3] = which;
-            }
-            before_last += total_last;
-            before_whole += total_whole;
         }
         __syncthreads();
         s.sequence = found[0];
