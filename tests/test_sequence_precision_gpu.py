@@ -75,15 +75,21 @@ def test_scores_enter_their_product_whole(kind, d):
     near(kind, dv[0, :-1, 0].double(), 2.0 ** -17)
 
 
+@pytest.mark.parametrize("kind", ["f16", "f32"])
 @pytest.mark.parametrize("d", [64, 128])
-def test_half_precision_is_multiplied_whole(d):
-    """Of 11 bits: the square of 1 + 3 2^-10 less its first two terms."""
-    q, k, v = zeros("f16", 1, d), zeros("f16", 1, d), zeros("f16", 1, d)
-    q[..., :3] = torch.tensor([1 + 3 * 2.0 ** -10, 1, 1])
-    k[0, 0, 0, 0] = 1 + 3 * 2.0 ** -10
-    k[0, 1, 0, 1:3] = torch.tensor([1, 6 * 2.0 ** -10])
+def test_second_parts_are_multiplied_with_each_other(kind, d):
+    """The square of 1 + 3 2^-10 less its first two terms: queries by keys, and scores (and keys) by values."""
+    x, y = 1 + 3 * 2.0 ** -10, 6 * 2.0 ** -10
+    q, k, v = zeros(kind, 1, d), zeros(kind, 1, d), zeros(kind, 1, d)
+    q[..., :3] = torch.tensor([x, 1, 1])
+    k[0, 0, 0, 0] = x
+    k[0, 1, 0, 1:3] = torch.tensor([1, y])
     v[0, 0], v[0, 1] = 1, -1
-    near("f16", forward("f16", q, k, v)[1:, 0], 9 * 2.0 ** -20)
+    near(kind, forward(kind, q, k, v)[1:, 0], 9 * 2.0 ** -20)
+    q[..., :3] = torch.tensor([1.0, 1, 0])
+    k[0, :2, 0, :3] = torch.tensor([[x, 0, 0], [0, 1, 0]])
+    v[0, 0], v[0, 1] = x, -(1 + y)
+    near(kind, forward(kind, q, k, v)[1:, 0], 9 * 2.0 ** -20)
 
 
 @pytest.mark.parametrize("of", ["q", "k", "v"])
