@@ -1,5 +1,5 @@
 // Linear attention with a decay for each head: entry points, the kernels for every type and head size, the step for single
-// tokens.  linear_attention.cuh has the mathematics; linear_attention_mma.cu the main pass on the tensor cores.
+// tokens.  linear_attention.cuh has the mathematics; linear_attention_mma.cuh the main pass on the tensor cores.
 #include "linear_attention.cuh"
 
 #include <algorithm>
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads) attention_pass_kernel(const __grid_c
 }
 
 // Turns the segments' own states into the states that they start from: one thread per entry of a state, walking a sequence's
-// segments in the order of time, 16 loads ahead.  Bound by the latency of offsets, powers and loads: 19 us with cold caches for 12 segments
+// segments in the order of time, 16 loads ahead.  Bound by the latency of offsets, powers and loads: 20 us with cold caches for 12 segments
 // of 16 heads of 128 x 128 (25 MB).  Taking the powers behind the first loads did not shorten it; with the power taken in every step and
 // one load at a time 144 segments took 89 us.
 template <class A>
@@ -571,8 +571,8 @@ std::string head_fault(const acro_b200_linear_attention_desc *d, bool packed)
 // walk over k and v (0.4 of the main pass on the tensor cores, 0.6 on the other path) and the join (as long as 6 chunks of 64 tokens): the cheapest number
 // is taken, for the CTAs that an SM holds (tensor-core pass: 1; the other: 2 at least).  Packed sequences are treated as one axis of all
 // their rows, since their lengths are not known here; segments of three quarters of that length cost the same over 15 packed shapes, half
-// the length 14 % more.  On the tensor cores a segment has 256 tokens at least: 13 shapes took 101 us on average with 512, 87 with 256 (4 x 1024
-// tokens of 12 heads in fp32 96 and 81 us), 86 with 128 but one of them 14 % more than before.
+// the length 14 % more.  On the tensor cores a segment has 256 tokens at least: 13 shapes took 108 us on average with 512, 93 with 256 (4 x 1024
+// tokens of 12 heads in fp32 101 and 88 us), 91 with 128, but a gradient of packed sequences 12 % more than with 256.
 int64_t segment_tokens(const acro_b200_linear_attention_desc &d, bool packed, bool tensor_cores, int passes)
 {
     const int64_t slots = (sm_count() > 0 ? sm_count() : 148) * (tensor_cores ? 1 : 2);

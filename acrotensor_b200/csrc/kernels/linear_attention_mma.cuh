@@ -12,14 +12,14 @@
 // Precision: accumulators and the state are fp32; every operand is a sum of bf16 parts (8 bits each).  Inputs: IN parts, 1 for bf16, 2 for
 // fp16 (exact) and 3 for fp32 (2^-26).  P~, S and K~: 3 parts whatever the inputs, so that scores and states have on their way into a product
 // the bits that they have in fp32 (with two parts of P~ and S, 2^-18, a few bf16 results in ten thousand were rounded the other way; a chunk of
-// 128 columns took 2.75 us where it takes 3.08 with three, of 64 columns 1.71 and 2.09).  Of the products of parts those are left out that lie
+// 128 columns took 2.75 us where it takes 3.07 with three, of 64 columns 1.71 and 2.06).  Of the products of parts those are left out that lie
 // below 2^-24 of the whole.  The small ones are multiplied first: the tensor cores' additions lose up to a step of the sum so far, so fewer
 // of them happen at its full size; and no sum of theirs spans more
 // than a chunk (spanning a segment of 58 cost the final state a digit).
 //
 // Bound, for bf16 and 128 columns: by HBM 64 KB a chunk, about 2850 cycles of an SM at its share of 6.5 TB/s.  Shared memory comes first:
 // the products' operands take about 2370 cycles of it (48 cycles for 64 columns with both operands there, measured alone), copies, K~, P~ and
-// stores 2170, of the 5500 cycles (3.08 us) that a chunk takes with all SMs at work.  64 columns: 2.09 us a chunk.  The roles overlap: one
+// stores 2170, of the 5500 cycles (3.07 us) that a chunk takes with all SMs at work.  64 columns: 2.06 us a chunk.  The roles overlap: one
 // warp issues copies and products, eight convert operands, sixteen keep the state and write; waiting warps sleep on barriers, one arrival
 // a warp; loops are short (the instruction cache held the first versions back).
 #ifndef ACRO_B200_KERNELS_LINEAR_ATTENTION_MMA_CUH
