@@ -440,9 +440,9 @@ typedef struct acro_b200_linear_attention_desc
  *                  and state_count is not looked at.
  *   scratch        acro_b200_linear_attention_scratch_bytes(desc, packed) bytes (0 is possible), 16-byte aligned; calls that share
  *                  it must not overlap on the device.
- * out must not be q, k or v.  No host synchronisation.  An infinity or NaN of a token reaches only the rows that see it by the
- * formula; an infinity of v may become a NaN there, in its column, and one of q or k in 32 and 16 bits a NaN in the rows and the state
- * that it meets.  Same bits on every run on one device.
+ * out must not be q, k or v.  No host synchronisation.  An infinity or NaN of a token or a state reaches only the rows and
+ * states that see it by the formula; an infinity may become a NaN there (one of v in its column alone).  Same bits on every run on one
+ * device.
  */
 size_t acro_b200_linear_attention_scratch_bytes(const acro_b200_linear_attention_desc *desc, int packed);
 int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
@@ -450,7 +450,8 @@ int acro_b200_linear_attention(const acro_b200_linear_attention_desc *desc, cons
                                const void *initial_state, void *final_state, const int32_t *slots, int64_t state_count, void *scratch, size_t scratch_bytes,
                                void *stream);
 /* One token of each of desc->sequences requests (desc->tokens = 1): state_out[slot] = lam state_in[slot] + k v^T,
- * out = scale q^T state_out[slot].  state_out may be state_in (but not overlap it otherwise); out must not be q, k or v.  Request n is sequence n of the arrays. */
+ * out = scale q^T state_out[slot].  state_out may be state_in (but not overlap it otherwise); out must not be q, k or v.  Request n is
+ * sequence n of the arrays. */
 int acro_b200_linear_attention_step(const acro_b200_linear_attention_desc *desc, const acro_b200_token_array *q, const acro_b200_token_array *k,
                                     const acro_b200_token_array *v, const acro_b200_token_array *out, const void *log_decay, const void *state_in,
                                     void *state_out, const int32_t *slots, int64_t state_count, void *stream);
